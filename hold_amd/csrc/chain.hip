@@ -288,8 +288,7 @@ constexpr int X6_UNITS = 3 * 512;  // 16-byte units per 16-wide k step
 
 struct Limbs3 { bf16x8 l[3]; };
 
-// Two values at a time: the compiler selects v_pk_add_f32 for the two remainders, so 8 values cost 16 v_and + 8 v_pk_add
-// + 12 v_perm = 36 VALU issue slots (44 with scalar subtractions).  Measured neutral: neither this nor halving the number
+// Two values at a time: 8 values cost 16 v_and + 16 v_sub + 12 v_perm = 44 VALU issue slots.  Their number was measured neutral: neither this nor halving the number
 // of splits (a four-wave variant, 64 features per wave) moved the kernel -- it is not VALU-issue-bound.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));

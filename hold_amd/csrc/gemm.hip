@@ -54,7 +54,7 @@ __device__ __forceinline__ Limbs3 split8s_trunc(const float (&x)[8]) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   u32x4 p1, p2, p3;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {  // two values at a time: v_pk_add_f32 for the remainders (36 VALU slots per 8 values)
+  for (int j = 0; j < 4; ++j) {  // two values at a time (44 VALU slots per 8 values)
     const f32x2 v = {x[2 * j], x[2 * j + 1]};
     const u32x2 xb = __builtin_bit_cast(u32x2, v);
     const f32x2 r1 = v - __builtin_bit_cast(f32x2, xb & 0xffff0000u);

@@ -163,7 +163,7 @@ __device__ __forceinline__ float knn_d2(float px, float py, float pz, float vx, 
   return __fmaf_rn(dz, dz, __fmaf_rn(dy, dy, dx * dx));
 }
 
-// two vertices at once on the packed fp32 instructions (v_pk_add / v_pk_mul / v_pk_fma): per element the operations and
+// two vertices at once: per element the operations and
 // their order are knn_d2's, so the bits are the same
 typedef float knn_f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ knn_f2 knn_d2x2(knn_f2 px, knn_f2 py, knn_f2 pz, knn_f2 vx, knn_f2 vy, knn_f2 vz) {

@@ -156,11 +156,14 @@ __device__ __forceinline__ void dma_pair(const char* src, uint32_t lane16, uint3
 // transcendentals as opaque volatile instructions: they stay where the schedule puts them without a pin behind them (an
 // empty asm right behind a builtin v_exp / v_log made the hazard recogniser pad a wait state -- 9 s_nop per k step); their
 // consumers are LAT_TRANS instruction slots away by construction of the schedule (tests/test_r6_pack_cpu.py checks the table)
-// packed fp32 arithmetic (two values per instruction) as volatile instructions as well: written as <2 x float> C
-// arithmetic the instruction selector scalarises most of it again (operands assembled from separately computed halves)
-__device__ __forceinline__ f32x2 pk_mul(f32x2 a, f32x2 b) { f32x2 r; asm volatile("v_pk_mul_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
-__device__ __forceinline__ f32x2 pk_add(f32x2 a, f32x2 b) { f32x2 r; asm volatile("v_pk_add_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
-__device__ __forceinline__ f32x2 pk_fma(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm volatile("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c)); return r; }
+// arithmetic on value PAIRS, two volatile scalar instructions each: the packed fp32 instructions (v_pk_*_f32) would halve the
+// issue slots, but some of their forms have given wrong results on this machine now and then, so the library is built without them
+__device__ __forceinline__ float mul_v(float a, float b) { float r; asm volatile("v_mul_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
+__device__ __forceinline__ float add_v(float a, float b) { float r; asm volatile("v_add_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
+__device__ __forceinline__ float fma_v(float a, float b, float c) { float r; asm volatile("v_fma_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c)); return r; }
+__device__ __forceinline__ f32x2 pair_mul(f32x2 a, f32x2 b) { return f32x2{mul_v(a[0], b[0]), mul_v(a[1], b[1])}; }
+__device__ __forceinline__ f32x2 pair_add(f32x2 a, f32x2 b) { return f32x2{add_v(a[0], b[0]), add_v(a[1], b[1])}; }
+__device__ __forceinline__ f32x2 pair_fma(f32x2 a, f32x2 b, f32x2 c) { return f32x2{fma_v(a[0], b[0], c[0]), fma_v(a[1], b[1], c[1])}; }
 __device__ __forceinline__ float exp2_v(float x) { float r; asm volatile("v_exp_f32 %0, %1" : "=v"(r) : "v"(x)); return r; }
 __device__ __forceinline__ float log2_v(float x) { float r; asm volatile("v_log_f32 %0, %1" : "=v"(r) : "v"(x)); return r; }
 
@@ -417,9 +420,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     f32x4 rb[4] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
     // Epilogue of k step j = (nt, q) of the finished layer: its 8 values P[nt][8 q + i] (features 32 nt + 16 q + 8 (i / 4) +
     // 4 hh + i % 4) as a flat list of micro-operations, ROUND-MAJOR: a round works on the 8 values (one instruction each) or, where
-    // a packed fp32 instruction exists, on the 4 value PAIRS (2 i, 2 i + 1) -- consecutive micro-operations are independent.
-    //   sampler query: y (8), ys = c3 y (4, v_pk_mul_f32), KE |ys| (8), exp2 (8), 1 + e (4, v_pk_add_f32), log2 (8),
-    //                  max(ys, 0) (8), CL log2 + max (4, v_pk_fma_f32) [skip override]                         = 52
+    // the operation is plain arithmetic, on the 4 value PAIRS (2 i, 2 i + 1) -- consecutive micro-operations are independent.
+    //   sampler query: y (8), ys = c3 y (4 pairs), KE |ys| (8), exp2 (8), 1 + e (4 pairs), log2 (8),
+    //                  max(ys, 0) (8), CL log2 + max (4 pairs) [skip override]                         = 52
     //   training:      y (8), ys (4), KE |ys| (8), exp2 (8), 1 + e (4), series (4 + 4 + 4 + 4), log2 (8), CL log2 (4), select (8),
     //                  max (8), + (4), [skip override] (8; the reference's `y > 0.2 -> y` branch needs no instruction: softplus(y) - y
     //                  <= 2.1e-11 there, far below half an ulp of y, so the sum IS y), 1 / SA = the stored value (4)   = 92
@@ -430,8 +433,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     static_assert(NOPS == SchedEpi<HEAD>::N, "regenerate rmlp_h3_sched.h");
 #define H3_PIN(x) asm volatile("" : "+v"(x))
 #define H3_PINP(x)  // (no pin behind a transcendental: see exp2_v)
-    // constants of the packed instructions as OPAQUE register pairs: with an inline constant or an SGPR operand the
-    // instruction selector scalarises a <2 x float> operation into two v_*_f32 (packed fp32 takes no literal per half)
+    // constants of the pair operations in vector registers (their instructions take "v" operands)
     f32x2 ONE2 = {1.0f, 1.0f}, CL2 = {CL, CL};
     H3_PIN(ONE2);
     H3_PIN(CL2);
@@ -463,13 +465,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         if (STORE && (j & 1) == 0 && k >= 2 && k < 6)  // ... which completed a tile: read it back (pieces 0..3)
           rb[k - 2] = *reinterpret_cast<const f32x4*>(rt_lane_r + (k - 2) * 1024);
         if (rd == 0) { st.y[p][c] = P[nt][8 * q + i]; H3_PIN(st.y[p]); }
-        else if (rd == 1) { st.y[i] = pk_mul(st.y[i], c3); }
+        else if (rd == 1) { st.y[i] = pair_mul(st.y[i], c3); }
         else if (rd == 2) { st.e[p][c] = KE * fabsf(st.y[p][c]); H3_PIN(st.e[p]); }
         else if (rd == 3) {
           if (ABL & 1) { float t = st.e[p][c] * 1e-3f; H3_PIN(t); st.e[p][c] = t; }
           else { st.e[p][c] = exp2_v(st.e[p][c]); H3_PINP(st.e[p]); }
         }
-        else if (rd == 4) { st.u[i] = pk_add(st.e[i], ONE2); }
+        else if (rd == 4) { st.u[i] = pair_add(st.e[i], ONE2); }
         else if (HEAD) {
           if (rd == 5) {
             if (ABL & 2) { float t = st.u[p][c] * 0.5f; H3_PIN(t); st.u[p][c] = t; }
@@ -477,22 +479,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
           }
           else if (rd == 6) { st.r[p][c] = relu1(st.y[p][c]); H3_PIN(st.r[p]); }
           else {
-            f32x2 r = pk_fma(st.u[i], CL2, st.r[i]);
+            f32x2 r = pair_fma(st.u[i], CL2, st.r[i]);
             if (j >= 13) { r[0] = skip(r[0], 2 * i); r[1] = skip(r[1], 2 * i + 1); H3_PIN(r); }
             st.r[i] = r;
           }
         } else {
-          if (rd == 5) { st.ser[i] = pk_fma(st.e[i], THIRD2, MHALF2); }
-          else if (rd == 6) { st.ser[i] = pk_fma(st.e[i], st.ser[i], ONE2); }
-          else if (rd == 7) { st.e[i] = pk_mul(st.e[i], E001_2); }
-          else if (rd == 8) { st.ser[i] = pk_mul(st.e[i], st.ser[i]); }
+          if (rd == 5) { st.ser[i] = pair_fma(st.e[i], THIRD2, MHALF2); }
+          else if (rd == 6) { st.ser[i] = pair_fma(st.e[i], st.ser[i], ONE2); }
+          else if (rd == 7) { st.e[i] = pair_mul(st.e[i], E001_2); }
+          else if (rd == 8) { st.ser[i] = pair_mul(st.e[i], st.ser[i]); }
           else if (rd == 9) { st.u[p][c] = log2_v(st.u[p][c]); H3_PINP(st.u[p]); }
-          else if (rd == 10) { st.u[i] = pk_mul(st.u[i], CL2); }
+          else if (rd == 10) { st.u[i] = pair_mul(st.u[i], CL2); }
           else if (rd == 11) { st.u[p][c] = (st.e[p][c] > 1e-5f * SA) ? st.u[p][c] : st.ser[p][c]; H3_PIN(st.u[p]); }  // e > 1e-3: log(1 + e) accurate
           else if (rd == 12) { st.r[p][c] = relu1(st.y[p][c]); H3_PIN(st.r[p]); }
-          else if (rd == 13) { st.r[i] = pk_add(st.r[i], st.u[i]); }
+          else if (rd == 13) { st.r[i] = pair_add(st.r[i], st.u[i]); }
           else if (rd == 14) { if (j >= 13) { st.r[p][c] = skip(st.r[p][c], i); H3_PIN(st.r[p]); } }
-          else { st.o[i] = pk_mul(st.r[i], ISA2); }
+          else { st.o[i] = pair_mul(st.r[i], ISA2); }
         }
       } else if (k < NSP + 16) {
         const int s = k - NSP, op = s >> 2, d = s & 3;

@@ -260,7 +260,7 @@ __device__ __forceinline__ void wgrad_r6_body(const float* R, int ldr, const flo
 // =====================================================================================================================
 // The same weight gradient in the TWO-LIMB fp16 arithmetic "f16x3" (see csrc/rmlp_h3.hip): both operands, scaled by a power
 // of two, as hi = RN_f16(s x), lo = RN_f16(s x - hi); hi hi + hi lo + lo hi on v_mfma_f32_32x32x16_f16 -- 48 MFMAs per
-// 16-point step instead of 96, a limb split of 5 instructions per two values (v_pk_mul_f32 by the scale, v_cvt_pk_f16_f32,
+// 16-point step instead of 96, a limb split of 6 instructions per two values (2 x v_mul_f32 by the scale, v_cvt_pk_f16_f32,
 // 2 x v_fma_mix_f32, v_cvt_pk_f16_f32) instead of 9 + 2 pins, and the fragment's 8 rows read as 4 ds_read2st64_b32.
 // SCALES.  The operands are activations (O(1)) and loss cotangents (1e-9 .. 1e-3 and anything else): every WORKGROUP picks
 // its own pair of scales from a sample of ITS rows (16 groups of four rows, evenly spread; all 256 -- for R: the first n_valid -- columns)
