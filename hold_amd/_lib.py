@@ -104,6 +104,14 @@ class ManoModel(C.Structure):
                                           "lbs_weights", "pose_mean", "tfs_c_inv")]
 
 
+class GatedDesc(C.Structure):  # hold_gated_desc
+    _fields_ = [("x", C.c_void_p), ("ldx", C.c_int64), ("w_gate", C.c_void_p), ("ldwg", C.c_int64), ("w_up", C.c_void_p),
+                ("ldwu", C.c_int64), ("b_gate", C.c_void_p), ("b_up", C.c_void_p), ("h", C.c_void_p), ("ldh", C.c_int64),
+                ("dh", C.c_void_p), ("lddh", C.c_int64), ("dx", C.c_void_p), ("dw_gate", C.c_void_p), ("dw_up", C.c_void_p),
+                ("db_gate", C.c_void_p), ("db_up", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+                ("T", C.c_int64), ("D", C.c_int32), ("H", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32)]
+
+
 _P, _I, _L, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 # developer-build-only symbols (HOLD_DEV=1 at build time): declared when present
 DEV_SIGNATURES = {
@@ -185,6 +193,9 @@ SIGNATURES = {
     "hold_trunk_h3": [_P, _I, _L, _P, _P, _P, _P, C.POINTER(C.c_void_p), _I, _P, _P, _P, _P],
     "hold_fused_sdf_r6_if": [_P, _I, _L, _P, _P, _P, _P, _P, _P, _I, _P, _P],
     "hold_trunk_r6_if": [_P, _I, _L, _P, _P, _P, C.POINTER(C.c_void_p), _I, _P, _P],
+    "hold_gated_workspace": [C.POINTER(GatedDesc), _I, C.POINTER(_L)],  # host only: no stream
+    "hold_gated_fwd": [C.POINTER(GatedDesc), _P],
+    "hold_gated_bwd": [C.POINTER(GatedDesc), _P],
     "hold_mano_lbs_fwd": [C.POINTER(ManoModel), _I, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "hold_mano_lbs_bwd": [C.POINTER(ManoModel), _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
 }

@@ -1,0 +1,266 @@
+// Tiled products on the 16-bit matrix cores, the core of gated.hip and muon.hip:   acc[i][j] += sum_k A(i, k) B(j, k).
+//
+// ARITHMETIC.  MODE_BF16: bf16 operands, v_mfma_f32_16x16x32_bf16.  MODE_F16X3: fp32 operands as two fp16 limbs, x 2^e = hi + lo
+// with hi = RN_f16(x 2^e), lo = RN_f16(x 2^e - hi) and the three limb products hi hi + hi lo + lo hi on v_mfma_f32_16x16x32_f16: the
+// dropped lo lo and the second rounding are <= 2^-22 of a product each (fp32's own rounding: 2^-24), accumulation is fp32 in both.
+//
+// OPERANDS.  Each of the two may lie in memory with k contiguous (KC: [row][k]) or with the rows contiguous (KS: [k][row]): no
+// transposed copy is ever made.  KC fragments are ds_read_b128; KS fragments are a pair of ds_read_b64_tr_b16, each of which hands
+// lane c of a 16-lane group column c of the 4 x 16 block that the group's lanes address.  Both come from LDS tiles that
+// buffer_load_dwordx4 ... lds fills directly; the 16-byte chunks of a tile row are permuted (on the global side, since the LDS side is
+// linear) so that the 16 rows that a fragment touches spread over all 64 banks.
+//
+// EDGES.  The buffer descriptor ends at the operand's last element, so rows behind it and k behind K arrive as zeros; a k tail inside
+// a KC row is masked per 16-byte chunk.  Required, and ensured by the callers' checks or padded copies: 16-byte aligned bases, leading
+// dimensions in multiples of 8 elements, K (KC) resp. row count (KS) rounded up to 8 inside the allocation.
+//
+// PIPELINE.  Two LDS stages: the loads of step k + 1 are in flight while step k is multiplied; one s_waitcnt + s_barrier per step.
+#ifndef HOLD_TILE16_H
+#define HOLD_TILE16_H
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace t16 {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+
+enum { MODE_BF16 = 0, MODE_F16X3 = 1 };
+enum { KC = 0, KS = 1 };
+constexpr uint32_t OOB = 0xC0000000u;  // a byte offset behind every descriptor's end
+
+template <int MODE> constexpr int limbs() { return MODE == MODE_BF16 ? 1 : 2; }
+template <int MODE> constexpr int step_k() { return MODE == MODE_BF16 ? 64 : 32; }
+
+// one operand of a tile: `p` points at the tile's first row and k = 0 (KC: row-major rows; KS: its first column at k = 0)
+struct Operand {
+  const uint16_t* p;
+  int64_t limb;  // elements from the hi array to the lo array (MODE_F16X3)
+  int64_t ld;
+  int64_t rows;  // rows of the operand from the tile's first one on (KS: columns, rounded up to 8)
+  int64_t k;     // k's of the operand (KC: rounded up to 8, the last ones zeros); the shorter of the two ends in zeros
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t bytes) {
+  const int64_t n = bytes < 0 ? 0 : (bytes > 0x7ffffff0ll ? 0x7ffffff0ll : bytes);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)n, 0x00020000);
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// LDS tile of R rows x BK k's of one limb
+template <int LAY, int R, int BK>
+struct Tile {
+  static constexpr int RB = (LAY == KC ? BK : R) * 2;   // bytes of a tile row
+  static constexpr int NR = LAY == KC ? R : BK;         // tile rows
+  static constexpr int C = RB / 16;                     // 16-byte chunks of a tile row
+  static constexpr int BYTES = RB * NR;
+  static constexpr int PIECES = BYTES / 1024;           // wave-wide 16-byte loads
+  static_assert(C >= 4 && BYTES % 1024 == 0, "tile row of at least 64 bytes");
+  static __device__ __forceinline__ int swz(int row) {
+    if (LAY == KC) return C >= 16 ? (row & 15) : C == 8 ? ((row >> 1) & 7) : ((row >> 2) & 3);
+    return C >= 16 ? 2 * ((row & 3) | ((row >> 1) & 4)) : 2 * (((row >> 1) & 1) | ((row >> 2) & 2));
+  }
+};
+
+// loads of one operand's tile; `first` = index of the wave's first piece, `stride` = waves
+template <int LAY, int R, int BK, int NW>
+struct Loader {
+  using T = Tile<LAY, R, BK>;
+  static constexpr int N = (T::PIECES + NW - 1) / NW;
+  static_assert(T::PIECES % NW == 0 || T::PIECES < NW, "whole rounds of pieces");
+  uint32_t off[N];
+  int kk[N];  // first k of the lane's chunk inside the step (KC)
+
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int q = (wave + i * NW) * 64 + lane, row = q / T::C, chunk = (q % T::C) ^ T::swz(row);
+      off[i] = (uint32_t)(row * (int)ld * 2 + chunk * 16);
+      kk[i] = chunk * 8;
+    }
+  }
+  // k0: first k of the step; lds: the tile's place in LDS
+  __device__ __forceinline__ void load(const Operand& o, int limb, int64_t k0, char* lds, int wave) const {
+    const uint16_t* p = o.p + limb * o.limb;
+    const int64_t left = o.k - k0;
+    const int kend = left < BK ? (int)left : BK;
+    __amdgpu_buffer_rsrc_t rs;
+    if (LAY == KC) {
+      const int64_t n = o.rows < R ? o.rows : R;
+      rs = rsrc(p + k0, n > 0 && left > 0 ? ((n - 1) * o.ld + left) * 2 : 0);
+    } else {
+      const int64_t n = kend;
+      rs = rsrc(p + k0 * o.ld, n > 0 && o.rows > 0 ? ((n - 1) * o.ld + (o.rows < R ? o.rows : R)) * 2 : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (T::PIECES < NW && wave >= T::PIECES) break;
+      const uint32_t v = (LAY == KC && kk[i] >= kend) ? OOB : off[i];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + (wave + i * NW) * 1024), 16, v, 0, 0, 0);
+    }
+  }
+};
+
+// the wave's fragments: 16 rows x 32 k's, lane l: row l % 16, k = 8 (l / 16) + 0..7
+template <int LAY, int R, int BK>
+struct Reader {
+  using T = Tile<LAY, R, BK>;
+  int base[LAY == KC ? BK / 32 : 1];
+  int s;
+  __device__ __forceinline__ void init(int lane) {
+    if (LAY == KC) {
+      const int row = lane & 15;
+#pragma unroll
+      for (int ks = 0; ks < (LAY == KC ? BK / 32 : 1); ++ks) base[ks] = row * T::RB + (((ks * 4 + (lane >> 4)) ^ T::swz(row)) * 16);
+      s = 0;
+    } else {
+      const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
+      base[0] = k * T::RB + ((lane & 3) >> 1) * 16 + (lane & 1) * 8;
+      s = T::swz(k) * 16;
+    }
+  }
+  __device__ __forceinline__ s16x8 frag(const char* lds, int row0, int ks) const {
+    if (LAY == KC) return *(const s16x8*)(lds + base[ks] + row0 * T::RB);
+    const char* a = lds + base[0] + ((row0 * 2) ^ s) + ks * 32 * T::RB;
+    const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)a);
+    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(a + 4 * T::RB));
+    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+template <int MODE>
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
+  if (MODE == MODE_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// A block of WM x WN waves computes a BM x BN tile for each of NB operands B that share A.  The matrix instruction's first operand
+// is B: a lane then holds FOUR CONSECUTIVE j of ONE row i, so results leave as 8- or 16-byte stores:
+//   acc[b][mi][ni][r]:  i = wm BM / WM + 16 mi + lane % 16,   j = wn BN / WN + 16 ni + 4 (lane / 16) + r
+template <int MODE, int LA, int LB, int BM, int BN, int NB, int WM, int WN>
+struct Core {
+  static constexpr int BK = step_k<MODE>(), NL = limbs<MODE>(), NW = WM * WN;
+  static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
+  using TA = Tile<LA, BM, BK>;
+  using TB = Tile<LB, BN, BK>;
+  static constexpr int STAGE = NL * (TA::BYTES + NB * TB::BYTES), LDS = 2 * STAGE;
+  static constexpr int THREADS = 64 * NW;
+  typedef f32x4 Acc[NB][MI][NI];
+
+  static __device__ __forceinline__ void zero(Acc& acc) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[b][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // A.k > 0.  Ends with every wave past its last read of the LDS stages.
+  static __device__ __forceinline__ void run(char* smem, const Operand& A, const Operand (&B)[NB], Acc& acc) {
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    Loader<LA, BM, BK, NW> la;
+    Loader<LB, BN, BK, NW> lb[NB];
+    la.init(wave, lane, A.ld);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) lb[b].init(wave, lane, B[b].ld);
+    Reader<LA, BM, BK> ra;
+    Reader<LB, BN, BK> rb;
+    ra.init(lane);
+    rb.init(lane);
+    const int nk = (int)((A.k + BK - 1) / BK);
+    auto stage = [&](int kt, char* s) {
+#pragma unroll
+      for (int l = 0; l < NL; ++l) {
+        la.load(A, l, (int64_t)kt * BK, s + l * TA::BYTES, wave);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) lb[b].load(B[b], l, (int64_t)kt * BK, s + NL * TA::BYTES + (b * NL + l) * TB::BYTES, wave);
+      }
+    };
+    stage(0, smem);
+    for (int kt = 0; kt < nk; ++kt) {
+      const char* s = smem + (kt & 1) * STAGE;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (kt + 1 < nk) stage(kt + 1, smem + ((kt + 1) & 1) * STAGE);
+      const char* sa = s;
+      const char* sb = s + NL * TA::BYTES;
+#pragma unroll
+      for (int ks = 0; ks < BK / 32; ++ks) {
+        s16x8 fb[NB][NI][NL];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int l = 0; l < NL; ++l) fb[b][j][l] = rb.frag(sb + (b * NL + l) * TB::BYTES, wn * (BN / WN) + 16 * j, ks);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+          s16x8 fa[NL];
+#pragma unroll
+          for (int l = 0; l < NL; ++l) fa[l] = ra.frag(sa + l * TA::BYTES, wm * (BM / WM) + 16 * i, ks);
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+              if (NL == 2) {  // the small products first: they meet the smaller partial sum
+                acc[b][i][j] = mfma<MODE>(fb[b][j][NL - 1], fa[0], acc[b][i][j]);
+                acc[b][i][j] = mfma<MODE>(fb[b][j][0], fa[NL - 1], acc[b][i][j]);
+              }
+              acc[b][i][j] = mfma<MODE>(fb[b][j][0], fa[0], acc[b][i][j]);
+            }
+        }
+      }
+    }
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+};
+
+// Block -> tile.  Consecutive blocks go to the 8 XCDs in turn and each has its own L2: XCD x gets the x-th contiguous eighth of the
+// tile list, and the list walks bands of `band` row tiles so that the tiles in flight on an XCD share their operands.
+__device__ __forceinline__ void tile_of(int id, int total, int tm, int tn, int band, int& m, int& n) {
+  const int q = total / 8, r = total % 8, x = id % 8, i = id / 8;
+  const int t = x * q + (x < r ? x : r) + i;
+  const int per = band * tn, b = t / per, first = b * band, h = (tm - first) < band ? (tm - first) : band;
+  m = first + (t - b * per) % h;
+  n = (t - b * per) / h;
+}
+
+__device__ __forceinline__ uint16_t bf16_bits(float x) {
+  return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
+__device__ __forceinline__ float bf16_value(uint16_t b) { return __builtin_bit_cast(float, (uint32_t)b << 16); }
+
+struct Split {
+  uint16_t hi, lo;
+};
+// hi + lo of an already scaled value; a value that is not finite has no low limb
+__device__ __forceinline__ Split split16(float x) {
+  const _Float16 h = (_Float16)x;
+  const float r = x - (float)h;
+  const _Float16 l = (_Float16)(r == r && fabsf(r) < 65504.f ? r : 0.f);
+  return {__builtin_bit_cast(uint16_t, h), __builtin_bit_cast(uint16_t, l)};
+}
+
+// exponent e with |x| < 2^e for |x| <= m (m finite and > 0; subnormals count as 2^-126)
+__device__ __forceinline__ int exp_above(float m) {
+  const int e = (int)((__builtin_bit_cast(uint32_t, m) >> 23) & 0xffu) - 126;
+  return e < -125 ? -125 : e;
+}
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < __builtin_inff() ? a : 0.f;  // infinities and NaN count as nothing: they pass the limb split by themselves
+}
+
+}  // namespace t16
+#endif

@@ -670,6 +670,37 @@ int hold_knn1_fwd(const float* q, int32_t B, int32_t Nq, const float* t, int32_t
 int hold_knn1_bwd(const float* q, int32_t B, int32_t Nq, const float* t, int32_t Nt, const int32_t* idx, const float* g,
                   float* dq, float* dt_accum, hold_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * The gated layer (csrc/gated.hip):  h = act(x Wg^T + bg) * (x Wu^T + bu)  in one launch over both
+ * projections, and its gradients.  x [T][D], W [H][D], h [T][H]; leading dimensions in elements, the
+ * innermost dimension contiguous; every tensor in `dtype` (fp32: two-limb fp16 products with fp32
+ * accumulation; bf16: bf16 products with fp32 accumulation).
+ * hold_gated_workspace (host only): *bytes = the scratch of one call (256-byte aligned); the pointers
+ * and leading dimensions of the descriptor have to be the call's own, and -- backward -- db_gate /
+ * db_up null or not as in the call.
+ * hold_gated_bwd: dx, dw_gate + dw_up, db_gate, db_up are contiguous and may be null (dw: both or none).
+ * ---------------------------------------------------------------------------------------- */
+enum hold_gated_dtype { HOLD_GATED_F32 = 0, HOLD_GATED_BF16 = 1 };
+enum hold_gated_act { HOLD_GATED_SILU = 0, HOLD_GATED_GELU = 1 /* erf */, HOLD_GATED_RELU = 2, HOLD_GATED_SIGMOID = 3 };
+
+typedef struct hold_gated_desc {
+  const void* x;      int64_t ldx;
+  const void* w_gate; int64_t ldwg;
+  const void* w_up;   int64_t ldwu;
+  const void* b_gate;               /* [H] or NULL */
+  const void* b_up;                 /* [H] or NULL */
+  void* h;            int64_t ldh;  /* forward result */
+  const void* dh;     int64_t lddh; /* backward: the result's gradient */
+  void* dx; void* dw_gate; void* dw_up; void* db_gate; void* db_up;
+  void* workspace;    int64_t workspace_bytes;
+  int64_t T;
+  int32_t D, H, dtype, act;
+} hold_gated_desc;
+
+int hold_gated_workspace(const hold_gated_desc* d, int32_t backward, int64_t* bytes);
+int hold_gated_fwd(const hold_gated_desc* d, hold_stream_t stream);
+int hold_gated_bwd(const hold_gated_desc* d, hold_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
