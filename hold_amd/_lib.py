@@ -112,6 +112,24 @@ class GatedDesc(C.Structure):  # hold_gated_desc
                 ("T", C.c_int64), ("D", C.c_int32), ("H", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32)]
 
 
+class OrthoDesc(C.Structure):  # hold_ortho_desc
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("coef", C.POINTER(C.c_float)), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64), ("batch", C.c_int32), ("rows", C.c_int32), ("cols", C.c_int32), ("dtype", C.c_int32),
+                ("steps", C.c_int32), ("eps", C.c_float)]
+
+
+class MuonItem(C.Structure):  # hold_muon_item
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("m", C.c_void_p), ("rows", C.c_int32), ("cols", C.c_int32), ("ldp", C.c_int32),
+                ("ldg", C.c_int32), ("ldm", C.c_int32), ("scale", C.c_float)]
+
+
+class MuonDesc(C.Structure):  # hold_muon_desc
+    _fields_ = [("items", C.POINTER(MuonItem)), ("coef", C.POINTER(C.c_float)), ("sumsq", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64), ("n_items", C.c_int32), ("steps", C.c_int32), ("nesterov", C.c_int32),
+                ("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("grad_mul", C.c_float),
+                ("clip_norm", C.c_float), ("eps", C.c_float)]
+
+
 _P, _I, _L, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 # developer-build-only symbols (HOLD_DEV=1 at build time): declared when present
 DEV_SIGNATURES = {
@@ -196,6 +214,10 @@ SIGNATURES = {
     "hold_gated_workspace": [C.POINTER(GatedDesc), _I, C.POINTER(_L)],  # host only: no stream
     "hold_gated_fwd": [C.POINTER(GatedDesc), _P],
     "hold_gated_bwd": [C.POINTER(GatedDesc), _P],
+    "hold_orthogonalize_workspace": [C.POINTER(OrthoDesc), C.POINTER(_L)],  # host only: no stream
+    "hold_orthogonalize": [C.POINTER(OrthoDesc), _P],
+    "hold_muon_workspace": [C.POINTER(MuonDesc), C.POINTER(_L)],  # host only: no stream
+    "hold_muon_step": [C.POINTER(MuonDesc), _P],
     "hold_mano_lbs_fwd": [C.POINTER(ManoModel), _I, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     "hold_mano_lbs_bwd": [C.POINTER(ManoModel), _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
 }

@@ -1,0 +1,486 @@
+// Orthogonalised updates: the polynomial iteration that brings the singular values of a matrix near one without a decomposition, and
+// the momentum step that applies it to weight matrices.
+//
+//   X0 = G / (|G|_F + eps)        A = X X^T        X <- (a I + b A + c A A) X       `steps` times, on the side with fewer rows
+//
+// Three products a step (ns_gram, ns_poly, ns_apply below) for ALL matrices of a call in one launch each: a list of matrices of any
+// shapes (or a batch of equal ones) is cut into tiles, and a block finds its matrix in the tile counts.
+//
+// ARITHMETIC.  Small singular values grow by a^steps (485 with the usual coefficients), and with them every rounding of X relative to
+// the largest one; bf16's 2^-9 would be the result there.  So X, A and C = a I + b A + c A A are kept as two fp16 limbs (tile16.h,
+// 2^-22 each) and multiplied by three limb products with fp32 accumulation.  Their scales need no pass over the data: the singular
+// values start at <= 1, the polynomial bounds them after every step (the host follows that bound), and no entry of a matrix is larger
+// than its largest singular value.  The norm is summed in fp64: neither huge nor tiny gradients leave its range.
+#include "tile16.h"
+
+#include <math.h>
+
+#include "../../include/hold_hip.h"
+
+using namespace t16;
+
+namespace {
+
+constexpr int MAXI = 36;  // items of one launch (kernel arguments stay below 4 KB)
+
+struct Item {
+  const void* g;  // the matrix (orthogonalise), the gradient (step)
+  void* m;        // momentum, or null
+  void* p;        // the result, or the parameter
+  int64_t stride; // elements from one matrix of the item to the next, in all three
+  int64_t x, c;   // this item's first X and first A, in elements of the workspace's halves
+  int rows, cols, ldg, ldm, ldp, count;
+  int part, nb;   // first partial sum, partial sums a matrix
+  float gain;     // the step's factor: learning rate times the scale of the matrix's shape
+};
+struct Items {
+  Item it[MAXI];
+  int n;
+};
+struct Step {
+  float mu, decay, grad_mul, clip, eps;
+  int nesterov, dtype;
+  const float* sumsq;
+};
+// per-launch tile counts: item k's tiles begin at first[k]
+struct Tiles {
+  int first[MAXI + 1];
+};
+
+__device__ __forceinline__ int item_of(const Tiles& t, int n, int id) {
+  int k = 0;
+  while (k + 1 < n && id >= t.first[k + 1]) ++k;
+  return k;
+}
+__host__ __device__ __forceinline__ int up8(int v) { return (v + 7) / 8 * 8; }
+
+__device__ __forceinline__ float value(const void* p, int64_t i, int dtype) {
+  if (dtype == HOLD_MUON_F32) return ((const float*)p)[i];
+  const uint16_t b = ((const uint16_t*)p)[i];
+  return dtype == HOLD_MUON_BF16 ? bf16_value(b) : (float)__builtin_bit_cast(_Float16, b);
+}
+__device__ __forceinline__ void put(void* p, int64_t i, int dtype, float v) {
+  if (dtype == HOLD_MUON_F32) ((float*)p)[i] = v;
+  else ((uint16_t*)p)[i] = dtype == HOLD_MUON_BF16 ? bf16_bits(v) : __builtin_bit_cast(uint16_t, (_Float16)v);
+}
+
+// the factor of the gradients: grad_mul and the clip to a global norm, as hold_adam_step has them
+__device__ __forceinline__ float grad_scale(const Step& s) {
+  float f = s.grad_mul;
+  if (s.clip > 0.f && s.sumsq) f *= fminf(1.f, s.clip / (sqrtf(s.sumsq[0]) * fabsf(s.grad_mul) + 1e-6f));
+  return f;
+}
+// the matrix to orthogonalise at element (r, c) once the momentum is updated
+__device__ __forceinline__ float update_of(const Item& it, const Step& s, float f, int64_t b, int r, int c) {
+  const float g = value(it.g, b + (int64_t)r * it.ldg + c, s.dtype);
+  if (!it.m) return g;
+  const float m = ((const float*)it.m)[b + (int64_t)r * it.ldm + c];
+  return s.nesterov ? (1.f - s.mu) * (g * f) + s.mu * m : m;
+}
+
+// momentum and the partial sums of squares, 256 threads on an equal share of a matrix's elements; partial sums are added in a fixed order
+__global__ __launch_bounds__(256) void ns_norm_kernel(Items a, Tiles t, Step s, double* part) {
+  const int k = item_of(t, a.n, blockIdx.x);
+  const Item& it = a.it[k];
+  const int q = blockIdx.x - t.first[k], mat = q / it.nb, blk = q % it.nb;
+  const int64_t b = mat * it.stride, n = (int64_t)it.rows * it.cols, per = (n + it.nb - 1) / it.nb;
+  const int64_t end = (blk + 1) * per < n ? (blk + 1) * per : n;
+  const float f = it.m ? grad_scale(s) : 1.f;
+  double sum = 0.;
+  const bool lin = it.ldg == it.cols && it.ldm == it.cols;
+  for (int64_t e = blk * per + threadIdx.x; e < end; e += 256) {
+    const int r = lin ? 0 : (int)(e / it.cols);
+    const int64_t c = e - (int64_t)r * it.cols;
+    const float g = value(it.g, b + (int64_t)r * it.ldg + c, s.dtype);
+    float u = g;
+    if (it.m) {
+      float* mp = (float*)it.m + b + (int64_t)r * it.ldm + c;
+      const float gf = g * f, m = s.mu * *mp + (1.f - s.mu) * gf;
+      *mp = m;
+      u = s.nesterov ? (1.f - s.mu) * gf + s.mu * m : m;
+    }
+    sum += (double)u * u;
+  }
+  __shared__ double w[4];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) part[it.part + q] = (w[0] + w[1]) + (w[2] + w[3]);
+}
+
+// X0 as limbs [min][max] (rounded up to 8, zeros behind), scaled by 2^xs: 64 x 64 tiles of the source through LDS, transposed where it is tall
+__global__ __launch_bounds__(256) void ns_load_kernel(Items a, Tiles t, Step s, const double* part, uint16_t* ws, int64_t limb, int xs) {
+  const int k = item_of(t, a.n, blockIdx.x);
+  const Item& it = a.it[k];
+  const bool tall = it.rows > it.cols;
+  const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols, mp = up8(m), np = up8(n);
+  const int tn = (np + 63) / 64, tm = (mp + 63) / 64;
+  const int q = blockIdx.x - t.first[k], mat = q / (tm * tn), tile = q % (tm * tn), i0 = tile / tn * 64, j0 = tile % tn * 64;
+  __shared__ float s_tile[64][65];
+  __shared__ double s_sum[4];
+  double sum = 0.;
+  for (int i = threadIdx.x; i < it.nb; i += 256) sum += part[it.part + mat * it.nb + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
+  const int64_t b = mat * it.stride;
+  const float f = it.m ? grad_scale(s) : 1.f;
+  const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;  // the tile's place in the source
+  for (int e = threadIdx.x; e < 4096; e += 256) {
+    const int r = e >> 6, c = e & 63;
+    s_tile[r][c] = r0 + r < it.rows && c0 + c < it.cols ? update_of(it, s, f, b, r0 + r, c0 + c) : 0.f;
+  }
+  __syncthreads();
+  const double inv = ldexp(1. / (sqrt((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])) + (double)s.eps), xs);
+  uint16_t* x = ws + it.x + (int64_t)mat * mp * np;
+  for (int e = threadIdx.x; e < 512; e += 256) {
+    const int i = e >> 3, j = (e & 7) * 8;
+    if (i0 + i >= mp || j0 + j >= np) continue;
+    u32x4 h, l;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float v = tall ? s_tile[j + 2 * r][i] : s_tile[i][j + 2 * r], w = tall ? s_tile[j + 2 * r + 1][i] : s_tile[i][j + 2 * r + 1];
+      const bool in = i0 + i < m;  // behind the last row and column: zeros, also where the norm is not finite
+      const Split y = split16(in && j0 + j + 2 * r < n ? (float)(v * inv) : 0.f), z = split16(in && j0 + j + 2 * r + 1 < n ? (float)(w * inv) : 0.f);
+      h[r] = y.hi | (uint32_t)z.hi << 16;
+      l[r] = y.lo | (uint32_t)z.lo << 16;
+    }
+    uint16_t* o = x + (int64_t)(i0 + i) * np + j0 + j;
+    *(u32x4*)o = h;
+    *(u32x4*)(o + limb) = l;
+  }
+}
+
+__device__ __forceinline__ void store_limbs(uint16_t* o, int64_t limb, f32x4 v) {
+  Split y[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = split16(v[r]);
+  *(u32x2*)o = u32x2{y[0].hi | (uint32_t)y[1].hi << 16, y[2].hi | (uint32_t)y[3].hi << 16};
+  *(u32x2*)(o + limb) = u32x2{y[0].lo | (uint32_t)y[1].lo << 16, y[2].lo | (uint32_t)y[3].lo << 16};
+}
+__device__ __forceinline__ float half_value(uint32_t w, int h) { return (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> (16 * h))); }
+__device__ __forceinline__ f32x4 load_limbs(const uint16_t* p, int64_t limb) {
+  const u32x2 h = *(const u32x2*)p, l = *(const u32x2*)(p + limb);
+  f32x4 v;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = half_value(h[r >> 1], r & 1) + half_value(l[r >> 1], r & 1);
+  return v;
+}
+
+enum { GRAM = 0, POLY = 1, APPLY = 2 };
+struct NsArgs {
+  const uint16_t* x;  // X: hi at the item's place, lo `limb` further
+  uint16_t* y;        // the next X
+  uint16_t* am;       // A
+  uint16_t* cm;       // C = a I + b A + c A A
+  int64_t xlimb, climb;
+  float a, b, c;      // POLY, already in the scales of its operands and its result
+  int shift;          // exponent from the accumulated sum to the stored limbs
+  int last;           // APPLY: write the result instead of the next X
+};
+
+template <int KIND, int T, int WM, int WN, int S>
+__global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(Items a, Tiles t, NsArgs s, Step st) {
+  using Cr = Core<MODE_F16X3, KC, KIND == APPLY ? KS : KC, T, T, 1, WM, WN, S>;
+  __shared__ __align__(1024) char smem[Cr::LDS];
+  // the tile list is cut into an eighth for each XCD, as tile_of does: neighbours share a matrix
+  const int total = gridDim.x, qq = total / 8, rr = total % 8, xcd = blockIdx.x % 8, ii = blockIdx.x / 8;
+  const int id = xcd * qq + (xcd < rr ? xcd : rr) + ii;
+  const int k = item_of(t, a.n, id);
+  const Item& it = a.it[k];
+  const bool tall = it.rows > it.cols;
+  const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols, mp = up8(m), np = up8(n);
+  const int tm = (mp + T - 1) / T, tn = KIND == APPLY ? (np + T - 1) / T : tm;
+  const int q = id - t.first[k], mat = q / (tm * tn), tile = q % (tm * tn);
+  // bands of 8 row tiles, column by column
+  const int per = 8 * tn, band = tile / per, f0 = band * 8, h = tm - f0 < 8 ? tm - f0 : 8, i0 = (f0 + (tile - band * per) % h) * T, j0 = (tile - band * per) / h * T;
+  const int64_t xo = it.x + (int64_t)mat * mp * np, co = it.c + (int64_t)mat * mp * mp;
+  typename Cr::Acc acc;
+  Cr::zero(acc);
+  if (KIND == GRAM) {
+    const Operand A = {s.x + xo + (int64_t)i0 * np, s.xlimb, np, mp - i0, np};
+    const Operand B[1] = {{s.x + xo + (int64_t)j0 * np, s.xlimb, np, mp - j0, np}};
+    Cr::run(smem, A, B, acc);
+  } else if (KIND == POLY) {
+    const Operand A = {s.am + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
+    const Operand B[1] = {{s.am + co + (int64_t)j0 * mp, s.climb, mp, mp - j0, mp}};
+    Cr::run(smem, A, B, acc);
+  } else {
+    const Operand A = {s.cm + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
+    const Operand B[1] = {{s.x + xo + j0, s.xlimb, np, np - j0, mp}};
+    Cr::run(smem, A, B, acc);
+  }
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  const int64_t b = mat * it.stride;
+#pragma unroll
+  for (int mi = 0; mi < Cr::MI; ++mi) {
+    const int i = i0 + wm * (T / WM) + 16 * mi + (lane & 15);
+#pragma unroll
+    for (int ni = 0; ni < Cr::NI; ++ni) {
+      const int j = j0 + wn * (T / WN) + 16 * ni + 4 * (lane >> 4);
+      if (i >= mp || j >= (KIND == APPLY ? np : mp)) continue;
+      f32x4 v = acc[0][mi][ni];
+      if (KIND == GRAM) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], s.shift);
+        store_limbs(s.am + co + (int64_t)i * mp + j, s.climb, v);
+      } else if (KIND == POLY) {
+        const f32x4 u = load_limbs(s.am + co + (int64_t)i * mp + j, s.climb);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = fmaf(s.c, v[r], s.b * u[r]) + (i == j + r ? s.a : 0.f);
+        store_limbs(s.cm + co + (int64_t)i * mp + j, s.climb, v);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], s.shift);
+        if (!s.last) {
+          store_limbs(s.y + xo + (int64_t)i * np + j, s.xlimb, v);
+        } else if (i < m) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (j + r >= n) continue;
+            const int64_t at = b + (tall ? (int64_t)(j + r) * it.ldp + i : (int64_t)i * it.ldp + j + r);
+            if (it.m) {
+              float* p = (float*)it.p + at;
+              *p = *p * st.decay - it.gain * v[r];
+            } else {
+              put(it.p, at, st.dtype, v[r]);
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+inline int ok() { return hipGetLastError() == hipSuccess ? HOLD_OK : HOLD_E_LAUNCH; }
+
+// The bounds of the singular values of X, and of the entries of A and C, through the iteration; false: they leave the range of the limbs
+struct Bounds {
+  int xs[33], as[33], cs[33];  // exponents of the scales: largest entry to below 2^14, a factor of 4 under fp16's range
+};
+bool follow(const float* coef, int steps, Bounds& o) {
+  double r = 1.;
+  for (int k = 0; k <= steps; ++k) {
+    if (!(r < 1e9) || !(r > 1e-9)) return false;
+    o.xs[k] = 14 - (int)ceil(log2(r));
+    if (k == steps) break;
+    o.as[k] = 14 - (int)ceil(2. * log2(r));
+    const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2], S = r * r;
+    if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
+    auto P = [&](double s) { return fabs(a + b * s + c * s * s); };
+    double top = fmax(P(0.), P(S));
+    if (c != 0. && -b / (2. * c) > 0. && -b / (2. * c) < S) top = fmax(top, P(-b / (2. * c)));
+    if (!(top < 1e9) || !(top > 1e-9)) return false;
+    o.cs[k] = 14 - (int)ceil(log2(top));
+    // the largest |s (a + b s^2 + c s^4)| on [0, r]: its ends and where a + 3 b s^2 + 5 c s^4 = 0
+    double next = r * P(S);
+    auto at = [&](double s2) {
+      if (s2 > 0. && s2 < S) next = fmax(next, sqrt(s2) * P(s2));
+    };
+    if (c != 0.) {
+      const double disc = 9. * b * b - 20. * a * c;
+      if (disc >= 0.) {
+        at((-3. * b + sqrt(disc)) / (10. * c));
+        at((-3. * b - sqrt(disc)) / (10. * c));
+      }
+    } else if (b != 0.) {
+      at(-a / (3. * b));
+    }
+    r = next;
+  }
+  return true;
+}
+
+inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// the workspace of one group of items: partial sums, X twice, A and C, all limbs
+struct Room {
+  int64_t part, x, y, am, cm, xn, cn, bytes;
+};
+Room room(Items& a) {
+  Room r = {};
+  int64_t parts = 0, xn = 0, cn = 0;
+  for (int k = 0; k < a.n; ++k) {
+    Item& it = a.it[k];
+    const int64_t mp = up8(it.rows < it.cols ? it.rows : it.cols), np = up8(it.rows < it.cols ? it.cols : it.rows), n = (int64_t)it.rows * it.cols;
+    const int64_t nb = (n + 16383) / 16384;
+    it.nb = (int)(nb > 1024 ? 1024 : nb);
+    it.part = (int)parts;
+    it.x = xn;
+    it.c = cn;
+    parts += (int64_t)it.nb * it.count;
+    xn += mp * np * it.count;
+    cn += mp * mp * it.count;
+  }
+  xn = up256(xn); cn = up256(cn);
+  int64_t o = 0;
+  auto take = [&](int64_t bytes) { const int64_t at = o; o += up256(bytes); return at; };
+  r.part = take(parts * 8);
+  r.x = take(xn * 4);
+  r.y = take(xn * 4);
+  r.am = take(cn * 4);
+  r.cm = take(cn * 4);
+  r.xn = xn; r.cn = cn;
+  r.bytes = o;
+  return r;
+}
+
+template <int KIND>
+int launch(const Items& a, const NsArgs& s, const Step& st, hipStream_t stream) {
+  auto tiles = [&](int T, Tiles& t) {
+    int64_t n = 0;
+    for (int k = 0; k < a.n; ++k) {
+      const Item& it = a.it[k];
+      const int64_t mp = up8(it.rows < it.cols ? it.rows : it.cols), np = up8(it.rows < it.cols ? it.cols : it.rows);
+      t.first[k] = (int)n;
+      n += ((mp + T - 1) / T) * ((KIND == APPLY ? np + T - 1 : mp + T - 1) / T) * it.count;
+      if (n > (1 << 30)) return (int64_t)-1;
+    }
+    t.first[a.n] = (int)n;
+    return n;
+  };
+  Tiles t = {};
+  int64_t n = tiles(128, t);
+  if (n < 0) return HOLD_E_ARG;
+  if (n >= 256) {
+    hipLaunchKernelGGL((ns_mma_kernel<KIND, 128, 2, 2, 2>), dim3((unsigned)n), dim3(256), 0, stream, a, t, s, st);
+  } else {
+    n = tiles(64, t);
+    if (n < 0) return HOLD_E_ARG;
+    hipLaunchKernelGGL((ns_mma_kernel<KIND, 64, 2, 2, 8>), dim3((unsigned)n), dim3(256), 0, stream, a, t, s, st);
+  }
+  return HOLD_OK;
+}
+
+int run_group(Items& a, const Step& st, const float* coef, int steps, char* ws, hipStream_t stream) {
+  Bounds bo;
+  if (!follow(coef, steps, bo)) return HOLD_E_ARG;
+  const Room r = room(a);
+  double* part = (double*)(ws + r.part);
+  uint16_t* x = (uint16_t*)(ws + r.x);
+  uint16_t* y = (uint16_t*)(ws + r.y);
+  Tiles tn = {}, tl = {};
+  int64_t nn = 0, nl = 0;
+  for (int k = 0; k < a.n; ++k) {
+    const Item& it = a.it[k];
+    const int64_t mp = up8(it.rows < it.cols ? it.rows : it.cols), np = up8(it.rows < it.cols ? it.cols : it.rows);
+    tn.first[k] = (int)nn;
+    tl.first[k] = (int)nl;
+    nn += (int64_t)it.nb * it.count;
+    nl += ((mp + 63) / 64) * ((np + 63) / 64) * it.count;
+    if (nn > (1 << 30) || nl > (1 << 30)) return HOLD_E_ARG;
+  }
+  hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)nn), dim3(256), 0, stream, a, tn, st, part);
+  hipLaunchKernelGGL(ns_load_kernel, dim3((unsigned)nl), dim3(256), 0, stream, a, tl, st, part, x, r.xn, bo.xs[0]);
+  NsArgs s = {};
+  s.am = (uint16_t*)(ws + r.am);
+  s.cm = (uint16_t*)(ws + r.cm);
+  s.xlimb = r.xn;
+  s.climb = r.cn;
+  for (int k = 0; k < steps; ++k) {
+    s.x = x;
+    s.y = y;
+    s.shift = bo.as[k] - 2 * bo.xs[k];
+    if (launch<GRAM>(a, s, st, stream) != HOLD_OK) return HOLD_E_ARG;
+    s.a = (float)ldexp((double)coef[3 * k], bo.cs[k]);
+    s.b = (float)ldexp((double)coef[3 * k + 1], bo.cs[k] - bo.as[k]);
+    s.c = (float)ldexp((double)coef[3 * k + 2], bo.cs[k] - 2 * bo.as[k]);
+    if (launch<POLY>(a, s, st, stream) != HOLD_OK) return HOLD_E_ARG;
+    s.last = k + 1 == steps;
+    s.shift = (s.last ? 0 : bo.xs[k + 1]) - bo.cs[k] - bo.xs[k];
+    if (launch<APPLY>(a, s, st, stream) != HOLD_OK) return HOLD_E_ARG;
+    uint16_t* z = x;
+    x = y;
+    y = z;
+  }
+  return ok();
+}
+
+bool sizes_ok(int64_t rows, int64_t cols, int64_t count) {
+  return rows >= 1 && cols >= 1 && count >= 1 && rows <= (1 << 20) && cols <= (1 << 20) && count <= (1 << 24);
+}
+bool one_item(const hold_ortho_desc* d, Items& a) {
+  if (!d || !sizes_ok(d->rows, d->cols, d->batch)) return false;
+  a.n = 1;
+  Item& it = a.it[0];
+  it = Item{};
+  it.rows = d->rows;
+  it.cols = it.ldg = it.ldm = it.ldp = d->cols;
+  it.count = d->batch;
+  it.stride = (int64_t)d->rows * d->cols;
+  return true;
+}
+// items first .. first + n - 1 of a step
+bool some_items(const hold_muon_desc* d, int first, Items& a) {
+  a.n = d->n_items - first < MAXI ? d->n_items - first : MAXI;
+  for (int k = 0; k < a.n; ++k) {
+    const hold_muon_item& i = d->items[first + k];
+    if (!sizes_ok(i.rows, i.cols, 1) || i.ldp < i.cols || i.ldg < i.cols || i.ldm < i.cols) return false;
+    Item& it = a.it[k];
+    it = Item{};
+    it.g = i.g; it.m = i.m; it.p = i.p;
+    it.rows = i.rows; it.cols = i.cols; it.count = 1;
+    it.ldg = i.ldg; it.ldm = i.ldm; it.ldp = i.ldp;
+    it.gain = d->lr * i.scale;
+  }
+  return true;
+}
+
+}  // namespace
+
+extern "C" int hold_orthogonalize_workspace(const hold_ortho_desc* d, int64_t* bytes) {
+  Items a;
+  if (!one_item(d, a) || !bytes) return HOLD_E_ARG;
+  *bytes = room(a).bytes;
+  return HOLD_OK;
+}
+
+extern "C" int hold_orthogonalize(const hold_ortho_desc* d, hold_stream_t stream) {
+  Items a;
+  if (!one_item(d, a) || !d->x || !d->out || !d->coef || d->steps < 1 || d->steps > 32 || d->dtype < 0 || d->dtype > 2 || !(d->eps >= 0.f)) return HOLD_E_ARG;
+  if (!d->workspace || room(a).bytes > d->workspace_bytes) return HOLD_E_ARG;
+  a.it[0].g = d->x;
+  a.it[0].p = d->out;
+  Step st = {};
+  st.eps = d->eps;
+  st.dtype = d->dtype;
+  return run_group(a, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+}
+
+extern "C" int hold_muon_workspace(const hold_muon_desc* d, int64_t* bytes) {
+  if (!d || !bytes || d->n_items < 1 || !d->items) return HOLD_E_ARG;
+  *bytes = 0;
+  for (int first = 0; first < d->n_items; first += MAXI) {
+    Items a;
+    if (!some_items(d, first, a)) return HOLD_E_ARG;
+    const int64_t n = room(a).bytes;
+    if (n > *bytes) *bytes = n;
+  }
+  return HOLD_OK;
+}
+
+extern "C" int hold_muon_step(const hold_muon_desc* d, hold_stream_t stream) {
+  int64_t need = 0;
+  Bounds bo;
+  if (hold_muon_workspace(d, &need) != HOLD_OK || !d->workspace || need > d->workspace_bytes) return HOLD_E_ARG;
+  if (!d->coef || d->steps < 1 || d->steps > 32 || !(d->eps >= 0.f) || !follow(d->coef, d->steps, bo)) return HOLD_E_ARG;
+  for (int k = 0; k < d->n_items; ++k)
+    if (!d->items[k].p || !d->items[k].g || !d->items[k].m) return HOLD_E_ARG;
+  Step st = {};
+  st.eps = d->eps;
+  st.dtype = HOLD_MUON_F32;
+  st.mu = d->momentum;
+  st.nesterov = d->nesterov;
+  st.decay = (float)(1.0 - (double)d->lr * (double)d->weight_decay);
+  st.grad_mul = d->grad_mul;
+  st.clip = d->clip_norm;
+  st.sumsq = d->sumsq;
+  for (int first = 0; first < d->n_items; first += MAXI) {  // groups share the workspace: they run one after the other
+    Items a;
+    some_items(d, first, a);
+    const int rc = run_group(a, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+    if (rc != HOLD_OK) return rc;
+  }
+  return HOLD_OK;
+}

@@ -14,7 +14,7 @@
 // a KC row is masked per 16-byte chunk.  Required, and ensured by the callers' checks or padded copies: 16-byte aligned bases, leading
 // dimensions in multiples of 8 elements, K (KC) resp. row count (KS) rounded up to 8 inside the allocation.
 //
-// PIPELINE.  Two LDS stages: the loads of step k + 1 are in flight while step k is multiplied; one s_waitcnt + s_barrier per step.
+// PIPELINE.  S LDS stages: the loads of the next S - 1 steps are in flight while one is multiplied; one s_waitcnt + s_barrier a step.
 #ifndef HOLD_TILE16_H
 #define HOLD_TILE16_H
 #include <hip/hip_runtime.h>
@@ -145,13 +145,13 @@ __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
 // A block of WM x WN waves computes a BM x BN tile for each of NB operands B that share A.  The matrix instruction's first operand
 // is B: a lane then holds FOUR CONSECUTIVE j of ONE row i, so results leave as 8- or 16-byte stores:
 //   acc[b][mi][ni][r]:  i = wm BM / WM + 16 mi + lane % 16,   j = wn BN / WN + 16 ni + 4 (lane / 16) + r
-template <int MODE, int LA, int LB, int BM, int BN, int NB, int WM, int WN>
+template <int MODE, int LA, int LB, int BM, int BN, int NB, int WM, int WN, int S = 2>
 struct Core {
   static constexpr int BK = step_k<MODE>(), NL = limbs<MODE>(), NW = WM * WN;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
   using TA = Tile<LA, BM, BK>;
   using TB = Tile<LB, BN, BK>;
-  static constexpr int STAGE = NL * (TA::BYTES + NB * TB::BYTES), LDS = 2 * STAGE;
+  static constexpr int STAGE = NL * (TA::BYTES + NB * TB::BYTES), LDS = S * STAGE;
   static constexpr int THREADS = 64 * NW;
   typedef f32x4 Acc[NB][MI][NI];
 
@@ -185,13 +185,22 @@ struct Core {
         for (int b = 0; b < NB; ++b) lb[b].load(B[b], l, (int64_t)kt * BK, s + NL * TA::BYTES + (b * NL + l) * TB::BYTES, wave);
       }
     };
-    stage(0, smem);
+    // loads a wave issues per stage (the same for every wave: Loader's static_assert, or PIECES < NW and then S == 2)
+    constexpr int LPS = NL * (Loader<LA, BM, BK, NW>::N + NB * Loader<LB, BN, BK, NW>::N), AHEAD = (S - 2) * LPS;
+    static_assert(S == 2 || (TA::PIECES % NW == 0 && TB::PIECES % NW == 0 && AHEAD < 63), "countable loads");
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+      if (i < nk) stage(i, smem + i * STAGE);
+    int at = 0, to = S - 1;  // the stage that is read, the stage that is filled
     for (int kt = 0; kt < nk; ++kt) {
-      const char* s = smem + (kt & 1) * STAGE;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const char* s = smem + at * STAGE;
+      if (S == 2 || kt + S - 1 > nk) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (kt + 1 < nk) stage(kt + 1, smem + ((kt + 1) & 1) * STAGE);
+      if (kt + S - 1 < nk) stage(kt + S - 1, smem + to * STAGE);
+      at = at + 1 == S ? 0 : at + 1;
+      to = to + 1 == S ? 0 : to + 1;
       const char* sa = s;
       const char* sb = s + NL * TA::BYTES;
 #pragma unroll

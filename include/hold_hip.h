@@ -701,6 +701,49 @@ int hold_gated_workspace(const hold_gated_desc* d, int32_t backward, int64_t* by
 int hold_gated_fwd(const hold_gated_desc* d, hold_stream_t stream);
 int hold_gated_bwd(const hold_gated_desc* d, hold_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Orthogonalised updates (csrc/muon.hip).  The iteration X0 = G / (|G|_F + eps), A = X X^T,
+ * X <- (a I + b A + c A A) X, `steps` times with coef[3 k .. 3 k + 2] = (a, b, c) of step k (HOST
+ * array), on the side with fewer rows.  HOLD_E_ARG where the polynomial lets the largest singular
+ * value grow or shrink beyond 1e9 / 1e-9.
+ * hold_orthogonalize: out[k] = the iteration's result for x[k], k < batch; both [batch][rows][cols]
+ *   contiguous, in `dtype`.
+ * hold_muon_step, for every item (fp32, rows of ld elements):
+ *   f = grad_mul * min(1, clip_norm / (sqrt(*sumsq) |grad_mul| + 1e-6))  (clip_norm 0 or sumsq NULL: grad_mul)
+ *   m = momentum m + (1 - momentum) f g;   u = nesterov ? (1 - momentum) f g + momentum m : m
+ *   p = (1 - lr weight_decay) p - lr scale O(u)
+ * The *_workspace functions (host only) give the scratch of one call (256-byte aligned).
+ * ---------------------------------------------------------------------------------------- */
+enum hold_muon_dtype { HOLD_MUON_F32 = 0, HOLD_MUON_BF16 = 1, HOLD_MUON_F16 = 2 };
+
+typedef struct hold_ortho_desc {
+  const void* x; void* out;
+  const float* coef;                /* HOST, [3 steps] */
+  void* workspace; int64_t workspace_bytes;
+  int32_t batch, rows, cols, dtype, steps;
+  float eps;
+} hold_ortho_desc;
+
+typedef struct hold_muon_item {
+  float* p; const float* g; float* m;
+  int32_t rows, cols, ldp, ldg, ldm;
+  float scale;
+} hold_muon_item;
+
+typedef struct hold_muon_desc {
+  const hold_muon_item* items;      /* HOST */
+  const float* coef;                /* HOST, [3 steps] */
+  const float* sumsq;               /* device scalar or NULL */
+  void* workspace; int64_t workspace_bytes;
+  int32_t n_items, steps, nesterov;
+  float lr, momentum, weight_decay, grad_mul, clip_norm, eps;
+} hold_muon_desc;
+
+int hold_orthogonalize_workspace(const hold_ortho_desc* d, int64_t* bytes);
+int hold_orthogonalize(const hold_ortho_desc* d, hold_stream_t stream);
+int hold_muon_workspace(const hold_muon_desc* d, int64_t* bytes);
+int hold_muon_step(const hold_muon_desc* d, hold_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
