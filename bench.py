@@ -65,6 +65,8 @@ def parse():
                     help="A/B: run every sample through every stage (hold_amd.field.COMPACT = False)")
     ap.add_argument("--precision", default=None, choices=["f32", "f32x6", "f16x3"],
                     help="arithmetic of the MFMA kernels (hold_amd/config.py); default: the package default")
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "muon"],
+                    help="adam: the reference's; muon: hidden matrices by orthogonalised momentum (hold_amd.optim.FlatMuon)")
     ap.add_argument("--no-profile", action="store_true")
     ap.add_argument("--c2-alt", action="store_true",
                     help="SURVEY 8(d)'s second reading of BASELINE's '64+64 samples': N_samples_eval=64 coarse + N_samples=64 fine, no extras "
@@ -314,7 +316,7 @@ def main():
     from hold_amd import synthetic as syn
     from hold_amd.hold_net import DEFAULT_SAMPLER
     from hold_amd.loss import Loss
-    from hold_amd.optim import FlatAdam
+    from hold_amd.optim import FlatAdam, FlatMuon
     from hold_amd.train import render_frame, train_step
 
     hold_amd.set_precision("f32" if args.fp32_mfma else (args.precision or hold_amd.config.DEFAULT_PRECISION))
@@ -356,7 +358,7 @@ def main():
                                      torch.cat([node.params.global_orient.weight[:1], node.params.pose.weight[:1]], 1),
                                      node.params.betas.weight[:1])
                     node.spawn_cano_mano(so)
-    opt = FlatAdam(net, lr=5e-4, clip_norm=0.5) if training else None
+    opt = (FlatMuon if args.optimizer == "muon" else FlatAdam)(net, lr=5e-4, clip_norm=0.5) if training else None
     frozen = opt.flat.clone() if (training and not args.no_freeze) else None
 
     uv = syn.make_uv(W, H)
@@ -579,7 +581,7 @@ def main():
                          else f"configs[2]-like 10-frame training step at {args.c3_pixels} random pixels per frame = {10 * args.c3_pixels} rays "
                               "(NOT the reference's batch size: --c3-pixels), ") + scene +
                         f"fwd + {'full Loss (loss targets on)' if loss_fn else 'rgb/sem loss'} + bwd incl. pose-table "
-                        "gradients + clip + Adam")
+                        f"gradients + clip + {'Adam' if args.optimizer == 'adam' else 'FlatMuon'}")
             metric = "rendered rays/sec (fwd+bwd) at the reference's 1 280-ray training batch -- secondary metric (configs[2])"
         elif args.mode == "c5":
             workload = (f"configs[4]: batch render, 1 sequence per GPU, {W}x{H} = {W * H} rays, N_samples = 128 (162 "
@@ -591,7 +593,7 @@ def main():
                          "importance + 2 samples per fg node (N_samples_extra = 0), 32 bg samples, " if args.c2_alt else
                          "128-sample error-bound hierarchy -> 64 importance + 2 + 32 extra samples per fg node, 32 bg samples, ") +
                         ("fwd + " + ("full reference Loss (eikonal, MANO-cano SDF, opacity-sparsity targets on)" if loss_fn else
-                                     "rgb/sem loss") + " + bwd + grad clip + Adam step" if training else "eval forward only"))
+                                     "rgb/sem loss") + f" + bwd + grad clip + {'Adam' if args.optimizer == 'adam' else 'FlatMuon'} step" if training else "eval forward only"))
             metric = ("rendered rays/sec (fwd+bwd) at 512x512, 64+64 samples read as N_samples_eval=64 + N_samples=64 -- secondary metric"
                       if (training and args.c2_alt) else "rendered rays/sec (fwd+bwd) at 512x512, 64+64 samples" if training else
                       "rendered rays/sec (forward only, eval mode) -- secondary metric")

@@ -125,8 +125,8 @@ class MuonItem(C.Structure):  # hold_muon_item
 
 class MuonDesc(C.Structure):  # hold_muon_desc
     _fields_ = [("items", C.POINTER(MuonItem)), ("coef", C.POINTER(C.c_float)), ("sumsq", C.c_void_p), ("workspace", C.c_void_p),
-                ("workspace_bytes", C.c_int64), ("n_items", C.c_int32), ("steps", C.c_int32), ("nesterov", C.c_int32),
-                ("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("grad_mul", C.c_float),
+                ("workspace_bytes", C.c_int64), ("lr", C.c_double), ("momentum", C.c_double), ("weight_decay", C.c_double),
+                ("n_items", C.c_int32), ("steps", C.c_int32), ("nesterov", C.c_int32), ("grad_mul", C.c_float),
                 ("clip_norm", C.c_float), ("eps", C.c_float)]
 
 

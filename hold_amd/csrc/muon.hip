@@ -38,7 +38,7 @@ struct Items {
   int n;
 };
 struct Step {
-  float mu, decay, grad_mul, clip, eps;
+  float mu, rest, decay, grad_mul, clip, eps;  // rest = 1 - mu
   int nesterov, dtype;
   const float* sumsq;
 };
@@ -75,7 +75,7 @@ __device__ __forceinline__ float update_of(const Item& it, const Step& s, float 
   const float g = value(it.g, b + (int64_t)r * it.ldg + c, s.dtype);
   if (!it.m) return g;
   const float m = ((const float*)it.m)[b + (int64_t)r * it.ldm + c];
-  return s.nesterov ? (1.f - s.mu) * (g * f) + s.mu * m : m;
+  return s.nesterov ? s.rest * (g * f) + s.mu * m : m;
 }
 
 // momentum and the partial sums of squares, 256 threads on an equal share of a matrix's elements; partial sums are added in a fixed order
@@ -95,9 +95,9 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Items a, Tiles t, Step s, 
     float u = g;
     if (it.m) {
       float* mp = (float*)it.m + b + (int64_t)r * it.ldm + c;
-      const float gf = g * f, m = s.mu * *mp + (1.f - s.mu) * gf;
+      const float gf = g * f, m = s.mu * *mp + s.rest * gf;
       *mp = m;
-      u = s.nesterov ? (1.f - s.mu) * gf + s.mu * m : m;
+      u = s.nesterov ? s.rest * gf + s.mu * m : m;
     }
     sum += (double)u * u;
   }
@@ -422,7 +422,7 @@ bool some_items(const hold_muon_desc* d, int first, Items& a) {
     it.g = i.g; it.m = i.m; it.p = i.p;
     it.rows = i.rows; it.cols = i.cols; it.count = 1;
     it.ldg = i.ldg; it.ldm = i.ldm; it.ldp = i.ldp;
-    it.gain = d->lr * i.scale;
+    it.gain = (float)(d->lr * i.scale);
   }
   return true;
 }
@@ -470,9 +470,10 @@ extern "C" int hold_muon_step(const hold_muon_desc* d, hold_stream_t stream) {
   Step st = {};
   st.eps = d->eps;
   st.dtype = HOLD_MUON_F32;
-  st.mu = d->momentum;
+  st.mu = (float)d->momentum;
+  st.rest = (float)(1.0 - d->momentum);
   st.nesterov = d->nesterov;
-  st.decay = (float)(1.0 - (double)d->lr * (double)d->weight_decay);
+  st.decay = (float)(1.0 - d->lr * d->weight_decay);
   st.grad_mul = d->grad_mul;
   st.clip = d->clip_norm;
   st.sumsq = d->sumsq;

@@ -43,7 +43,7 @@ class FlatAdam:
     def __init__(self, net, lr=5e-4, pose_lr_scale=0.1, betas=(0.9, 0.999), eps=1e-8, clip_norm=0.5, group=None):
         self.net, self.lr, self.pose_lr_scale = net, float(lr), float(pose_lr_scale)
         self.betas, self.eps, self.clip_norm, self.group = betas, float(eps), float(clip_norm or 0.0), group
-        low, main = split_params(net)
+        low, main = self.split(net)
         self.params = low + main
         assert self.params, "no trainable parameters"
         dev = self.params[0].device
@@ -77,6 +77,10 @@ class FlatAdam:
         self.step_count = 0
 
     ALIGN = 64  # floats
+
+    def split(self, net):
+        """(pose-table parameters, the others) in the order of the bucket"""
+        return split_params(net)
 
     def zero_grad(self):
         self.grad.zero_()
@@ -297,10 +301,14 @@ class FlatAdam:
         ws = reduce_workspace(self.grad.device)
         if self.clip_norm > 0:
             call("hold_sumsq", ptr(self.grad), self.n, ptr(self.sumsq), 0, ptr(ws))
-        call("hold_adam_step", ptr(self.flat), ptr(self.grad), ptr(self.m), ptr(self.v), self.n, self.n_low,
-             self.lr * self.pose_lr_scale, self.lr, self.betas[0], self.betas[1], self.eps, self.step_count,
-             float(grad_mul), self.clip_norm, ptr(self.sumsq) if self.clip_norm > 0 else None)
+        self.update(float(grad_mul))
         config.bump_weights_epoch()  # parameters changed behind torch's version counters: cached weight packs are stale
+
+    def update(self, grad_mul, n=None):
+        """Adam on the first ``n`` elements of the bucket (default: all of it)"""
+        call("hold_adam_step", ptr(self.flat), ptr(self.grad), ptr(self.m), ptr(self.v), self.n if n is None else n, self.n_low,
+             self.lr * self.pose_lr_scale, self.lr, self.betas[0], self.betas[1], self.eps, self.step_count,
+             grad_mul, self.clip_norm, ptr(self.sumsq) if self.clip_norm > 0 else None)
 
     def grad_norm(self):
         """global L2 norm of the (reduced) gradient bucket -- a host read, for logging / tests only."""
@@ -308,3 +316,79 @@ class FlatAdam:
         out = torch.zeros(1, device=self.grad.device)
         call("hold_sumsq", ptr(self.grad), self.n, ptr(out), 0, ptr(ws))
         return float(out.sqrt())
+
+
+def hidden_matrices(net, smallest=64):
+    """the trainable weight matrices of a model's layers (``weight``, or ``weight_v`` under weight norm) with both sides at least
+    ``smallest``: in the model's networks every layer but those that read few coordinates or write the colour"""
+    out = []
+    for module in net.modules():
+        if isinstance(module, torch.nn.Linear):
+            w = module.weight_v if hasattr(module, "weight_v") else module.weight
+            if w.requires_grad and w.dim() == 2 and min(w.shape) >= smallest and not any(w is o for o in out):
+                out.append(w)
+    return out
+
+
+class FlatMuon(FlatAdam):
+    """FlatAdam whose hidden weight matrices move by orthogonalised momentum (hold_amd.muon.muon_step) instead: the same bucket, the
+    same all-reduce and clip to a global norm, Adam for everything else.  ``matrices``: the parameters it applies to (default:
+    ``hidden_matrices(net)``); ``matrix_lr`` with ``scale`` "rms" has the size of an Adam step of that rate.  The momentum of a
+    matrix is kept in its place of ``m`` (the same running mean as Adam's first moment, with ``momentum`` for beta1); its place of
+    ``v`` stays zero."""
+
+    def __init__(self, net, lr=5e-4, matrix_lr=None, momentum=0.95, nesterov=True, weight_decay=0.0, scale="rms", steps=5, coefficients=None,
+                 matrices=None, **adam):
+        from . import muon
+        self.matrices = list(hidden_matrices(net) if matrices is None else matrices)
+        if any(p.dim() != 2 for p in self.matrices):
+            raise ValueError(f"FlatMuon: matrices are 2-D parameters, got {[tuple(p.shape) for p in self.matrices if p.dim() != 2]}")
+        self.matrix_lr, self.momentum, self.nesterov = float(lr if matrix_lr is None else matrix_lr), float(momentum), bool(nesterov)
+        self.weight_decay, self.scale, self.ns_steps = float(weight_decay), scale, int(steps)
+        self.coefficients = muon.QUINTIC if coefficients is None else coefficients
+        super().__init__(net, lr=lr, **adam)
+        self.n_adam = min([off for p, off in zip(self.params, self.offsets) if self._is_matrix(p)], default=self.n)
+
+    def _is_matrix(self, p):
+        return any(p is o for o in self.matrices)
+
+    def split(self, net):
+        low, main = split_params(net)
+        missing = [tuple(p.shape) for p in self.matrices if not any(p is o for o in main)]
+        if missing:
+            raise ValueError(f"FlatMuon: matrices have to be trainable parameters of the model outside its pose tables, got others of shapes {missing}")
+        return low, [p for p in main if not self._is_matrix(p)] + [p for p in main if self._is_matrix(p)]
+
+    def _views(self, flat):
+        return [flat[off:off + p.numel()].view(p.shape) for p, off in zip(self.params, self.offsets) if off >= self.n_adam]
+
+    def update(self, grad_mul):
+        from . import muon
+        if self.n_adam:
+            super().update(grad_mul, self.n_adam)
+        muon.muon_step(self._views(self.flat), self._views(self.grad), self._views(self.m), lr=self.matrix_lr, momentum=self.momentum,
+                       nesterov=self.nesterov, weight_decay=self.weight_decay, scale=self.scale, steps=self.ns_steps,
+                       coefficients=self.coefficients, grad_mul=grad_mul, clip_norm=self.clip_norm, sumsq=self.sumsq)
+
+    def named_state(self):
+        """Adam's per-parameter state of the parameters that Adam moves (a matrix has no second moment to hand over)"""
+        names = {id(p): n for n, p in self.net.named_parameters()}
+        return {n: st for n, st in super().named_state().items() if n not in {names[id(p)] for p in self.matrices}}
+
+    def export_to(self, opt):
+        """as FlatAdam's, without the matrices: a torch optimiser starts those anew"""
+        super().export_to(opt)
+        for p in self.matrices:
+            opt.state.pop(p, None)
+
+    HYPER = ("matrix_lr", "momentum", "nesterov", "weight_decay", "scale", "ns_steps", "coefficients")
+
+    def state_dict(self):
+        return {**super().state_dict(), "n_adam": self.n_adam, "muon": {k: getattr(self, k) for k in self.HYPER}}
+
+    def load_state_dict(self, sd):
+        if "muon" not in sd or int(sd["n_adam"]) != self.n_adam:
+            raise ValueError("FlatMuon.load_state_dict: the state of a FlatMuon over the same matrices is wanted")
+        super().load_state_dict(sd)
+        for k in self.HYPER:
+            setattr(self, k, sd["muon"][k])

@@ -735,8 +735,9 @@ typedef struct hold_muon_desc {
   const float* coef;                /* HOST, [3 steps] */
   const float* sumsq;               /* device scalar or NULL */
   void* workspace; int64_t workspace_bytes;
+  double lr, momentum, weight_decay; /* double: 1 - momentum and 1 - lr weight_decay are rounded once */
   int32_t n_items, steps, nesterov;
-  float lr, momentum, weight_decay, grad_mul, clip_norm, eps;
+  float grad_mul, clip_norm, eps;
 } hold_muon_desc;
 
 int hold_orthogonalize_workspace(const hold_ortho_desc* d, int64_t* bytes);

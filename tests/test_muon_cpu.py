@@ -117,3 +117,55 @@ def test_entry_points_refuse_bad_descriptors():
         setattr(i, name, keep)
     d.n_items = 0
     assert L.hold_muon_step(C.byref(d), None) == -1
+
+
+class _Net(torch.nn.Module):
+    """what the flat optimisers need of a model: .nodes[*].params (pose tables) and layers"""
+
+    def __init__(self):
+        super().__init__()
+        torch.manual_seed(3)
+        self.nodes = torch.nn.ModuleDict({"right": torch.nn.Module()})
+        self.nodes["right"].params = torch.nn.Embedding(5, 3)
+        self.first = torch.nn.Linear(3, 96)
+        self.hidden = torch.nn.utils.weight_norm(torch.nn.Linear(96, 64))
+        self.wide = torch.nn.Linear(64, 200, bias=False)
+        self.last = torch.nn.Linear(200, 3)
+
+
+def test_flat_muon_bucket_and_state():
+    from hold_amd.optim import FlatAdam, FlatMuon, hidden_matrices
+    net = _Net()
+    assert [tuple(p.shape) for p in hidden_matrices(net)] == [(64, 96), (200, 64)]
+    assert len(hidden_matrices(net, smallest=65)) == 0
+    values = {n: p.detach().clone() for n, p in net.named_parameters()}
+    a = FlatMuon(net, lr=1e-3, matrix_lr=0.02)
+    assert all(torch.equal(p, values[n]) for n, p in net.named_parameters())  # re-homed, unchanged
+    assert a.n_adam == a.offsets[-2] and [tuple(v.shape) for v in a._views(a.m)] == [(64, 96), (200, 64)]
+    assert all(v.data_ptr() == p.data_ptr() for v, p in zip(a._views(a.flat), a.matrices))
+    g = torch.Generator().manual_seed(1)
+    a.m.copy_(torch.randn(a.m.shape, generator=g))
+    a.step_count, a.momentum = 7, 0.9
+    b = FlatMuon(_Net(), lr=5e-4)
+    b.load_state_dict(a.state_dict())
+    assert torch.equal(b.m, a.m) and (b.step_count, b.momentum, b.matrix_lr, b.lr, b.scale) == (7, 0.9, 0.02, 1e-3, "rms")
+    assert set(a.named_state()) == {n for n, _ in net.named_parameters()} - {"hidden.weight_v", "wide.weight"}
+    assert not any(p in a.torch_optimizer().state for p in a.matrices)
+    for other in (FlatAdam(_Net(), lr=5e-4).state_dict(), FlatMuon(_Net(), lr=5e-4, matrices=[]).state_dict()):
+        with pytest.raises(ValueError):
+            b.load_state_dict(other)
+    net = _Net()
+    for bad in ([net.first.bias], [net.nodes["right"].params.weight], [torch.nn.Parameter(torch.zeros(4, 4))]):
+        with pytest.raises(ValueError):
+            FlatMuon(net, matrices=bad)
+
+
+def test_flat_muon_finds_the_models_matrices():
+    import hold_amd
+    from parity_common import syn
+    from hold_amd.optim import hidden_matrices
+    sc = syn.make_scene(n_frames=4)
+    net = hold_amd.build_from_scene(sc, syn.make_state_dict(sc), device="cpu")
+    names = {id(p): n for n, p in net.named_parameters()}
+    got = [names[id(p)] for p in hidden_matrices(net)]
+    assert len(got) >= 30 and all(n.endswith(("weight", "weight_v")) for n in got) and not any(".params." in n for n in got)

@@ -221,3 +221,88 @@ def test_other_stream_and_captured_graphs():
         assert torch.equal(y, orthogonalize(x))
         muon_step([p2], [g], [m2], lr=0.1)
         assert torch.equal(p, p2) and torch.equal(m, m2)
+
+
+class _GatedNet(torch.nn.Module):
+    """two gated layers between a first and a last linear one, as a coordinate network has them; .nodes as the optimiser wants it"""
+
+    def __init__(self):
+        super().__init__()
+        torch.manual_seed(4)
+        self.nodes = torch.nn.ModuleDict()
+        self.first = torch.nn.Linear(3, 96)
+        self.gates = torch.nn.ModuleList([torch.nn.Linear(96, 128), torch.nn.Linear(128, 96)])
+        self.ups = torch.nn.ModuleList([torch.nn.Linear(96, 128), torch.nn.Linear(128, 96)])
+        self.last = torch.nn.Linear(96, 3)
+
+    def forward(self, x, layer):
+        h = torch.sin(self.first(x))
+        for g, u in zip(self.gates, self.ups):
+            h = layer(h, g.weight, u.weight, g.bias, u.bias)
+        return self.last(h)
+
+
+def _layer64(x, wg, wu, bg, bu):
+    return torch.nn.functional.silu(x @ wg.T + bg) * (x @ wu.T + bu)
+
+
+def test_gated_layers_trained_by_orthogonalised_momentum():
+    """three steps of a network of gated layers under FlatMuon: every gradient against the formula's in 64 bits, every update against the
+    optimiser's formulas applied to the gradients that it was given.  Gradients: float32 layers in a row, each adding some 2^-18 of
+    its terms (the layer's own bound), six of them with cancellation: 2^-12 of a gradient's norm"""
+    from hold_amd.gated import gated_linear
+    from hold_amd.optim import FlatMuon
+    net, twin = _GatedNet().to(DEV), _GatedNet().double()
+    opt = FlatMuon(net, lr=1e-3, matrix_lr=0.02, momentum=0.9, weight_decay=0.01, clip_norm=0.5)
+    assert len(opt.matrices) == 4
+    gen = torch.Generator().manual_seed(8)
+    for k in range(3):
+        x, y = torch.randn(700, 3, generator=gen), torch.randn(700, 3, generator=gen)
+        with torch.no_grad():
+            for p, q in zip(net.parameters(), twin.parameters()):
+                q.copy_(p)
+        opt.zero_grad()
+        ((net(x.to(DEV), gated_linear) - y.to(DEV)) ** 2).mean().backward()
+        opt.gather_stray_grads()
+        grads = torch.autograd.grad(((twin(x.double(), _layer64) - y.double()) ** 2).mean(), list(twin.parameters()))
+        for (n, p), g in zip(net.named_parameters(), grads):
+            assert float((p.grad.cpu().double() - g).norm()) <= 2.0 ** -12 * float(g.norm()), n
+        before, m0, g0 = opt.flat.clone(), opt.m.clone(), opt.grad.clone()
+        f = min(1.0, 0.5 / (opt.grad_norm() + 1e-6))
+        opt.step()
+        for p, c, d, e, m in zip(opt.matrices, opt._views(before), opt._views(m0), opt._views(g0), opt._views(opt.m)):
+            s = 0.2 * max(p.shape) ** 0.5
+            check_step(p.detach(), m, c, d, step64(c, e, d, 0.02, 0.9, True, 0.01, s, f), 0.02, s, f)
+        n = opt.n_adam
+        b1, b2 = opt.betas
+        m, v = (1 - b1) * g0[:n].double() * f + b1 * m0[:n].double(), opt.v[:n].double()  # v: as the step left it
+        want = before[:n].double() - 1e-3 * (m / (1 - b1 ** (k + 1))) / ((v / (1 - b2 ** (k + 1))).sqrt() + opt.eps)
+        assert float((opt.flat[:n].double() - want).abs().max()) <= 1e-6 and float(opt.v[n:].abs().max()) == 0.0
+
+
+def test_flat_muon_on_the_model():
+    """a step of the scene's model: Adam's part has the bits of FlatAdam, the matrices those of muon_step"""
+    from parity_common import hip_net, setup
+    from hold_amd.muon import muon_step
+    from hold_amd.optim import FlatAdam, FlatMuon
+    sc, sd_np, _, _ = setup()
+    a, b = hip_net(sc, sd_np, train=True), hip_net(sc, sd_np, train=True)
+    muon, adam = FlatMuon(a, lr=5e-4, matrix_lr=1e-3, clip_norm=0.0), FlatAdam(b, lr=5e-4, clip_norm=0.0)
+    other, names = dict(b.named_parameters()), {id(p): n for n, p in a.named_parameters()}
+    assert len(muon.matrices) >= 30
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    p, m = [t.clone() for t in muon._views(muon.flat)], [t.clone() for t in muon._views(muon.m)]
+    for _ in range(2):
+        muon.zero_grad()
+        adam.zero_grad()
+        for q in muon.params:
+            q.grad.copy_(torch.randn(q.shape, device=DEV, generator=gen))
+            other[names[id(q)]].grad.copy_(q.grad)
+        g = [t.clone() for t in muon._views(muon.grad)]
+        muon.step()
+        adam.step()
+        muon_step(p, g, m, lr=1e-3, scale="rms")
+        for q in muon.params:
+            if not any(q is o for o in muon.matrices):
+                assert torch.equal(q, other[names[id(q)]]), names[id(q)]
+        assert all(torch.equal(x, y) for x, y in zip(p, muon._views(muon.flat))) and all(torch.equal(x, y) for x, y in zip(m, muon._views(muon.m)))
