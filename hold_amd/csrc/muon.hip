@@ -28,7 +28,7 @@ struct Item {
   void* m;        // momentum, or null
   void* p;        // the result, or the parameter
   int64_t stride; // elements from one matrix of the item to the next, in all three
-  int64_t x, c;   // this item's first X and first A, in elements of the workspace's halves
+  int64_t x;      // this item's first X, in elements of the workspace
   int rows, cols, ldg, ldm, ldp, count;
   int part, nb;   // first partial sum, partial sums a matrix
   float gain;     // the step's factor: learning rate times the scale of the matrix's shape
@@ -42,14 +42,31 @@ struct Step {
   int nesterov, dtype;
   const float* sumsq;
 };
-// per-launch tile counts: item k's tiles begin at first[k]
-struct Tiles {
+// the items' blocks of a launch begin at first[k]
+struct Firsts {
   int first[MAXI + 1];
 };
+// Matrices of equal shape lie one after the other in the workspace: the products in between know them as classes only, and a call
+// whose matrices all have one shape (ONE) finds everything in the first bytes of its arguments instead of a chain of loads
+struct Class {
+  int64_t x, c;      // the class's first X and first A, in elements
+  int m, n, mp, np;  // the smaller and the larger side, and both rounded up to 8
+  int mats, item;    // matrices, the first one's item
+  int tile;          // first tile in the launch
+};
+struct Classes {
+  Class k[MAXI];
+  int n;
+};
+struct OneClass {
+  Class k[1];
+  int n;
+};
 
-__device__ __forceinline__ int item_of(const Tiles& t, int n, int id) {
+template <class F>
+__device__ __forceinline__ int last_below(int n, int id, F first) {
   int k = 0;
-  while (k + 1 < n && id >= t.first[k + 1]) ++k;
+  while (k + 1 < n && id >= first(k + 1)) ++k;
   return k;
 }
 __host__ __device__ __forceinline__ int up8(int v) { return (v + 7) / 8 * 8; }
@@ -78,28 +95,80 @@ __device__ __forceinline__ float update_of(const Item& it, const Step& s, float 
   return s.nesterov ? s.rest * (g * f) + s.mu * m : m;
 }
 
-// momentum and the partial sums of squares, 256 threads on an equal share of a matrix's elements; partial sums are added in a fixed order
-__global__ __launch_bounds__(256) void ns_norm_kernel(Items a, Tiles t, Step s, double* part) {
-  const int k = item_of(t, a.n, blockIdx.x);
+// Momentum and the partial sums of squares: a block takes an equal share of a matrix's elements, the partial sums are added in a fixed
+// order.  Matrices without gaps between rows, on 16-byte boundaries, go by 16 bytes, two of each operand in flight per thread
+// (36 matrices of 256 x 256: 46.7 us element by element).
+__global__ __launch_bounds__(256) void ns_norm_kernel(Items a, Firsts t, Step s, double* part) {
+  const int k = last_below(a.n, blockIdx.x, [&](int i) { return t.first[i]; });
   const Item& it = a.it[k];
   const int q = blockIdx.x - t.first[k], mat = q / it.nb, blk = q % it.nb;
-  const int64_t b = mat * it.stride, n = (int64_t)it.rows * it.cols, per = (n + it.nb - 1) / it.nb;
-  const int64_t end = (blk + 1) * per < n ? (blk + 1) * per : n;
+  const int64_t b = mat * it.stride, n = (int64_t)it.rows * it.cols, per = ((n + it.nb - 1) / it.nb + 7) / 8 * 8;
+  const int64_t begin = blk * per, end = begin + per < n ? begin + per : n;
   const float f = it.m ? grad_scale(s) : 1.f;
   double sum = 0.;
-  const bool lin = it.ldg == it.cols && it.ldm == it.cols;
-  for (int64_t e = blk * per + threadIdx.x; e < end; e += 256) {
-    const int r = lin ? 0 : (int)(e / it.cols);
-    const int64_t c = e - (int64_t)r * it.cols;
-    const float g = value(it.g, b + (int64_t)r * it.ldg + c, s.dtype);
+  auto one = [&](float g, float& m) {
     float u = g;
     if (it.m) {
-      float* mp = (float*)it.m + b + (int64_t)r * it.ldm + c;
-      const float gf = g * f, m = s.mu * *mp + s.rest * gf;
-      *mp = m;
+      const float gf = g * f;
+      m = s.mu * m + s.rest * gf;
       u = s.nesterov ? s.rest * gf + s.mu * m : m;
     }
     sum += (double)u * u;
+  };
+  const bool lin = it.ldg == it.cols && (!it.m || it.ldm == it.cols);
+  float* mp = (float*)it.m + b;
+  if (lin && s.dtype == HOLD_MUON_F32 && ((uintptr_t)it.g | (uintptr_t)it.m | (uint64_t)(4 * b)) % 16 == 0) {
+    const float* gp = (const float*)it.g + b;
+    const int64_t whole = end & ~(int64_t)3;
+    for (int64_t e = begin + 4 * threadIdx.x; e < whole; e += 2048) {
+      const bool two = e + 1024 < whole;
+      f32x4 g0 = *(const f32x4*)(gp + e), g1 = two ? *(const f32x4*)(gp + e + 1024) : f32x4{0.f, 0.f, 0.f, 0.f};
+      f32x4 m0 = {0.f, 0.f, 0.f, 0.f}, m1 = m0;
+      if (it.m) {
+        m0 = *(const f32x4*)(mp + e);
+        if (two) m1 = *(const f32x4*)(mp + e + 1024);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = m0[r], y = m1[r];
+        one(g0[r], x);
+        if (two) one(g1[r], y);
+        m0[r] = x;
+        m1[r] = y;
+      }
+      if (it.m) {
+        *(f32x4*)(mp + e) = m0;
+        if (two) *(f32x4*)(mp + e + 1024) = m1;
+      }
+    }
+    const int64_t e = whole + threadIdx.x;
+    if (e >= begin && e < end) {
+      float m = it.m ? mp[e] : 0.f;
+      one(gp[e], m);
+      if (it.m) mp[e] = m;
+    }
+  } else if (lin && s.dtype != HOLD_MUON_F32 && ((uintptr_t)it.g | (uint64_t)(2 * b)) % 16 == 0) {
+    const uint16_t* gp = (const uint16_t*)it.g + b;
+    const int64_t whole = end & ~(int64_t)7;
+    for (int64_t e = begin + 8 * threadIdx.x; e < whole; e += 2048) {
+      const u32x4 w = *(const u32x4*)(gp + e);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const uint16_t h = (uint16_t)(w[r >> 1] >> (16 * (r & 1)));
+        float m = 0.f;
+        one(s.dtype == HOLD_MUON_BF16 ? bf16_value(h) : (float)__builtin_bit_cast(_Float16, h), m);
+      }
+    }
+    const int64_t e = whole + threadIdx.x;
+    float m = 0.f;
+    if (e >= begin && e < end) one(value(gp, e, s.dtype), m);
+  } else {
+    for (int64_t e = begin + threadIdx.x; e < end; e += 256) {
+      const int64_t r = lin ? 0 : e / it.cols, c = e - r * it.cols;
+      float m = it.m ? mp[r * it.ldm + c] : 0.f;
+      one(value(it.g, b + r * it.ldg + c, s.dtype), m);
+      if (it.m) mp[r * it.ldm + c] = m;
+    }
   }
   __shared__ double w[4];
 #pragma unroll
@@ -110,8 +179,8 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Items a, Tiles t, Step s, 
 }
 
 // X0 as limbs [min][max] (rounded up to 8, zeros behind), scaled by 2^xs: 64 x 64 tiles of the source through LDS, transposed where it is tall
-__global__ __launch_bounds__(256) void ns_load_kernel(Items a, Tiles t, Step s, const double* part, uint16_t* ws, int64_t limb, int xs) {
-  const int k = item_of(t, a.n, blockIdx.x);
+__global__ __launch_bounds__(256) void ns_load_kernel(Items a, Firsts t, Step s, const double* part, uint16_t* ws, int64_t limb, int xs) {
+  const int k = last_below(a.n, blockIdx.x, [&](int i) { return t.first[i]; });
   const Item& it = a.it[k];
   const bool tall = it.rows > it.cols;
   const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols, mp = up8(m), np = up8(n);
@@ -177,78 +246,119 @@ struct NsArgs {
   int64_t xlimb, climb;
   float a, b, c;      // POLY, already in the scales of its operands and its result
   int shift;          // exponent from the accumulated sum to the stored limbs
-  int last;           // APPLY: write the result instead of the next X
 };
 
-template <int KIND, int T, int WM, int WN, int S>
-__global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(Items a, Tiles t, NsArgs s, Step st) {
+struct NoItems {};
+template <bool LAST> struct ItemArg { typedef NoItems type; };
+template <> struct ItemArg<true> { typedef Items type; };
+
+// GRAM and POLY: only the tiles on and below the diagonal; what is right of it is written as their mirror image, turned in LDS
+template <int KIND, int T, int WM, int WN, int S, bool PHASED, bool LAST, class CLASSES>
+__global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs s, Step st, typename ItemArg<LAST>::type items) {
   using Cr = Core<MODE_F16X3, KC, KIND == APPLY ? KS : KC, T, T, 1, WM, WN, S>;
-  __shared__ __align__(1024) char smem[Cr::LDS];
+  constexpr int PITCH = T + 8, TURN = KIND == APPLY ? 0 : T * PITCH * 2;
+  __shared__ __align__(1024) char smem[Cr::LDS > TURN ? Cr::LDS : TURN];
   // the tile list is cut into an eighth for each XCD, as tile_of does: neighbours share a matrix
   const int total = gridDim.x, qq = total / 8, rr = total % 8, xcd = blockIdx.x % 8, ii = blockIdx.x / 8;
   const int id = xcd * qq + (xcd < rr ? xcd : rr) + ii;
-  const int k = item_of(t, a.n, id);
-  const Item& it = a.it[k];
-  const bool tall = it.rows > it.cols;
-  const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols, mp = up8(m), np = up8(n);
-  const int tm = (mp + T - 1) / T, tn = KIND == APPLY ? (np + T - 1) / T : tm;
-  const int q = id - t.first[k], mat = q / (tm * tn), tile = q % (tm * tn);
-  // bands of 8 row tiles, column by column
-  const int per = 8 * tn, band = tile / per, f0 = band * 8, h = tm - f0 < 8 ? tm - f0 : 8, i0 = (f0 + (tile - band * per) % h) * T, j0 = (tile - band * per) / h * T;
-  const int64_t xo = it.x + (int64_t)mat * mp * np, co = it.c + (int64_t)mat * mp * mp;
+  constexpr bool ONE = sizeof(CLASSES) == sizeof(OneClass);
+  const int k = ONE ? 0 : last_below(cl.n, id, [&](int i) { return cl.k[i].tile; });
+  const Class& c = cl.k[k];
+  const int m = c.m, n = c.n, mp = c.mp, np = c.np, tm = (mp + T - 1) / T, tn = KIND == APPLY ? (np + T - 1) / T : tm;
+  const int per = KIND == APPLY ? tm * tn : tm * (tm + 1) / 2, q = id - c.tile, mat = q / per, tile = q % per;
+  int i0, j0;
+  if (KIND == APPLY) {  // bands of 8 row tiles, column by column
+    const int w = 8 * tn, band = tile / w, f0 = band * 8, h = tm - f0 < 8 ? tm - f0 : 8;
+    i0 = (f0 + (tile - band * w) % h) * T;
+    j0 = (tile - band * w) / h * T;
+  } else {  // row bi of the triangle begins at tile bi (bi + 1) / 2
+    int bi = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+    while (bi * (bi + 1) / 2 > tile) --bi;
+    while ((bi + 1) * (bi + 2) / 2 <= tile) ++bi;
+    i0 = bi * T;
+    j0 = (tile - bi * (bi + 1) / 2) * T;
+  }
+  const int64_t xo = c.x + (int64_t)mat * mp * np, co = c.c + (int64_t)mat * mp * mp;
   typename Cr::Acc acc;
   Cr::zero(acc);
+  Operand A, B[1];
   if (KIND == GRAM) {
-    const Operand A = {s.x + xo + (int64_t)i0 * np, s.xlimb, np, mp - i0, np};
-    const Operand B[1] = {{s.x + xo + (int64_t)j0 * np, s.xlimb, np, mp - j0, np}};
-    Cr::run(smem, A, B, acc);
+    A = Operand{s.x + xo + (int64_t)i0 * np, s.xlimb, np, mp - i0, np};
+    B[0] = Operand{s.x + xo + (int64_t)j0 * np, s.xlimb, np, mp - j0, np};
   } else if (KIND == POLY) {
-    const Operand A = {s.am + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
-    const Operand B[1] = {{s.am + co + (int64_t)j0 * mp, s.climb, mp, mp - j0, mp}};
-    Cr::run(smem, A, B, acc);
+    A = Operand{s.am + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
+    B[0] = Operand{s.am + co + (int64_t)j0 * mp, s.climb, mp, mp - j0, mp};
   } else {
-    const Operand A = {s.cm + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
-    const Operand B[1] = {{s.x + xo + j0, s.xlimb, np, np - j0, mp}};
-    Cr::run(smem, A, B, acc);
+    A = Operand{s.cm + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
+    B[0] = Operand{s.x + xo + j0, s.xlimb, np, np - j0, mp};
   }
+  if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
+  else Cr::run(smem, A, B, acc);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  const int64_t b = mat * it.stride;
+  uint16_t* sym = (KIND == GRAM ? s.am : s.cm) + co;
+  uint16_t* turn = (uint16_t*)smem;
 #pragma unroll
   for (int mi = 0; mi < Cr::MI; ++mi) {
-    const int i = i0 + wm * (T / WM) + 16 * mi + (lane & 15);
+    const int it = wm * (T / WM) + 16 * mi + (lane & 15), i = i0 + it;
 #pragma unroll
     for (int ni = 0; ni < Cr::NI; ++ni) {
-      const int j = j0 + wn * (T / WN) + 16 * ni + 4 * (lane >> 4);
-      if (i >= mp || j >= (KIND == APPLY ? np : mp)) continue;
-      f32x4 v = acc[0][mi][ni];
+      const int jt = wn * (T / WN) + 16 * ni + 4 * (lane >> 4), j = j0 + jt;
+      f32x4& v = acc[0][mi][ni];
+      const bool in = i < mp && j < (KIND == APPLY ? np : mp);
       if (KIND == GRAM) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], s.shift);
-        store_limbs(s.am + co + (int64_t)i * mp + j, s.climb, v);
+        if (in) store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
       } else if (KIND == POLY) {
-        const f32x4 u = load_limbs(s.am + co + (int64_t)i * mp + j, s.climb);
+        if (in) {
+          const f32x4 u = load_limbs(s.am + co + (int64_t)i * mp + j, s.climb);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = fmaf(s.c, v[r], s.b * u[r]) + (i == j + r ? s.a : 0.f);
-        store_limbs(s.cm + co + (int64_t)i * mp + j, s.climb, v);
+          for (int r = 0; r < 4; ++r) v[r] = fmaf(s.c, v[r], s.b * u[r]) + (i == j + r ? s.a : 0.f);
+          store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
+        }
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], s.shift);
-        if (!s.last) {
-          store_limbs(s.y + xo + (int64_t)i * np + j, s.xlimb, v);
+        if constexpr (!LAST) {
+          if (in) store_limbs(s.y + xo + (int64_t)i * np + j, s.xlimb, v);
         } else if (i < m) {
+          const bool list = items.it[c.item].count == 1;  // a class is a run of single items, or one item of many matrices
+          const Item& d = items.it[c.item + (list ? mat : 0)];
+          const bool tall = d.rows > d.cols;
+          const int64_t b = list ? 0 : mat * d.stride;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if (j + r >= n) continue;
-            const int64_t at = b + (tall ? (int64_t)(j + r) * it.ldp + i : (int64_t)i * it.ldp + j + r);
-            if (it.m) {
-              float* p = (float*)it.p + at;
-              *p = *p * st.decay - it.gain * v[r];
+            const int64_t at = b + (tall ? (int64_t)(j + r) * d.ldp + i : (int64_t)i * d.ldp + j + r);
+            if (d.m) {
+              float* p = (float*)d.p + at;
+              *p = *p * st.decay - d.gain * v[r];
             } else {
-              put(it.p, at, st.dtype, v[r]);
+              put(d.p, at, st.dtype, v[r]);
             }
           }
         }
       }
+    }
+  }
+  if (KIND != APPLY && i0 != j0) {  // limb by limb: [j][i] in LDS, whole rows out
+#pragma unroll 1
+    for (int l = 0; l < 2; ++l) {
+#pragma unroll
+      for (int mi = 0; mi < Cr::MI; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < Cr::NI; ++ni)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const Split y = split16(acc[0][mi][ni][r]);
+            turn[(wn * (T / WN) + 16 * ni + 4 * (lane >> 4) + r) * PITCH + wm * (T / WM) + 16 * mi + (lane & 15)] = l ? y.lo : y.hi;
+          }
+      __syncthreads();
+      for (int e = threadIdx.x; e < T * T / 8; e += 64 * WM * WN) {
+        const int r = e / (T / 8), q8 = e % (T / 8) * 8;
+        if (j0 + r < mp && i0 + q8 < mp) *(u32x4*)(sym + (int64_t)(j0 + r) * mp + i0 + q8 + (l ? s.climb : 0)) = *(const u32x4*)(turn + r * PITCH + q8);
+      }
+      __syncthreads();
     }
   }
 }
@@ -298,17 +408,31 @@ inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 struct Room {
   int64_t part, x, y, am, cm, xn, cn, bytes;
 };
-Room room(Items& a) {
+// sorts the items by shape, finds the classes and lays out the workspace
+Room room(Items& a, Classes& cl) {
+  auto small = [](const Item& i) { return i.rows < i.cols ? i.rows : i.cols; };
+  auto large = [](const Item& i) { return i.rows < i.cols ? i.cols : i.rows; };
+  for (int k = 1; k < a.n; ++k) {  // by insertion: equal shapes keep their order
+    const Item it = a.it[k];
+    int q = k;
+    while (q > 0 && (small(a.it[q - 1]) > small(it) || (small(a.it[q - 1]) == small(it) && large(a.it[q - 1]) > large(it)))) {
+      a.it[q] = a.it[q - 1];
+      --q;
+    }
+    a.it[q] = it;
+  }
   Room r = {};
   int64_t parts = 0, xn = 0, cn = 0;
+  cl.n = 0;
   for (int k = 0; k < a.n; ++k) {
     Item& it = a.it[k];
-    const int64_t mp = up8(it.rows < it.cols ? it.rows : it.cols), np = up8(it.rows < it.cols ? it.cols : it.rows), n = (int64_t)it.rows * it.cols;
-    const int64_t nb = (n + 16383) / 16384;
-    it.nb = (int)(nb > 1024 ? 1024 : nb);
+    const int m = small(it), n = large(it);
+    const int64_t mp = up8(m), np = up8(n), nb = ((int64_t)m * n + 4095) / 4096;
+    it.nb = (int)(nb > 512 ? 512 : nb);
     it.part = (int)parts;
     it.x = xn;
-    it.c = cn;
+    if (cl.n && it.count == 1 && a.it[cl.k[cl.n - 1].item].count == 1 && cl.k[cl.n - 1].m == m && cl.k[cl.n - 1].n == n) ++cl.k[cl.n - 1].mats;
+    else cl.k[cl.n++] = Class{xn, cn, m, n, (int)mp, (int)np, it.count, k, 0};
     parts += (int64_t)it.nb * it.count;
     xn += mp * np * it.count;
     cn += mp * mp * it.count;
@@ -327,48 +451,73 @@ Room room(Items& a) {
 }
 
 template <int KIND>
-int launch(const Items& a, const NsArgs& s, const Step& st, hipStream_t stream) {
-  auto tiles = [&](int T, Tiles& t) {
-    int64_t n = 0;
-    for (int k = 0; k < a.n; ++k) {
-      const Item& it = a.it[k];
-      const int64_t mp = up8(it.rows < it.cols ? it.rows : it.cols), np = up8(it.rows < it.cols ? it.cols : it.rows);
-      t.first[k] = (int)n;
-      n += ((mp + T - 1) / T) * ((KIND == APPLY ? np + T - 1 : mp + T - 1) / T) * it.count;
-      if (n > (1 << 30)) return (int64_t)-1;
-    }
-    t.first[a.n] = (int)n;
-    return n;
-  };
-  Tiles t = {};
-  int64_t n = tiles(128, t);
-  if (n < 0) return HOLD_E_ARG;
-  if (n >= 256) {
-    hipLaunchKernelGGL((ns_mma_kernel<KIND, 128, 2, 2, 2>), dim3((unsigned)n), dim3(256), 0, stream, a, t, s, st);
-  } else {
-    n = tiles(64, t);
-    if (n < 0) return HOLD_E_ARG;
-    hipLaunchKernelGGL((ns_mma_kernel<KIND, 64, 2, 2, 8>), dim3((unsigned)n), dim3(256), 0, stream, a, t, s, st);
+int64_t count_tiles(Classes& cl, int T) {
+  int64_t n = 0;
+  for (int k = 0; k < cl.n; ++k) {
+    Class& c = cl.k[k];
+    c.tile = (int)n;
+    const int64_t tm = (c.mp + T - 1) / T, tn = (c.np + T - 1) / T;
+    n += (KIND == APPLY ? tm * tn : tm * (tm + 1) / 2) * c.mats;
+    if (n > (1 << 30)) return -1;
   }
+  return n;
+}
+
+template <int KIND, int T, int WM, int WN, int S, bool PHASED, bool LAST>
+void launch_tiles(const Classes& cl, const NsArgs& s, const Step& st, const Items& a, unsigned n, hipStream_t stream) {
+  typename ItemArg<LAST>::type items;
+  if constexpr (LAST) items = a;
+  if (cl.n == 1) {
+    const OneClass one = {{cl.k[0]}, 1};
+    hipLaunchKernelGGL((ns_mma_kernel<KIND, T, WM, WN, S, PHASED, LAST, OneClass>), dim3(n), dim3(64 * WM * WN), 0, stream, one, s, st, items);
+  } else {
+    hipLaunchKernelGGL((ns_mma_kernel<KIND, T, WM, WN, S, PHASED, LAST, Classes>), dim3(n), dim3(64 * WM * WN), 0, stream, cl, s, st, items);
+  }
+}
+
+// The tile size by the time of the launch in units of one 256 x 256 tile per compute unit: rounds of blocks over the 256 units times a
+// block's share.  256 and 192: one block a unit; 128: two, 64: four; the smaller tiles' lower rates (more LDS reads and loads a product)
+// are measured on 4096^3: 1310 / 1400 (192, counted without its idle units) / 1135 / 620 TFLOP/s of limb products.
+template <int KIND, bool LAST>
+int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStream_t stream) {
+  const int T[4] = {256, 192, 128, 64}, at_once[4] = {256, 256, 512, 1024};
+  const double cost[4] = {1., 0.55, 0.58, 0.55};  // of a full round
+  int best = -1;
+  double least = 0.;
+  for (int k = 0; k < 4; ++k) {
+    const int64_t n = count_tiles<KIND>(cl, T[k]);
+    if (n < 0) continue;
+    const int64_t rounds = (n + at_once[k] - 1) / at_once[k], per_unit = (n + 255) / 256;
+    // a round that does not fill the units' places is as long as its blocks alone, half of a full one for 128, a third for 64
+    double t = cost[k] * (double)rounds;
+    if (rounds == 1 && k >= 2) t = cost[k] * (0.35 + 0.65 * (double)per_unit / (k == 2 ? 2. : 4.));
+    if (best < 0 || t < least) { best = k; least = t; }
+  }
+  if (best < 0) return HOLD_E_ARG;
+  const unsigned n = (unsigned)count_tiles<KIND>(cl, T[best]);
+  if (best == 0) launch_tiles<KIND, 256, 4, 4, 2, true, LAST>(cl, s, st, a, n, stream);
+  else if (best == 1) launch_tiles<KIND, 192, 3, 4, 2, false, LAST>(cl, s, st, a, n, stream);
+  else if (best == 2) launch_tiles<KIND, 128, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
+  else launch_tiles<KIND, 64, 2, 2, 4, false, LAST>(cl, s, st, a, n, stream);
   return HOLD_OK;
 }
 
 int run_group(Items& a, const Step& st, const float* coef, int steps, char* ws, hipStream_t stream) {
   Bounds bo;
   if (!follow(coef, steps, bo)) return HOLD_E_ARG;
-  const Room r = room(a);
+  Classes cl;
+  const Room r = room(a, cl);
   double* part = (double*)(ws + r.part);
   uint16_t* x = (uint16_t*)(ws + r.x);
   uint16_t* y = (uint16_t*)(ws + r.y);
-  Tiles tn = {}, tl = {};
+  Firsts tn = {}, tl = {};
   int64_t nn = 0, nl = 0;
   for (int k = 0; k < a.n; ++k) {
     const Item& it = a.it[k];
-    const int64_t mp = up8(it.rows < it.cols ? it.rows : it.cols), np = up8(it.rows < it.cols ? it.cols : it.rows);
     tn.first[k] = (int)nn;
     tl.first[k] = (int)nl;
     nn += (int64_t)it.nb * it.count;
-    nl += ((mp + 63) / 64) * ((np + 63) / 64) * it.count;
+    nl += (int64_t)((up8(it.rows) + 63) / 64) * ((up8(it.cols) + 63) / 64) * it.count;
     if (nn > (1 << 30) || nl > (1 << 30)) return HOLD_E_ARG;
   }
   hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)nn), dim3(256), 0, stream, a, tn, st, part);
@@ -378,23 +527,26 @@ int run_group(Items& a, const Step& st, const float* coef, int steps, char* ws, 
   s.cm = (uint16_t*)(ws + r.cm);
   s.xlimb = r.xn;
   s.climb = r.cn;
-  for (int k = 0; k < steps; ++k) {
+  int rc = HOLD_OK;
+  for (int k = 0; k < steps && rc == HOLD_OK; ++k) {
     s.x = x;
     s.y = y;
     s.shift = bo.as[k] - 2 * bo.xs[k];
-    if (launch<GRAM>(a, s, st, stream) != HOLD_OK) return HOLD_E_ARG;
+    rc = launch<GRAM, false>(cl, s, st, a, stream);
+    if (rc != HOLD_OK) break;
     s.a = (float)ldexp((double)coef[3 * k], bo.cs[k]);
     s.b = (float)ldexp((double)coef[3 * k + 1], bo.cs[k] - bo.as[k]);
     s.c = (float)ldexp((double)coef[3 * k + 2], bo.cs[k] - 2 * bo.as[k]);
-    if (launch<POLY>(a, s, st, stream) != HOLD_OK) return HOLD_E_ARG;
-    s.last = k + 1 == steps;
-    s.shift = (s.last ? 0 : bo.xs[k + 1]) - bo.cs[k] - bo.xs[k];
-    if (launch<APPLY>(a, s, st, stream) != HOLD_OK) return HOLD_E_ARG;
+    rc = launch<POLY, false>(cl, s, st, a, stream);
+    if (rc != HOLD_OK) break;
+    const bool last = k + 1 == steps;
+    s.shift = (last ? 0 : bo.xs[k + 1]) - bo.cs[k] - bo.xs[k];
+    rc = last ? launch<APPLY, true>(cl, s, st, a, stream) : launch<APPLY, false>(cl, s, st, a, stream);
     uint16_t* z = x;
     x = y;
     y = z;
   }
-  return ok();
+  return rc == HOLD_OK ? ok() : rc;
 }
 
 bool sizes_ok(int64_t rows, int64_t cols, int64_t count) {
@@ -431,15 +583,17 @@ bool some_items(const hold_muon_desc* d, int first, Items& a) {
 
 extern "C" int hold_orthogonalize_workspace(const hold_ortho_desc* d, int64_t* bytes) {
   Items a;
+  Classes cl;
   if (!one_item(d, a) || !bytes) return HOLD_E_ARG;
-  *bytes = room(a).bytes;
+  *bytes = room(a, cl).bytes;
   return HOLD_OK;
 }
 
 extern "C" int hold_orthogonalize(const hold_ortho_desc* d, hold_stream_t stream) {
   Items a;
+  Classes cl;
   if (!one_item(d, a) || !d->x || !d->out || !d->coef || d->steps < 1 || d->steps > 32 || d->dtype < 0 || d->dtype > 2 || !(d->eps >= 0.f)) return HOLD_E_ARG;
-  if (!d->workspace || room(a).bytes > d->workspace_bytes) return HOLD_E_ARG;
+  if (!d->workspace || room(a, cl).bytes > d->workspace_bytes) return HOLD_E_ARG;
   a.it[0].g = d->x;
   a.it[0].p = d->out;
   Step st = {};
@@ -453,8 +607,9 @@ extern "C" int hold_muon_workspace(const hold_muon_desc* d, int64_t* bytes) {
   *bytes = 0;
   for (int first = 0; first < d->n_items; first += MAXI) {
     Items a;
+    Classes cl;
     if (!some_items(d, first, a)) return HOLD_E_ARG;
-    const int64_t n = room(a).bytes;
+    const int64_t n = room(a, cl).bytes;
     if (n > *bytes) *bytes = n;
   }
   return HOLD_OK;

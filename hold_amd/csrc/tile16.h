@@ -48,11 +48,6 @@ struct Operand {
   int64_t k;     // k's of the operand (KC: rounded up to 8, the last ones zeros); the shorter of the two ends in zeros
 };
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, int64_t bytes) {
-  const int64_t n = bytes < 0 ? 0 : (bytes > 0x7ffffff0ll ? 0x7ffffff0ll : bytes);
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)n, 0x00020000);
-}
-
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // LDS tile of R rows x BK k's of one limb
@@ -63,9 +58,11 @@ struct Tile {
   static constexpr int C = RB / 16;                     // 16-byte chunks of a tile row
   static constexpr int BYTES = RB * NR;
   static constexpr int PIECES = BYTES / 1024;           // wave-wide 16-byte loads
-  static_assert(C >= 4 && BYTES % 1024 == 0, "tile row of at least 64 bytes");
+  static_assert((LAY == KC ? C == 4 || C == 8 : C >= 8) && BYTES % 1024 == 0, "tile rows of 64 or 128 bytes (KC), 128 and more (KS)");
   static __device__ __forceinline__ int swz(int row) {
-    if (LAY == KC) return C >= 16 ? (row & 15) : C == 8 ? ((row >> 1) & 7) : ((row >> 2) & 3);
+    // a 16-byte read is served 16 lanes at a time: of two neighbouring 16-lane groups (two chunks), rows 0-3 and 12-15 of one with
+    // rows 4-11 of the other
+    if (LAY == KC) return C == 8 ? ((row >> 1) & 7) : (-(row >> 2) & 3);
     return C >= 16 ? 2 * ((row & 3) | ((row >> 1) & 4)) : 2 * (((row >> 1) & 1) | ((row >> 2) & 2));
   }
 };
@@ -75,7 +72,7 @@ template <int LAY, int R, int BK, int NW>
 struct Loader {
   using T = Tile<LAY, R, BK>;
   static constexpr int N = (T::PIECES + NW - 1) / NW;
-  static_assert(T::PIECES % NW == 0 || T::PIECES < NW, "whole rounds of pieces");
+  static constexpr bool EVEN = T::PIECES % NW == 0;
   uint32_t off[N];
   int kk[N];  // first k of the lane's chunk inside the step (KC)
 
@@ -89,20 +86,15 @@ struct Loader {
   }
   // k0: first k of the step; lds: the tile's place in LDS
   __device__ __forceinline__ void load(const Operand& o, int limb, int64_t k0, char* lds, int wave) const {
-    const uint16_t* p = o.p + limb * o.limb;
+    // lengths in 32 bits: at most 256 rows (KC) or BK rows (KS) of at most 2^21 elements
+    const uint16_t* p = o.p + limb * o.limb + (LAY == KC ? k0 : k0 * o.ld);
     const int64_t left = o.k - k0;
-    const int kend = left < BK ? (int)left : BK;
-    __amdgpu_buffer_rsrc_t rs;
-    if (LAY == KC) {
-      const int64_t n = o.rows < R ? o.rows : R;
-      rs = rsrc(p + k0, n > 0 && left > 0 ? ((n - 1) * o.ld + left) * 2 : 0);
-    } else {
-      const int64_t n = kend;
-      rs = rsrc(p + k0 * o.ld, n > 0 && o.rows > 0 ? ((n - 1) * o.ld + (o.rows < R ? o.rows : R)) * 2 : 0);
-    }
+    const int kend = left < BK ? (int)left : BK, rows = o.rows < R ? (int)o.rows : R;
+    const int len = LAY == KC ? ((rows - 1) * (int)o.ld + kend) * 2 : ((kend - 1) * (int)o.ld + rows) * 2;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, kend > 0 && rows > 0 ? len : 0, 0x00020000);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (T::PIECES < NW && wave >= T::PIECES) break;
+      if (!EVEN && wave + i * NW >= T::PIECES) break;
       const uint32_t v = (LAY == KC && kk[i] >= kend) ? OOB : off[i];
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + (wave + i * NW) * 1024), 16, v, 0, 0, 0);
     }
@@ -145,9 +137,9 @@ __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c) {
 // A block of WM x WN waves computes a BM x BN tile for each of NB operands B that share A.  The matrix instruction's first operand
 // is B: a lane then holds FOUR CONSECUTIVE j of ONE row i, so results leave as 8- or 16-byte stores:
 //   acc[b][mi][ni][r]:  i = wm BM / WM + 16 mi + lane % 16,   j = wn BN / WN + 16 ni + 4 (lane / 16) + r
-template <int MODE, int LA, int LB, int BM, int BN, int NB, int WM, int WN, int S = 2>
+template <int MODE, int LA, int LB, int BM, int BN, int NB, int WM, int WN, int S = 2, int BK_ = step_k<MODE>()>
 struct Core {
-  static constexpr int BK = step_k<MODE>(), NL = limbs<MODE>(), NW = WM * WN;
+  static constexpr int BK = BK_, NL = limbs<MODE>(), NW = WM * WN;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
   using TA = Tile<LA, BM, BK>;
   using TB = Tile<LB, BN, BK>;
@@ -162,6 +154,127 @@ struct Core {
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j) acc[b][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // matrix instructions of rows i0 .. i0 + n - 1 of the tile with all columns; the three limb products one after the other over the
+  // columns, the small ones first (they meet the smaller partial sum), so that no instruction waits for the one before it
+  template <int N>
+  static __device__ __forceinline__ void rows_mfma(const s16x8 (&fa)[N][NL], const s16x8 (&fb)[NB][NI][NL], Acc& acc, int i0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int p = NL == 2 ? 0 : 2; p < 3; ++p)
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) acc[b][i0 + i][j] = mfma<MODE>(fb[b][j][p == 0 ? NL - 1 : 0], fa[i][p == 1 ? NL - 1 : 0], acc[b][i0 + i][j]);
+  }
+
+  // The same sums as run(), software-pipelined inside a wave: a step is cut into phases of half the tile's rows and 32 k's; while a
+  // phase's matrix instructions run, the next phase's fragments are read.  The last phase of a step already reads the next stage, so the
+  // barrier stands in the middle of the arithmetic, and the loads issued behind it have a whole step to arrive.
+  // the order of a phase: its LDS reads and its loads spread evenly between its matrix instructions
+  template <int M, int D, int V, int g = 0>
+  static __device__ __forceinline__ void interleave() {
+    constexpr int G = M < 16 ? M : 16;
+    if constexpr (g < G) {
+      constexpr int m = M * (g + 1) / G - M * g / G, v = V * (g + 1) / G - V * g / G, d = D * (g + 1) / G - D * g / G;
+      if constexpr (m > 0) __builtin_amdgcn_sched_group_barrier(0x8, m, 0);
+      if constexpr (v > 0) __builtin_amdgcn_sched_group_barrier(0x10, v, 0);
+      if constexpr (d > 0) __builtin_amdgcn_sched_group_barrier(0x100, d, 0);
+      interleave<M, D, V, g + 1>();
+    }
+  }
+
+  static __device__ __forceinline__ void run_phased(char* smem, const Operand& A, const Operand (&B)[NB], Acc& acc) {
+    static_assert(S == 2 && MI % 2 == 0, "two stages, halves of the rows");
+    constexpr int HA = MI / 2, Q = 2 * (BK / 32), P = NL == 2 ? 3 : 1;
+    constexpr int RA = LA == KC ? 1 : 2, RB = LB == KC ? 1 : 2;  // LDS reads a fragment
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    Loader<LA, BM, BK, NW> la;
+    Loader<LB, BN, BK, NW> lb[NB];
+    la.init(wave, lane, A.ld);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) lb[b].init(wave, lane, B[b].ld);
+    Reader<LA, BM, BK> ra;
+    Reader<LB, BN, BK> rb;
+    ra.init(lane);
+    rb.init(lane);
+    const int nk = (int)((A.k + BK - 1) / BK);
+    auto stage_a = [&](int kt, char* s) {
+#pragma unroll
+      for (int l = 0; l < NL; ++l) la.load(A, l, (int64_t)kt * BK, s + l * TA::BYTES, wave);
+    };
+    auto stage_b = [&](int kt, char* s) {
+#pragma unroll
+      for (int l = 0; l < NL; ++l)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) lb[b].load(B[b], l, (int64_t)kt * BK, s + NL * TA::BYTES + (b * NL + l) * TB::BYTES, wave);
+    };
+    constexpr int VA = NL * Loader<LA, BM, BK, NW>::N, VB = NL * NB * Loader<LB, BN, BK, NW>::N;
+    s16x8 fa[2][HA][NL], fb[NB][NI][NL];
+    auto read_a = [&](s16x8 (&f)[HA][NL], const char* s, int q) {
+#pragma unroll
+      for (int i = 0; i < HA; ++i)
+#pragma unroll
+        for (int l = 0; l < NL; ++l) f[i][l] = ra.frag(s + l * TA::BYTES, wm * (BM / WM) + 16 * (i + (q & 1) * HA), q >> 1);
+    };
+    auto read_b = [&](int b, int j, const char* s, int ks) {
+#pragma unroll
+      for (int l = 0; l < NL; ++l) fb[b][j][l] = rb.frag(s + NL * TA::BYTES + (b * NL + l) * TB::BYTES, wn * (BN / WN) + 16 * j, ks);
+    };
+    stage_a(0, smem);
+    stage_b(0, smem);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (nk > 1) stage_a(1, smem + STAGE);
+    read_a(fa[0], smem, 0);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) read_b(b, j, smem, 0);
+    for (int kt = 0; kt < nk; ++kt) {
+      char* s = smem + (kt & 1) * STAGE;
+      char* t = smem + ((kt + 1) & 1) * STAGE;
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        const bool last = q == Q - 1;
+        const char* next = last ? t : s;  // behind the last step: leftovers of the other stage, read and never used
+        if (last) {
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          stage_a(kt + 2, s);  // behind the last step: nothing arrives, the descriptor is empty
+        }
+        if ((q & 1) == 0) {
+          if (q == 0) stage_b(kt + 1, t);
+          read_a(fa[1], next, q + 1);
+          rows_mfma<HA>(fa[0], fb, acc, 0);
+          if (q == 0) interleave<HA * NB * NI * P, HA * NL * RA, VB>();
+          else interleave<HA * NB * NI * P, HA * NL * RA, 0>();
+        } else {
+          read_a(fa[0], next, last ? 0 : q + 1);
+          // column by column: a column's fragments are read anew as soon as its last product is issued
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+#pragma unroll
+              for (int p = NL == 2 ? 0 : 2; p < 3; ++p)
+#pragma unroll
+                for (int i = 0; i < HA; ++i) acc[b][HA + i][j] = mfma<MODE>(fb[b][j][p == 0 ? NL - 1 : 0], fa[1][i][p == 1 ? NL - 1 : 0], acc[b][HA + i][j]);
+              read_b(b, j, next, last ? 0 : (q + 1) >> 1);
+            }
+          if (last) interleave<HA * NB * NI * P, HA * NL * RA + NB * NI * NL * RB, VA>();
+          else interleave<HA * NB * NI * P, HA * NL * RA + NB * NI * NL * RB, 0>();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   }
 
   // A.k > 0.  Ends with every wave past its last read of the LDS stages.
@@ -185,9 +298,9 @@ struct Core {
         for (int b = 0; b < NB; ++b) lb[b].load(B[b], l, (int64_t)kt * BK, s + NL * TA::BYTES + (b * NL + l) * TB::BYTES, wave);
       }
     };
-    // loads a wave issues per stage (the same for every wave: Loader's static_assert, or PIECES < NW and then S == 2)
+    // loads a wave issues per stage: the same for every wave, or S == 2
     constexpr int LPS = NL * (Loader<LA, BM, BK, NW>::N + NB * Loader<LB, BN, BK, NW>::N), AHEAD = (S - 2) * LPS;
-    static_assert(S == 2 || (TA::PIECES % NW == 0 && TB::PIECES % NW == 0 && AHEAD < 63), "countable loads");
+    static_assert(S == 2 || (Loader<LA, BM, BK, NW>::EVEN && Loader<LB, BN, BK, NW>::EVEN && AHEAD < 63), "countable loads");
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
       if (i < nk) stage(i, smem + i * STAGE);
@@ -214,19 +327,10 @@ struct Core {
             for (int l = 0; l < NL; ++l) fb[b][j][l] = rb.frag(sb + (b * NL + l) * TB::BYTES, wn * (BN / WN) + 16 * j, ks);
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-          s16x8 fa[NL];
+          s16x8 fa[1][NL];
 #pragma unroll
-          for (int l = 0; l < NL; ++l) fa[l] = ra.frag(sa + l * TA::BYTES, wm * (BM / WM) + 16 * i, ks);
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) {
-              if (NL == 2) {  // the small products first: they meet the smaller partial sum
-                acc[b][i][j] = mfma<MODE>(fb[b][j][NL - 1], fa[0], acc[b][i][j]);
-                acc[b][i][j] = mfma<MODE>(fb[b][j][0], fa[NL - 1], acc[b][i][j]);
-              }
-              acc[b][i][j] = mfma<MODE>(fb[b][j][0], fa[0], acc[b][i][j]);
-            }
+          for (int l = 0; l < NL; ++l) fa[0][l] = ra.frag(sa + l * TA::BYTES, wm * (BM / WM) + 16 * i, ks);
+          rows_mfma<1>(fa, fb, acc, i);
         }
       }
     }
