@@ -3,8 +3,15 @@
 //
 //   X0 = G / (|G|_F + eps)        A = X X^T        X <- (a I + b A + c A A) X       `steps` times, on the side with fewer rows
 //
-// Three products a step (ns_gram, ns_poly, ns_apply below) for ALL matrices of a call in one launch each: a list of matrices of any
-// shapes (or a batch of equal ones) is cut into tiles, and a block finds its matrix in the tile counts.
+// Three products a step (GRAM: A; POLY: C = a I + b A + c A A; APPLY: C X) for ALL matrices of a call in one launch each: a list of
+// matrices of any shapes (or a batch of equal ones) is cut into tiles, and a block finds its matrix in the tile counts.
+//
+// WIDE MATRICES (n columns, m rows, n >= 1.5 m) spend most of a step on X's two products.  C is a polynomial of A, so A of the next step is
+// C A C, and k steps on X are one with Q = C_k .. C_1: of the steps' products k - 1 GRAMs and APPLYs turn into three symmetric m x m
+// products each (PROD), which for 5 steps of 1024 x 4096 in groups of 2 and 3 leaves 38 of 65 units of m^3.  Groups stay short because A's
+// rounding errors grow by a^2 = 12 a step where X's grow by a.  The result is 4 times less exact than step by step (9e-6 against 2.4e-6
+// of the norm, float32's own plain evaluation: 2.4e-6, at 736 x 1408): nothing to a weight's update or to a result in 16 bits, and done
+// for those only.
 //
 // ARITHMETIC.  Small singular values grow by a^steps (485 with the usual coefficients), and with them every rounding of X relative to
 // the largest one; bf16's 2^-9 would be the result there.  So X, A and C = a I + b A + c A A are kept as two fp16 limbs (tile16.h,
@@ -237,12 +244,13 @@ __device__ __forceinline__ f32x4 load_limbs(const uint16_t* p, int64_t limb) {
   return v;
 }
 
-enum { GRAM = 0, POLY = 1, APPLY = 2 };
+enum { GRAM = 0, POLY = 1, APPLY = 2, PROD = 3 };
 struct NsArgs {
   const uint16_t* x;  // X: hi at the item's place, lo `limb` further
   uint16_t* y;        // the next X
-  uint16_t* am;       // A
-  uint16_t* cm;       // C = a I + b A + c A A
+  const uint16_t* l;  // m x m operands: POLY's A; APPLY's C; PROD's two factors
+  const uint16_t* r;
+  uint16_t* o;        // m x m result of GRAM, POLY and PROD
   int64_t xlimb, climb;
   float a, b, c;      // POLY, already in the scales of its operands and its result
   int shift;          // exponent from the accumulated sum to the stored limbs
@@ -252,7 +260,7 @@ struct NoItems {};
 template <bool LAST> struct ItemArg { typedef NoItems type; };
 template <> struct ItemArg<true> { typedef Items type; };
 
-// GRAM and POLY: only the tiles on and below the diagonal; what is right of it is written as their mirror image, turned in LDS
+// Symmetric results (all but APPLY's): only the tiles on and below the diagonal; what is right of it is written as their mirror image, turned in LDS
 template <int KIND, int T, int WM, int WN, int S, bool PHASED, bool LAST, class CLASSES>
 __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs s, Step st, typename ItemArg<LAST>::type items) {
   using Cr = Core<MODE_F16X3, KC, KIND == APPLY ? KS : KC, T, T, 1, WM, WN, S>;
@@ -285,17 +293,17 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
   if (KIND == GRAM) {
     A = Operand{s.x + xo + (int64_t)i0 * np, s.xlimb, np, mp - i0, np};
     B[0] = Operand{s.x + xo + (int64_t)j0 * np, s.xlimb, np, mp - j0, np};
-  } else if (KIND == POLY) {
-    A = Operand{s.am + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
-    B[0] = Operand{s.am + co + (int64_t)j0 * mp, s.climb, mp, mp - j0, mp};
+  } else if (KIND != APPLY) {
+    A = Operand{s.l + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
+    B[0] = Operand{(KIND == POLY ? s.l : s.r) + co + (int64_t)j0 * mp, s.climb, mp, mp - j0, mp};
   } else {
-    A = Operand{s.cm + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
+    A = Operand{s.l + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
     B[0] = Operand{s.x + xo + j0, s.xlimb, np, np - j0, mp};
   }
   if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
   else Cr::run(smem, A, B, acc);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  uint16_t* sym = (KIND == GRAM ? s.am : s.cm) + co;
+  uint16_t* sym = s.o + co;
   uint16_t* turn = (uint16_t*)smem;
 #pragma unroll
   for (int mi = 0; mi < Cr::MI; ++mi) {
@@ -305,13 +313,13 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
       const int jt = wn * (T / WN) + 16 * ni + 4 * (lane >> 4), j = j0 + jt;
       f32x4& v = acc[0][mi][ni];
       const bool in = i < mp && j < (KIND == APPLY ? np : mp);
-      if (KIND == GRAM) {
+      if (KIND == GRAM || KIND == PROD) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], s.shift);
         if (in) store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
       } else if (KIND == POLY) {
         if (in) {
-          const f32x4 u = load_limbs(s.am + co + (int64_t)i * mp + j, s.climb);
+          const f32x4 u = load_limbs(s.l + co + (int64_t)i * mp + j, s.climb);
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = fmaf(s.c, v[r], s.b * u[r]) + (i == j + r ? s.a : 0.f);
           store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
@@ -367,7 +375,8 @@ inline int ok() { return hipGetLastError() == hipSuccess ? HOLD_OK : HOLD_E_LAUN
 
 // The bounds of the singular values of X, and of the entries of A and C, through the iteration; false: they leave the range of the limbs
 struct Bounds {
-  int xs[33], as[33], cs[33];  // exponents of the scales: largest entry to below 2^14, a factor of 4 under fp16's range
+  int xs[33], as[33], cs[33];  // exponents of the scales of X, A, C: largest entry to below 2^14, a factor of 4 under fp16's range
+  int cb[33], ab[33];          // exponents above the bounds of C's and A's singular values
 };
 bool follow(const float* coef, int steps, Bounds& o) {
   double r = 1.;
@@ -375,14 +384,16 @@ bool follow(const float* coef, int steps, Bounds& o) {
     if (!(r < 1e9) || !(r > 1e-9)) return false;
     o.xs[k] = 14 - (int)ceil(log2(r));
     if (k == steps) break;
-    o.as[k] = 14 - (int)ceil(2. * log2(r));
+    o.ab[k] = (int)ceil(2. * log2(r));
+    o.as[k] = 14 - o.ab[k];
     const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2], S = r * r;
     if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
     auto P = [&](double s) { return fabs(a + b * s + c * s * s); };
     double top = fmax(P(0.), P(S));
     if (c != 0. && -b / (2. * c) > 0. && -b / (2. * c) < S) top = fmax(top, P(-b / (2. * c)));
     if (!(top < 1e9) || !(top > 1e-9)) return false;
-    o.cs[k] = 14 - (int)ceil(log2(top));
+    o.cb[k] = (int)ceil(log2(top));
+    o.cs[k] = 14 - o.cb[k];
     // the largest |s (a + b s^2 + c s^4)| on [0, r]: its ends and where a + 3 b s^2 + 5 c s^4 = 0
     double next = r * P(S);
     auto at = [&](double s2) {
@@ -404,12 +415,19 @@ bool follow(const float* coef, int steps, Bounds& o) {
 
 inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// the workspace of one group of items: partial sums, X twice, A and C, all limbs
+// the workspace of one group of items: partial sums, X twice, A and C (and Q and one more where steps are joined), all limbs
 struct Room {
-  int64_t part, x, y, am, cm, xn, cn, bytes;
+  int64_t part, x, y, mm[4], xn, cn, bytes;
 };
+// Whether an item's steps are joined: measured on 6 x 1024 x 4096 (1.77 -> 1.22 ms) and 3 x 1531 x 517 (294 -> 259 us); with less
+// work launches are what counts, and a result in float32 keeps float32's exactness
+bool joined(const Item& it, bool exact) {
+  if (exact) return false;
+  const double m = it.rows < it.cols ? it.rows : it.cols, n = it.rows < it.cols ? it.cols : it.rows;
+  return n >= 1.5 * m && m * m * n * it.count >= 1e9;
+}
 // sorts the items by shape, finds the classes and lays out the workspace
-Room room(Items& a, Classes& cl) {
+Room room(Items& a, Classes& cl, bool join) {
   auto small = [](const Item& i) { return i.rows < i.cols ? i.rows : i.cols; };
   auto large = [](const Item& i) { return i.rows < i.cols ? i.cols : i.rows; };
   for (int k = 1; k < a.n; ++k) {  // by insertion: equal shapes keep their order
@@ -443,8 +461,7 @@ Room room(Items& a, Classes& cl) {
   r.part = take(parts * 8);
   r.x = take(xn * 4);
   r.y = take(xn * 4);
-  r.am = take(cn * 4);
-  r.cm = take(cn * 4);
+  for (int k = 0; k < (join ? 4 : 2); ++k) r.mm[k] = take(cn * 4);
   r.xn = xn; r.cn = cn;
   r.bytes = o;
   return r;
@@ -502,14 +519,16 @@ int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStre
   return HOLD_OK;
 }
 
-int run_group(Items& a, const Step& st, const float* coef, int steps, char* ws, hipStream_t stream) {
+int run_group(Items& a, bool join, const Step& st, const float* coef, int steps, char* ws, hipStream_t stream) {
   Bounds bo;
   if (!follow(coef, steps, bo)) return HOLD_E_ARG;
   Classes cl;
-  const Room r = room(a, cl);
+  const Room r = room(a, cl, join);
   double* part = (double*)(ws + r.part);
   uint16_t* x = (uint16_t*)(ws + r.x);
   uint16_t* y = (uint16_t*)(ws + r.y);
+  uint16_t* mm[4];
+  for (int k = 0; k < 4; ++k) mm[k] = (uint16_t*)(ws + r.mm[k]);
   Firsts tn = {}, tl = {};
   int64_t nn = 0, nl = 0;
   for (int k = 0; k < a.n; ++k) {
@@ -520,31 +539,79 @@ int run_group(Items& a, const Step& st, const float* coef, int steps, char* ws, 
     nl += (int64_t)((up8(it.rows) + 63) / 64) * ((up8(it.cols) + 63) / 64) * it.count;
     if (nn > (1 << 30) || nl > (1 << 30)) return HOLD_E_ARG;
   }
+  if (count_tiles<APPLY>(cl, 256) < 0) return HOLD_E_ARG;
   hipLaunchKernelGGL(ns_norm_kernel, dim3((unsigned)nn), dim3(256), 0, stream, a, tn, st, part);
   hipLaunchKernelGGL(ns_load_kernel, dim3((unsigned)nl), dim3(256), 0, stream, a, tl, st, part, x, r.xn, bo.xs[0]);
   NsArgs s = {};
-  s.am = (uint16_t*)(ws + r.am);
-  s.cm = (uint16_t*)(ws + r.cm);
   s.xlimb = r.xn;
   s.climb = r.cn;
   int rc = HOLD_OK;
-  for (int k = 0; k < steps && rc == HOLD_OK; ++k) {
+  auto gram = [&](int k) {
     s.x = x;
-    s.y = y;
+    s.o = mm[0];
     s.shift = bo.as[k] - 2 * bo.xs[k];
-    rc = launch<GRAM, false>(cl, s, st, a, stream);
-    if (rc != HOLD_OK) break;
+    if (rc == HOLD_OK) rc = launch<GRAM, false>(cl, s, st, a, stream);
+  };
+  auto poly = [&](int k, uint16_t* o) {
+    s.l = mm[0];
+    s.o = o;
     s.a = (float)ldexp((double)coef[3 * k], bo.cs[k]);
     s.b = (float)ldexp((double)coef[3 * k + 1], bo.cs[k] - bo.as[k]);
     s.c = (float)ldexp((double)coef[3 * k + 2], bo.cs[k] - 2 * bo.as[k]);
-    rc = launch<POLY, false>(cl, s, st, a, stream);
-    if (rc != HOLD_OK) break;
-    const bool last = k + 1 == steps;
-    s.shift = (last ? 0 : bo.xs[k + 1]) - bo.cs[k] - bo.xs[k];
-    rc = last ? launch<APPLY, true>(cl, s, st, a, stream) : launch<APPLY, false>(cl, s, st, a, stream);
+    if (rc == HOLD_OK) rc = launch<POLY, false>(cl, s, st, a, stream);
+  };
+  auto prod = [&](const uint16_t* l, const uint16_t* p, uint16_t* o, int shift) {
+    s.l = l;
+    s.r = p;
+    s.o = o;
+    s.shift = shift;
+    if (rc == HOLD_OK) rc = launch<PROD, false>(cl, s, st, a, stream);
+  };
+  auto apply = [&](const uint16_t* c, int cs, int from, int to) {  // X of step `from` -> X before step `to`
+    s.l = c;
+    s.x = x;
+    s.y = y;
+    s.shift = (to == steps ? 0 : bo.xs[to]) - cs - bo.xs[from];
+    if (rc == HOLD_OK) rc = to == steps ? launch<APPLY, true>(cl, s, st, a, stream) : launch<APPLY, false>(cl, s, st, a, stream);
     uint16_t* z = x;
     x = y;
     y = z;
+  };
+  if (!join) {
+    for (int k = 0; k < steps; ++k) {
+      gram(k);
+      poly(k, mm[1]);
+      apply(mm[1], bo.cs[k], k, k + 1);
+    }
+  } else {
+    const int groups = (steps + 2) / 3;
+    for (int g = 0, k = 0; g < groups; ++g) {
+      const int first = k, end = steps * (g + 1) / groups;
+      uint16_t *A = mm[0], *C = mm[1], *Q = mm[2], *T = mm[3];
+      int qb = 0;  // exponent above Q's singular values
+      gram(k);
+      for (; k < end; ++k) {
+        const uint16_t* c = C;
+        if (k == first) {
+          poly(k, Q);
+          c = Q;
+          qb = bo.cb[k];
+        } else {
+          poly(k, C);
+          qb += bo.cb[k];
+          prod(C, Q, T, 14 - qb - bo.cs[k] - (14 - (qb - bo.cb[k])));
+          uint16_t* z = Q;
+          Q = T;
+          T = z;
+        }
+        if (k + 1 < end) {  // A <- (C A) C
+          const int ts = 14 - bo.cb[k] - bo.ab[k];
+          prod(c, A, T, ts - bo.cs[k] - bo.as[k]);
+          prod(T, c, A, bo.as[k + 1] - ts - bo.cs[k]);
+        }
+      }
+      apply(Q, 14 - qb, first, end);
+    }
   }
   return rc == HOLD_OK ? ok() : rc;
 }
@@ -563,18 +630,33 @@ bool one_item(const hold_ortho_desc* d, Items& a) {
   it.stride = (int64_t)d->rows * d->cols;
   return true;
 }
-// items first .. first + n - 1 of a step
-bool some_items(const hold_muon_desc* d, int first, Items& a) {
-  a.n = d->n_items - first < MAXI ? d->n_items - first : MAXI;
-  for (int k = 0; k < a.n; ++k) {
-    const hold_muon_item& i = d->items[first + k];
-    if (!sizes_ok(i.rows, i.cols, 1) || i.ldp < i.cols || i.ldg < i.cols || i.ldm < i.cols) return false;
-    Item& it = a.it[k];
-    it = Item{};
-    it.g = i.g; it.m = i.m; it.p = i.p;
-    it.rows = i.rows; it.cols = i.cols; it.count = 1;
-    it.ldg = i.ldg; it.ldm = i.ldm; it.ldp = i.ldp;
-    it.gain = (float)(d->lr * i.scale);
+bool read_item(const hold_muon_desc* d, int k, Item& it) {
+  const hold_muon_item& i = d->items[k];
+  if (!sizes_ok(i.rows, i.cols, 1) || i.ldp < i.cols || i.ldg < i.cols || i.ldm < i.cols) return false;
+  it = Item{};
+  it.g = i.g; it.m = i.m; it.p = i.p;
+  it.rows = i.rows; it.cols = i.cols; it.count = 1;
+  it.ldg = i.ldg; it.ldm = i.ldm; it.ldp = i.ldp;
+  it.gain = (float)(d->lr * i.scale);
+  return true;
+}
+// calls f(items, join) for the groups of a step: those whose steps are joined, then the others, up to MAXI a group; false: a bad item
+template <class F>
+bool groups_of(const hold_muon_desc* d, F f) {
+  for (int join = 1; join >= 0; --join) {
+    Items a;
+    a.n = 0;
+    for (int k = 0; k < d->n_items; ++k) {
+      Item it;
+      if (!read_item(d, k, it)) return false;
+      if (joined(it, false) != (join != 0)) continue;
+      a.it[a.n++] = it;
+      if (a.n == MAXI) {
+        if (!f(a, join != 0)) return false;
+        a.n = 0;
+      }
+    }
+    if (a.n && !f(a, join != 0)) return false;
   }
   return true;
 }
@@ -585,34 +667,32 @@ extern "C" int hold_orthogonalize_workspace(const hold_ortho_desc* d, int64_t* b
   Items a;
   Classes cl;
   if (!one_item(d, a) || !bytes) return HOLD_E_ARG;
-  *bytes = room(a, cl).bytes;
+  *bytes = room(a, cl, joined(a.it[0], d->dtype == HOLD_MUON_F32)).bytes;
   return HOLD_OK;
 }
 
 extern "C" int hold_orthogonalize(const hold_ortho_desc* d, hold_stream_t stream) {
   Items a;
-  Classes cl;
-  if (!one_item(d, a) || !d->x || !d->out || !d->coef || d->steps < 1 || d->steps > 32 || d->dtype < 0 || d->dtype > 2 || !(d->eps >= 0.f)) return HOLD_E_ARG;
-  if (!d->workspace || room(a, cl).bytes > d->workspace_bytes) return HOLD_E_ARG;
+  int64_t need = 0;
+  if (hold_orthogonalize_workspace(d, &need) != HOLD_OK || !d->workspace || need > d->workspace_bytes || !one_item(d, a)) return HOLD_E_ARG;
+  if (!d->x || !d->out || !d->coef || d->steps < 1 || d->steps > 32 || d->dtype < 0 || d->dtype > 2 || !(d->eps >= 0.f)) return HOLD_E_ARG;
   a.it[0].g = d->x;
   a.it[0].p = d->out;
   Step st = {};
   st.eps = d->eps;
   st.dtype = d->dtype;
-  return run_group(a, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+  return run_group(a, joined(a.it[0], d->dtype == HOLD_MUON_F32), st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
 }
 
 extern "C" int hold_muon_workspace(const hold_muon_desc* d, int64_t* bytes) {
   if (!d || !bytes || d->n_items < 1 || !d->items) return HOLD_E_ARG;
   *bytes = 0;
-  for (int first = 0; first < d->n_items; first += MAXI) {
-    Items a;
+  return groups_of(d, [&](Items& a, bool join) {
     Classes cl;
-    if (!some_items(d, first, a)) return HOLD_E_ARG;
-    const int64_t n = room(a, cl).bytes;
+    const int64_t n = room(a, cl, join).bytes;
     if (n > *bytes) *bytes = n;
-  }
-  return HOLD_OK;
+    return true;
+  }) ? HOLD_OK : HOLD_E_ARG;
 }
 
 extern "C" int hold_muon_step(const hold_muon_desc* d, hold_stream_t stream) {
@@ -632,11 +712,10 @@ extern "C" int hold_muon_step(const hold_muon_desc* d, hold_stream_t stream) {
   st.grad_mul = d->grad_mul;
   st.clip = d->clip_norm;
   st.sumsq = d->sumsq;
-  for (int first = 0; first < d->n_items; first += MAXI) {  // groups share the workspace: they run one after the other
-    Items a;
-    some_items(d, first, a);
-    const int rc = run_group(a, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
-    if (rc != HOLD_OK) return rc;
-  }
-  return HOLD_OK;
+  int rc = HOLD_OK;  // groups share the workspace: they run one after the other
+  groups_of(d, [&](Items& a, bool join) {
+    rc = run_group(a, join, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+    return rc == HOLD_OK;
+  });
+  return rc;
 }

@@ -58,12 +58,14 @@ struct Tile {
   static constexpr int C = RB / 16;                     // 16-byte chunks of a tile row
   static constexpr int BYTES = RB * NR;
   static constexpr int PIECES = BYTES / 1024;           // wave-wide 16-byte loads
-  static_assert((LAY == KC ? C == 4 || C == 8 : C >= 8) && BYTES % 1024 == 0, "tile rows of 64 or 128 bytes (KC), 128 and more (KS)");
+  static_assert((LAY == KC ? C == 4 || C == 8 : C % 8 == 0) && BYTES % 1024 == 0, "tile rows of 64 or 128 bytes (KC), multiples of 128 (KS): the exchange of chunks stays inside a row");
   static __device__ __forceinline__ int swz(int row) {
     // a 16-byte read is served 16 lanes at a time: of two neighbouring 16-lane groups (two chunks), rows 0-3 and 12-15 of one with
     // rows 4-11 of the other
     if (LAY == KC) return C == 8 ? ((row >> 1) & 7) : (-(row >> 2) & 3);
-    return C >= 16 ? 2 * ((row & 3) | ((row >> 1) & 4)) : 2 * (((row >> 1) & 1) | ((row >> 2) & 2));
+    // of the 16 rows k that a transposing read touches, 8 at a time: by the whole 256 bytes of the banks where a row is a multiple of
+    // that; where it is an odd multiple of 128 its parity already moves it by half of them
+    return C % 16 == 0 ? 2 * ((row & 3) | ((row >> 1) & 4)) : 2 * (((row >> 1) & 1) | ((row >> 2) & 2));
   }
 };
 
@@ -245,7 +247,7 @@ struct Core {
           asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
-          stage_a(kt + 2, s);  // behind the last step: nothing arrives, the descriptor is empty
+          stage_a(kt + 2, s);  // behind the last step the descriptor is empty: zeros, waited for below
         }
         if ((q & 1) == 0) {
           if (q == 0) stage_b(kt + 1, t);
@@ -272,7 +274,8 @@ struct Core {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // also the loads behind the last step, which write zeros: the caller may use the stages at once
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   }
