@@ -107,28 +107,41 @@ __device__ __forceinline__ float wave_fmax(float v) {
 }
 
 constexpr int NPART = 256;  // blocks that look for the weights' maxima
-// exponents kept by a call in fp32 (ints): [0] Wg, [1] Wu, [2] bg, [3] bu (all: exp_above of the largest magnitude, NONE of nothing), [4] R,
-// [5] and [6] the exponents by which Wg and Wu are scaled (a matrix of zeros takes the other's)
+// exponents kept by a backward call in fp32 (ints): [0] Wg, [1] Wu, [2] bg, [3] bu (exp_above of the largest magnitude, NONE of nothing),
+// [4] R, [5] and [6] the exponents by which Wg and Wu are scaled (a matrix of zeros takes the other's)
 constexpr int NONE = -100000;
 __device__ __forceinline__ int exp_or_none(float m) { return m > 0.f ? exp_above(m) : NONE; }
 
-// bits of the largest finite magnitude of a tensor, per block of the grid: part[which][block]
-__global__ __launch_bounds__(256) void gated_amax_kernel(const float* wg, int64_t ldg, const float* wu, int64_t ldu, const float* bg,
-                                                         const float* bu, int H, int D, float* part) {
-  const float* src[4] = {wg, wu, bg, bu};
-  const int which = blockIdx.y;
-  const float* p = src[which];
+// a wave's rows: 4 consecutive elements a lane, 256 a piece; `vec`: rows on 16-byte boundaries
+__device__ __forceinline__ f32x4 row4(const float* p, int c, int K, bool vec) { return load4<MODE_F16X3>(p, c, K - c, vec); }
+
+__device__ __forceinline__ float row_max(const float* p, int K, bool vec) {
+  const int lane = threadIdx.x & 63;
   float m = 0.f;
-  if (p && which < 2) {
+  for (int c = 4 * lane; c < K; c += 256) {
+    const f32x4 v = row4(p, c, K, vec);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m = fmaxf(m, finite_abs(v[r]));
+  }
+  return wave_fmax(m);
+}
+
+// largest finite magnitude of the weights and biases, per block of the grid: part[which][block]
+__global__ __launch_bounds__(256) void gated_amax_kernel(const float* wg, int64_t ldg, const float* wu, int64_t ldu, const float* bg,
+                                                         const float* bu, int H, int D, int vec, float* part) {
+  const int which = blockIdx.y;
+  float m = 0.f;
+  if (which < 2) {
+    const float* p = which ? wu : wg;
     const int64_t ld = which ? ldu : ldg;
-    const int lane = threadIdx.x & 63;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < H; r += gridDim.x * 4)
-      for (int c = lane; c < D; c += 64) m = fmaxf(m, finite_abs(p[r * ld + c]));
-  } else if (p) {
-    for (int c = blockIdx.x * 256 + threadIdx.x; c < H; c += gridDim.x * 256) m = fmaxf(m, finite_abs(p[c]));
+    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < H; r += gridDim.x * 4) m = fmaxf(m, row_max(p + r * ld, D, vec));
+  } else {
+    const float* p = which == 2 ? bg : bu;
+    if (p)
+      for (int c = blockIdx.x * 256 + threadIdx.x; c < H; c += gridDim.x * 256) m = fmaxf(m, finite_abs(p[c]));
+    m = wave_fmax(m);
   }
   __shared__ float s[4];
-  m = wave_fmax(m);
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
   __syncthreads();
   if (threadIdx.x == 0) part[which * NPART + blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
@@ -136,107 +149,116 @@ __global__ __launch_bounds__(256) void gated_amax_kernel(const float* wg, int64_
 
 __device__ __forceinline__ float part_max(const float* part, int which) {  // every wave of a block by itself; NPART values
   const int lane = threadIdx.x & 63;
-  float m = 0.f;
-  for (int i = lane; i < NPART; i += 64) m = fmaxf(m, part[which * NPART + i]);
-  return wave_fmax(m);
+  const f32x4 v = *(const f32x4*)(part + which * NPART + 4 * lane);
+  static_assert(NPART == 256, "four values a lane");
+  return wave_fmax(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
 }
 
-__device__ __forceinline__ void write_limbs(uint16_t* hi, uint16_t* lo, const float (&v)[8]) {
-  u32x4 h, l;
+// 4 scaled values as limbs; columns behind K up to Kp as zeros
+__device__ __forceinline__ void put_limbs(uint16_t* o, int64_t limb, f32x4 v, int k) {
+  Split y[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const Split a = split16(v[2 * i]), b = split16(v[2 * i + 1]);
-    h[i] = a.hi | (uint32_t)b.hi << 16;
-    l[i] = a.lo | (uint32_t)b.lo << 16;
-  }
-  *(u32x4*)hi = h;
-  *(u32x4*)lo = l;
+  for (int r = 0; r < 4; ++r) y[r] = split16(ldexpf(v[r], k));
+  *(u32x2*)o = u32x2{y[0].hi | (uint32_t)y[1].hi << 16, y[2].hi | (uint32_t)y[3].hi << 16};
+  *(u32x2*)(o + limb) = u32x2{y[0].lo | (uint32_t)y[1].lo << 16, y[2].lo | (uint32_t)y[3].lo << 16};
 }
-
-// fp32 rows -> limbs [R][Kp], each row scaled to [2^14, 2^15) by its own exponent (rowexp: exp_above of the row, NONE of an empty one)
-__global__ __launch_bounds__(256) void gated_pack_rows_kernel(const float* x, int64_t ld, int64_t R, int K, int Kp, uint16_t* out, int64_t limb,
-                                                              int* rowexp) {
+// one row to limbs by 2^k
+__device__ __forceinline__ void pack_row(const float* p, int K, int Kp, bool vec, int k, uint16_t* o, int64_t limb) {
   const int lane = threadIdx.x & 63;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < R; r += (int64_t)gridDim.x * 4) {
-    const float* p = x + r * ld;
-    float m = 0.f;
-    for (int c = lane; c < K; c += 64) m = fmaxf(m, finite_abs(p[c]));
-    m = wave_fmax(m);
-    const int e = exp_or_none(m), k = e == NONE ? 0 : 15 - e;
-    if (lane == 0) rowexp[r] = e;
-    for (int c = lane * 8; c < Kp; c += 512) {
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c + i < K ? ldexpf(p[c + i], k) : 0.f;
-      write_limbs(out + r * Kp + c, out + limb + r * Kp + c, v);
-    }
-  }
+  for (int c = 4 * lane; c < Kp; c += 256) put_limbs(o + c, limb, row4(p, c, K, vec), k);
 }
 
-// both weight matrices -> limbs [H][Dp], one exponent a matrix; block 0 leaves the exponents in `exps`
-__global__ __launch_bounds__(256) void gated_pack_weights_kernel(const float* wg, int64_t ldg, const float* wu, int64_t ldu, int H, int D, int Dp,
-                                                                 const float* part, uint16_t* out, int64_t limb, int64_t second, int* exps) {
-  const int lane = threadIdx.x & 63, which = blockIdx.y;
-  const int e = exp_or_none(part_max(part, which)), other = exp_or_none(part_max(part, 1 - which));
-  const int scale = e != NONE ? e : other != NONE ? other : 15, k = 15 - scale;
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    exps[which] = e;
-    exps[5 + which] = scale;
-  }
-  if (blockIdx.x == 0 && threadIdx.x < 64) {
-    const int eb = exp_or_none(part_max(part, 2 + which));
-    if (lane == 0) exps[2 + which] = eb;
-  }
-  const float* w = which ? wu : wg;
-  const int64_t ld = which ? ldu : ldg;
-  uint16_t* o = out + which * second;
-  for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < H; r += gridDim.x * 4)
-    for (int c = lane * 8; c < Dp; c += 512) {
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c + i < D ? ldexpf(w[r * ld + c + i], k) : 0.f;
-      write_limbs(o + (int64_t)r * Dp + c, o + limb + (int64_t)r * Dp + c, v);
-    }
-}
+struct PackArgs {
+  const float* x; int64_t ldx, T;
+  const float* w[2]; int64_t ldw[2];
+  int H, D, Dp, xvec, wvec;
+  uint16_t* ox; int64_t xlimb;
+  uint16_t* ow; int64_t wlimb, second;
+  int* rowexp;       // [T]
+  int* colexp;       // [2][Hp]: the exponent of a weight row's scale
+  int64_t Hp;
+  // backward
+  const float* part; // the weights' maxima: one scale a matrix, and the exponents below
+  int* exps;
+  const float* dh; int64_t lddh; int dvec, act;
+  int* rscale; int* rpart;
+};
 
-// backward, fp32: the scale exponent r_t of every row of dg and du, and per block the largest exponent of x_t 2^-r_t.
+// All rows to limbs [rows][Dp], a wave a row: x's scaled to [2^14, 2^15) by their own exponents, the weights' too (forward, where they only
+// meet x) or by one a matrix (backward, where the sum also runs over H).  Backward: also the scale exponent r_t of a row of dg and du and
+// the block's largest exponent of x_t 2^-r_t:
 //   |g| <= D max|x_t| max|Wg| + max|bg|, |u| likewise; |act(g)| <= |g| (sigmoid: 1); |act'| < 2 (relu: 1, sigmoid: 1/4)
-__global__ __launch_bounds__(256) void gated_row_scale_kernel(const float* dh, int64_t ld, int64_t T, int H, int D, int act, const int* rowexp,
-                                                              const int* exps, int* rscale, int* part) {
-  const int lane = threadIdx.x & 63;
-  int ld2 = 0;
-  while ((1 << ld2) < D) ++ld2;
-  int top = NONE;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < T; r += (int64_t)gridDim.x * 4) {
-    float m = 0.f;
-    for (int c = lane; c < H; c += 64) m = fmaxf(m, finite_abs(dh[r * ld + c]));
-    const int ed = exp_or_none(wave_fmax(m)), ex = rowexp[r];
-    auto proj = [&](int w) {  // exponent above a projection's magnitude
-      const int a = (ex == NONE || exps[w] == NONE) ? NONE : ex + exps[w] + ld2, b = exps[2 + w];
-      return (a > b ? a : b) == NONE ? NONE : (a > b ? a : b) + 1;
-    };
-    const int eg = proj(0), eu = proj(1);
-    const int ea = act == ACT_SIGMOID ? 0 : eg, edg = eu + (act == ACT_SIGMOID ? -2 : act == ACT_RELU ? 0 : 1);
-    // r_t of dg such that dg 2^r_t and du 2^(r_t + shift) both stay below 2^15
-    const int shift = exps[6] - exps[5], top2 = edg > ea + shift ? edg : ea + shift;
-    const bool none = ed == NONE || top2 < -50000;
-    const int k = none ? NONE : 15 - (ed + top2);
-    if (lane == 0) rscale[r] = k;
-    if (!none && ex != NONE && ex - k > top) top = ex - k;
+template <bool BWD>
+__global__ __launch_bounds__(256) void gated_pack_kernel(PackArgs a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int e[4] = {NONE, NONE, NONE, NONE}, ws[2] = {0, 0}, ld2 = 0, top = NONE;
+  if (BWD) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = exp_or_none(part_max(a.part, i));
+    ws[0] = e[0] != NONE ? e[0] : e[1] != NONE ? e[1] : 15;
+    ws[1] = e[1] != NONE ? e[1] : e[0] != NONE ? e[0] : 15;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      a.exps[5] = ws[0];
+      a.exps[6] = ws[1];
+    }
+    while ((1 << ld2) < a.D) ++ld2;
   }
-  __shared__ int s[4];
-  if (lane == 0) s[threadIdx.x >> 6] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int v = s[0];
-    for (int i = 1; i < 4; ++i) v = s[i] > v ? s[i] : v;
-    part[blockIdx.x] = v;
+  const int64_t rows = a.T + 2 * (int64_t)a.H;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows; r += (int64_t)gridDim.x * 4) {
+    if (r >= a.T) {
+      const int w = r - a.T >= a.H, j = (int)(r - a.T) - w * a.H;
+      const float* p = a.w[w] + j * a.ldw[w];
+      int ex = BWD ? ws[w] : 0;
+      if (!BWD) {
+        ex = exp_or_none(row_max(p, a.D, a.wvec));
+        ex = ex == NONE ? 15 : ex;
+      }
+      if (lane == 0) a.colexp[w * a.Hp + j] = ex;
+      pack_row(p, a.D, a.Dp, a.wvec, 15 - ex, a.ow + w * a.second + (int64_t)j * a.Dp, a.wlimb);
+      continue;
+    }
+    const float* p = a.x + r * a.ldx;
+    uint16_t* o = a.ox + r * a.Dp;
+    int ex;
+    if (a.Dp <= 256) {  // the row stays in registers
+      const f32x4 v = row4(p, 4 * lane, a.D, a.xvec);
+      ex = exp_or_none(wave_fmax(fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3])))));
+      if (4 * lane < a.Dp) put_limbs(o + 4 * lane, a.xlimb, v, ex == NONE ? 0 : 15 - ex);
+    } else {
+      ex = exp_or_none(row_max(p, a.D, a.xvec));
+      pack_row(p, a.D, a.Dp, a.xvec, ex == NONE ? 0 : 15 - ex, o, a.xlimb);
+    }
+    if (lane == 0) a.rowexp[r] = ex;
+    if (BWD) {
+      const int ed = exp_or_none(row_max(a.dh + r * a.lddh, a.H, a.dvec));
+      auto proj = [&](int w) {  // exponent above a projection's magnitude
+        const int m = (ex == NONE || e[w] == NONE) ? NONE : ex + e[w] + ld2, b = e[2 + w];
+        return (m > b ? m : b) == NONE ? NONE : (m > b ? m : b) + 1;
+      };
+      const int eg = proj(0), eu = proj(1);
+      const int ea = a.act == ACT_SIGMOID ? 0 : eg, edg = eu + (a.act == ACT_SIGMOID ? -2 : a.act == ACT_RELU ? 0 : 1);
+      // r_t of dg such that dg 2^r_t and du 2^(r_t + shift) both stay below 2^15
+      const int shift = ws[1] - ws[0], top2 = edg > ea + shift ? edg : ea + shift;
+      const bool none = ed == NONE || top2 < -50000;
+      const int k = none ? NONE : 15 - (ed + top2);
+      if (lane == 0) a.rscale[r] = k;
+      if (!none && ex != NONE && ex - k > top) top = ex - k;
+    }
+  }
+  if (BWD) {
+    __shared__ int s[4];
+    if (lane == 0) s[wave] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const int u = s[0] > s[1] ? s[0] : s[1], v = s[2] > s[3] ? s[2] : s[3];
+      a.rpart[blockIdx.x] = u > v ? u : v;
+    }
   }
 }
 
 // x_t 2^(R - r_t) as limbs for the sum over tokens; rows without a gradient are zeros (where finite).  exps[4] = R
-__global__ __launch_bounds__(256) void gated_pack_tokens_kernel(const float* x, int64_t ld, int64_t T, int D, int Dp, const int* rscale, const int* part,
-                                                                int nparts, uint16_t* out, int64_t limb, int* exps) {
+__global__ __launch_bounds__(256) void gated_pack_tokens_kernel(const float* x, int64_t ld, int64_t T, int D, int Dp, int vec, const int* rscale,
+                                                                const int* part, int nparts, uint16_t* out, int64_t limb, int* exps) {
   const int lane = threadIdx.x & 63;
   int top = NONE;
   for (int i = lane; i < nparts; i += 64) top = part[i] > top ? part[i] : top;
@@ -245,23 +267,33 @@ __global__ __launch_bounds__(256) void gated_pack_tokens_kernel(const float* x, 
   if (blockIdx.x == 0 && threadIdx.x == 0) exps[4] = R;
   for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < T; r += (int64_t)gridDim.x * 4) {
     const int k = rscale[r];
-    for (int c = lane * 8; c < Dp; c += 512) {
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = c + i < D ? x[r * ld + c + i] : 0.f;
-        v[i] = k == NONE ? y * 0.f : ldexpf(y, R - k);
-      }
-      write_limbs(out + r * Dp + c, out + limb + r * Dp + c, v);
+    for (int c = 4 * lane; c < Dp; c += 256) {
+      f32x4 v = row4(x + r * ld, c, D, vec);
+      if (k == NONE) v *= 0.f;
+      put_limbs(out + r * Dp + c, limb, v, k == NONE ? 0 : R - k);
     }
   }
 }
 
-// bf16 rows whose base, stride or length the tile loads cannot take -> [R][Kp], zeros behind K
-__global__ __launch_bounds__(256) void gated_copy_rows_kernel(const uint16_t* x, int64_t ld, int64_t R, int K, int Kp, uint16_t* out) {
+// bf16 rows whose base, stride or length the tile loads cannot take -> [rows][Kp], zeros behind K; up to three matrices of equal length
+struct CopyArgs {
+  const uint16_t* x[3]; int64_t ld[3], rows[3];
+  uint16_t* out[3];
+  int K, Kp;
+};
+__global__ __launch_bounds__(256) void gated_copy_rows_kernel(CopyArgs a) {
   const int lane = threadIdx.x & 63;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < R; r += (int64_t)gridDim.x * 4)
-    for (int c = lane; c < Kp; c += 64) out[r * Kp + c] = c < K ? x[r * ld + c] : (uint16_t)0;
+  const int64_t all = a.rows[0] + a.rows[1] + a.rows[2];
+  for (int64_t q = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); q < all; q += (int64_t)gridDim.x * 4) {
+    const int w = q < a.rows[0] ? 0 : q < a.rows[0] + a.rows[1] ? 1 : 2;
+    const int64_t r = q - (w > 0 ? a.rows[0] : 0) - (w > 1 ? a.rows[1] : 0);
+    const uint16_t* p = a.x[w] + r * a.ld[w];
+    uint16_t* o = a.out[w] + r * a.Kp;
+    for (int c = 2 * lane; c < a.Kp; c += 128) {
+      const uint32_t u = c < a.K ? p[c] : 0, v = c + 1 < a.K ? p[c + 1] : 0;
+      *(uint32_t*)(o + c) = u | v << 16;
+    }
+  }
 }
 
 // ---- both projections and what follows them -------------------------------------------------------------------------------------------
@@ -270,7 +302,7 @@ struct MmaArgs {
   const uint16_t* wg; const uint16_t* wu; int64_t ldwg, ldwu, wlimb;
   const void* bg; const void* bu;
   int64_t T; int H; int K; int act;
-  const int* rowexp; const int* exps;            // fp32: the scales of x's rows and of the weights
+  const int* rowexp; const int* colexp; const int* exps;  // fp32: the scales of x's rows, of the weights' rows; backward's exponents
   void* h; int64_t ldh;                          // forward
   const void* dh; int64_t lddh;                  // backward
   uint16_t* dg; uint16_t* du; int64_t Hp, dlimb; // [T][Hp] limbs of dg and du
@@ -279,7 +311,7 @@ struct MmaArgs {
   int tm, tn;
 };
 
-template <int MODE, bool BWD, int BM, int BN, int WM, int WN>
+template <int MODE, bool BWD, int BM, int BN, int WM, int WN, bool PHASED>
 __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
   using Cr = Core<MODE, KC, KC, BM, BN, 2, WM, WN>;
   __shared__ __align__(1024) char smem[Cr::LDS];
@@ -291,10 +323,11 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
   Cr::zero(acc);
   const Operand A = {a.x + m0 * a.ldx, a.xlimb, a.ldx, a.T - m0, a.K};
   const Operand B[2] = {{a.wg + (int64_t)n0 * a.ldwg, a.wlimb, a.ldwg, a.H - n0, a.K}, {a.wu + (int64_t)n0 * a.ldwu, a.wlimb, a.ldwu, a.H - n0, a.K}};
-  Cr::run(smem, A, B, acc);
+  if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
+  else Cr::run(smem, A, B, acc);
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  const int eg = MODE == MODE_F16X3 ? a.exps[5] - 15 : 0, eu = MODE == MODE_F16X3 ? a.exps[6] - 15 : 0;
+  const int shift = MODE == MODE_F16X3 && BWD ? a.exps[6] - a.exps[5] : 0;
   constexpr int ES = MODE == MODE_BF16 ? 2 : 4;
   const bool hvec = BWD ? (a.lddh % 4 == 0 && (uintptr_t)a.dh % (4 * ES) == 0) : (a.ldh % 4 == 0 && (uintptr_t)a.h % (4 * ES) == 0);
   const bool bvec = (uintptr_t)a.bg % (4 * ES) == 0 && (uintptr_t)a.bu % (4 * ES) == 0;
@@ -305,6 +338,14 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
     f32x4 bg = {0.f, 0.f, 0.f, 0.f}, bu = {0.f, 0.f, 0.f, 0.f};
     if (a.bg && n > 0) bg = load4<MODE>(a.bg, j, n, bvec);
     if (a.bu && n > 0) bu = load4<MODE>(a.bu, j, n, bvec);
+    int eg[4] = {0, 0, 0, 0}, eu[4] = {0, 0, 0, 0};
+    if (MODE == MODE_F16X3 && n > 0) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {  // [2][Hp]: four entries are inside
+        eg[r] = a.colexp[j + r] - 15;
+        eu[r] = a.colexp[a.Hp + j + r] - 15;
+      }
+    }
     f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int mi = 0; mi < Cr::MI; ++mi) {
@@ -315,8 +356,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
         const int e = row ? a.rowexp[i] : NONE, ex = e == NONE ? 0 : e - 15;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          g[r] = ldexpf(g[r], ex + eg);
-          u[r] = ldexpf(u[r], ex + eu);
+          g[r] = ldexpf(g[r], ex + eg[r]);
+          u[r] = ldexpf(u[r], ex + eu[r]);
         }
       }
       g += bg;
@@ -350,7 +391,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
             store4<MODE>(a.dg, o, 4, true, dg);
             store4<MODE>(a.du, o, 4, true, du);
           } else {
-            const int k = a.rscale[i] == NONE ? 0 : a.rscale[i], ku = a.rscale[i] == NONE ? 0 : k + eu - eg;
+            const int k = a.rscale[i] == NONE ? 0 : a.rscale[i], ku = a.rscale[i] == NONE ? 0 : k + shift;
             uint16_t hg[4], lg[4], hu[4], lu[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -394,20 +435,23 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
   }
 }
 
-// db[w][j] = sum over the row tiles, in 4 interleaved chains per column joined in a fixed order
+// db[w][j] = sum over the row tiles, in 16 interleaved chains per column joined in a fixed order
 template <int MODE>
-__global__ __launch_bounds__(256) void gated_db_kernel(const float* part, int tiles, int H, void* dbg, void* dbu) {
-  const int w = blockIdx.y, j = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-  __shared__ float s[4][64];
+__global__ __launch_bounds__(1024) void gated_db_kernel(const float* part, int tiles, int H, void* dbg, void* dbu) {
+  const int w = blockIdx.y, c = threadIdx.x & 63, j = blockIdx.x * 64 + c, q = threadIdx.x >> 6;
+  __shared__ float s[16][64];
   float v = 0.f;
   if (j < H)
-    for (int t = q; t < tiles; t += 4) v += part[((int64_t)t * 2 + w) * H + j];
-  s[q][threadIdx.x & 63] = v;
+    for (int t = q; t < tiles; t += 16) v += part[((int64_t)t * 2 + w) * H + j];
+  s[q][c] = v;
   __syncthreads();
   void* out = w ? dbu : dbg;
   if (q == 0 && j < H && out) {
-    const int c = threadIdx.x;
-    store1<MODE>(out, j, (s[0][c] + s[1][c]) + (s[2][c] + s[3][c]));
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1)
+#pragma unroll
+      for (int i = 0; i < k; ++i) s[i][c] += s[i + k][c];
+    store1<MODE>(out, j, s[0][c]);
   }
 }
 
@@ -417,30 +461,35 @@ struct DxArgs {
   const uint16_t* wg; const uint16_t* wu; int64_t ldwg, ldwu, wlimb;
   int64_t T; int H, D;
   const int* rscale; const int* exps;
-  void* dx; int64_t lddx;
+  void* dx;
+  int64_t chunk; int splits;  // the sum over H is split, `chunk` each
+  float* part;                // [split][T][D], where splits > 1
   int tm, tn;
 };
 
-template <int MODE, int BM, int BN, int WM, int WN>
+template <int MODE, int BM, int BN, int WM, int WN, bool PHASED>
 __global__ __launch_bounds__(64 * WM * WN) void gated_dx_kernel(DxArgs a) {
   using Cr = Core<MODE, KC, KS, BM, BN, 1, WM, WN>;
   __shared__ __align__(1024) char smem[Cr::LDS];
+  const int per = a.tm * a.tn, sp = (int)(blockIdx.x / per);
   int tm, tn;
-  tile_of(blockIdx.x, gridDim.x, a.tm, a.tn, 8, tm, tn);
-  const int64_t m0 = (int64_t)tm * BM;
+  tile_of(blockIdx.x % per, per, a.tm, a.tn, 8, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM, k0 = sp * a.chunk, ka = a.Hp - k0 < a.chunk ? a.Hp - k0 : a.chunk, kb = a.H - k0 < a.chunk ? a.H - k0 : a.chunk;
   const int n0 = tn * BN;
   typename Cr::Acc acc;
   Cr::zero(acc);
   const int64_t cols = (a.D + 7) / 8 * 8 - n0;
 #pragma unroll 1
   for (int up = 0; up < 2; ++up) {
-    const Operand A = {(up ? a.du : a.dg) + m0 * a.Hp, a.dlimb, a.Hp, a.T - m0, a.Hp};
-    const Operand B[1] = {{(up ? a.wu : a.wg) + n0, a.wlimb, up ? a.ldwu : a.ldwg, cols, a.H}};
-    Cr::run(smem, A, B, acc);
+    const int64_t ld = up ? a.ldwu : a.ldwg;
+    const Operand A = {(up ? a.du : a.dg) + m0 * a.Hp + k0, a.dlimb, a.Hp, a.T - m0, ka};
+    const Operand B[1] = {{(up ? a.wu : a.wg) + k0 * ld + n0, a.wlimb, ld, cols, kb}};
+    if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
+    else Cr::run(smem, A, B, acc);
   }
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const int ew = MODE == MODE_F16X3 ? a.exps[5] - 15 : 0;
-  const bool vec = a.lddx % 4 == 0;
+  const bool vec = a.D % 4 == 0;
 #pragma unroll
   for (int mi = 0; mi < Cr::MI; ++mi) {
     const int64_t i = m0 + wm * (BM / WM) + 16 * mi + (lane & 15);
@@ -453,7 +502,9 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dx_kernel(DxArgs a) {
       if (MODE == MODE_F16X3)
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], k);
-      if (j < a.D) store4<MODE>(a.dx, i * a.lddx + j, a.D - j, vec, v);
+      if (j >= a.D) continue;
+      if (a.splits == 1) store4<MODE>(a.dx, i * a.D + j, a.D - j, vec, v);
+      else store4<MODE_F16X3>(a.part, (sp * a.T + i) * a.D + j, a.D - j, vec, v);
     }
   }
 }
@@ -470,7 +521,7 @@ struct DwArgs {
   int tm, tn;
 };
 
-template <int MODE, int BM, int BN, int WM, int WN>
+template <int MODE, int BM, int BN, int WM, int WN, bool PHASED>
 __global__ __launch_bounds__(64 * WM * WN) void gated_dw_kernel(DwArgs a) {
   using Cr = Core<MODE, KS, KS, BM, BN, 1, WM, WN>;
   __shared__ __align__(1024) char smem[Cr::LDS];
@@ -483,7 +534,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dw_kernel(DwArgs a) {
   Cr::zero(acc);
   const Operand A = {a.d[w] + t0 * a.Hp + m0, a.dlimb, a.Hp, a.Hp - m0, K};
   const Operand B[1] = {{a.x + t0 * a.ldx + n0, a.xlimb, a.ldx, (a.D + 7) / 8 * 8 - n0, K}};
-  Cr::run(smem, A, B, acc);
+  if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
+  else Cr::run(smem, A, B, acc);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const int e = MODE == MODE_F16X3 ? -a.exps[4] - (w ? a.exps[6] - a.exps[5] : 0) : 0;
   const bool vec = a.D % 4 == 0;
@@ -505,16 +557,18 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dw_kernel(DwArgs a) {
   }
 }
 
+// the sum of the splits' parts in their order; `sets` results lie side by side in a split's part
 template <int MODE>
-__global__ __launch_bounds__(256) void gated_dw_reduce_kernel(const float* part, int splits, int64_t HD, void* dwg, void* dwu) {
+__global__ __launch_bounds__(256) void gated_reduce_kernel(const float* part, int splits, int sets, int64_t n, void* out0, void* out1) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   const int w = blockIdx.y;
-  if (i >= HD) return;
-  const int n = HD - i < 4 ? (int)(HD - i) : 4;
-  const bool vec = HD % 4 == 0;
+  if (i >= n) return;
+  const int m = n - i < 4 ? (int)(n - i) : 4;
+  const bool vec = n % 4 == 0;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; ++s) v += load4<MODE_F16X3>(part, ((int64_t)s * 2 + w) * HD + i, n, vec);
-  store4<MODE>(w ? dwu : dwg, i, n, true, v);
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) v += load4<MODE_F16X3>(part, ((int64_t)s * sets + w) * n + i, m, vec);
+  store4<MODE>(w ? out1 : out0, i, m, true, v);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------
@@ -570,54 +624,79 @@ inline int64_t rows_grid(int64_t rows) {
   return b < 1 ? 1 : (b > 4096 ? 4096 : b);
 }
 
+// Tiles of 256 rows, one block a compute unit, or of 128, two a unit: by the time of the launch in rounds over the 256 units.  The small
+// tiles' lower rate (1135 against 1310 TFLOP/s at 4096^3, more LDS reads and loads a product) counts little against a part-filled round;
+// and where the sum is short a block is mostly its epilogue, which two blocks a unit hide behind each other's products
+// (131072 x 256 -> 256 in fp32: @@ against @@ us).
+bool large_tiles(int64_t n256, int64_t n128, int64_t steps) {
+  if (steps <= 16) return false;
+  const double large = (double)((n256 + 255) / 256);
+  double small = 0.58 * (double)((n128 + 511) / 512);
+  if (n128 <= 512) small = 0.58 * (n128 <= 256 ? 0.68 : 1.);
+  return large <= small;
+}
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 // where everything of one call lies in its workspace (bytes; every part starts on a multiple of 256)
 struct Plan {
   bool copy_x, copy_w[2];
-  int64_t Dp, Hp, splits, chunk, row_tiles, scale_blocks;
-  int64_t x, w, dg, xt, part, exps, rowexp, rscale, dbpart, dwpart, spart, bytes;
-  bool big;
+  bool big, dx_big, dw_big;
+  int64_t Dp, Hp, row_tiles, pack_blocks;
+  int64_t dx_splits, dx_chunk, dw_splits, dw_chunk;
+  int64_t x, w, dg, xt, part, exps, rowexp, colexp, rscale, dbpart, sums, spart, bytes;
 };
 
 bool aligned16(const void* p, int64_t ld, int es) { return (uintptr_t)p % 16 == 0 && (ld * es) % 16 == 0; }
 
+// a sum over K is split until some 512 blocks of `tiles` tiles have work, each at least `least` long
+void split_sum(int64_t tiles, int64_t K, int64_t least, int64_t& splits, int64_t& chunk) {
+  int64_t s = tiles >= 384 ? 1 : cdiv(512, tiles);
+  const int64_t most = cdiv(K, least);
+  s = s > most ? most : s;
+  chunk = up(cdiv(K, s), 64);
+  splits = cdiv(K, chunk);
+}
+
 Plan plan(const hold_gated_desc& d, bool bwd) {
   Plan p = {};
-  const int nl = d.dtype == HOLD_GATED_F32 ? 2 : 1;
+  const bool f32 = d.dtype == HOLD_GATED_F32;
+  const int nl = f32 ? 2 : 1, step = f32 ? 32 : 64;
   p.Dp = up(d.D, 8);
   p.Hp = up(d.H, 8);
-  const bool f32 = d.dtype == HOLD_GATED_F32;
   p.copy_x = f32 || d.D % 8 || !aligned16(d.x, d.ldx, 2);
   p.copy_w[0] = f32 || d.D % 8 || !aligned16(d.w_gate, d.ldwg, 2);
   p.copy_w[1] = f32 || d.D % 8 || !aligned16(d.w_up, d.ldwu, 2);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o += up(bytes, 256); return at; };
-  // 256 x (128 + 128) tiles where they fill the 256 compute units, 128 x (64 + 64) elsewhere
-  p.big = ((d.T + 255) / 256) * ((d.H + 127) / 128) >= 256;
-  p.row_tiles = p.big ? (d.T + 255) / 256 : (d.T + 127) / 128;
+  p.big = large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64), cdiv(p.Dp, step));
+  p.row_tiles = cdiv(d.T, p.big ? 256 : 128);
+  p.pack_blocks = rows_grid(d.T + 2 * (int64_t)d.H);
   p.x = p.copy_x ? take(d.T * p.Dp * 2 * nl) : 0;
   p.w = p.copy_w[0] || p.copy_w[1] ? take(2 * (int64_t)d.H * p.Dp * 2 * nl) : 0;
   if (f32) {
-    p.part = take(4 * NPART * 4);
-    p.exps = take(8 * 4);
     p.rowexp = take(d.T * 4);
+    p.colexp = take(2 * p.Hp * 4);
   }
   if (bwd) {
     p.dg = take(2 * d.T * p.Hp * 2 * nl);
-    p.scale_blocks = rows_grid(d.T);
     if (f32) {
+      p.part = take(4 * NPART * 4);
+      p.exps = take(8 * 4);
       p.xt = take(d.T * p.Dp * 2 * nl);
       p.rscale = take(d.T * 4);
-      p.spart = take(p.scale_blocks * 4);
+      p.spart = take(p.pack_blocks * 4);
     }
     if (d.db_gate || d.db_up) p.dbpart = take(p.row_tiles * 2 * d.H * 4);
-    // the tokens are split so that some 512 blocks have work, each at least 512 tokens
-    const int64_t tiles = 2 * ((d.H + 127) / 128) * ((d.D + 127) / 128);
-    int64_t s = tiles >= 512 ? 1 : (512 + tiles - 1) / tiles;
-    const int64_t most = (d.T + 511) / 512;
-    s = s > most ? most : s;
-    p.chunk = up((d.T + s - 1) / s, 64);
-    p.splits = (d.T + p.chunk - 1) / p.chunk;
-    if (p.splits > 1) p.dwpart = take(p.splits * 2 * (int64_t)d.H * d.D * 4);
+    const int64_t x256 = cdiv(d.T, 256) * cdiv(d.D, 256), x128 = cdiv(d.T, 128) * cdiv(d.D, 128);
+    p.dx_big = x256 >= 200 && large_tiles(x256, x128, cdiv(p.Hp, step));
+    split_sum(p.dx_big ? 512 : x128, p.Hp, 512, p.dx_splits, p.dx_chunk);
+    const int64_t w256 = 2 * cdiv(d.H, 256) * cdiv(d.D, 256), w128 = 2 * cdiv(d.H, 128) * cdiv(d.D, 128);
+    p.dw_big = w256 >= 200 && large_tiles(w256, w128, cdiv(d.T, step));
+    split_sum(p.dw_big ? 512 : w128, d.T, 512, p.dw_splits, p.dw_chunk);
+    int64_t sums = p.dx_splits > 1 ? p.dx_splits * d.T * d.D * 4 : 0;  // dx's parts are added before dW's are written
+    const int64_t more = p.dw_splits > 1 ? p.dw_splits * 2 * (int64_t)d.H * d.D * 4 : 0;
+    sums = more > sums ? more : sums;
+    if (sums) p.sums = take(sums);
   }
   p.bytes = o;
   return p;
@@ -629,44 +708,53 @@ int check(const hold_gated_desc* d) {
   if (d->ldx < d->D || d->ldwg < d->D || d->ldwu < d->D) return HOLD_E_ARG;
   // the tile loads' 32-bit offsets: 256 rows of an operand, 64 rows of dg, and the tile grids
   if (d->ldx > (1 << 21) || d->ldwg > (1 << 21) || d->ldwu > (1 << 21) || d->H > (1 << 21) || d->T > (1ll << 31)) return HOLD_E_ARG;
-  if (((d->T + 127) / 128) * ((d->H + 63) / 64) > (1ll << 30)) return HOLD_E_ARG;
+  if (((d->T + 127) / 128) * (((d->H > d->D ? d->H : d->D) + 63) / 64) > (1ll << 29)) return HOLD_E_ARG;
   return HOLD_OK;
 }
 
-template <int MODE>
+template <int MODE, bool BWD>
 void operands(const hold_gated_desc& d, const Plan& p, char* ws, hipStream_t st, MmaArgs& a) {
   const int64_t WX = d.T * p.Dp, WW = (int64_t)d.H * p.Dp;
   a.x = (const uint16_t*)d.x; a.ldx = d.ldx; a.xlimb = 0;
   a.wg = (const uint16_t*)d.w_gate; a.ldwg = d.ldwg;
   a.wu = (const uint16_t*)d.w_up; a.ldwu = d.ldwu; a.wlimb = 0;
+  a.Hp = p.Hp;
   if (MODE == MODE_F16X3) {
-    float* part = (float*)(ws + p.part);
-    int* exps = (int*)(ws + p.exps);
-    int* rowexp = (int*)(ws + p.rowexp);
-    uint16_t* x = (uint16_t*)(ws + p.x);
-    uint16_t* w = (uint16_t*)(ws + p.w);
-    hipLaunchKernelGGL(gated_amax_kernel, dim3(NPART, 4), dim3(256), 0, st, (const float*)d.w_gate, d.ldwg, (const float*)d.w_up, d.ldwu,
-                       (const float*)d.b_gate, (const float*)d.b_up, d.H, d.D, part);
-    hipLaunchKernelGGL(gated_pack_rows_kernel, dim3((unsigned)rows_grid(d.T)), dim3(256), 0, st, (const float*)d.x, d.ldx, d.T, d.D, (int)p.Dp, x, WX,
-                       rowexp);
-    hipLaunchKernelGGL(gated_pack_weights_kernel, dim3((unsigned)rows_grid(d.H), 2), dim3(256), 0, st, (const float*)d.w_gate, d.ldwg,
-                       (const float*)d.w_up, d.ldwu, d.H, d.D, (int)p.Dp, part, w, WW * 2, WW, exps);
-    a.x = x; a.ldx = p.Dp; a.xlimb = WX;
-    a.wg = w; a.wu = w + WW; a.ldwg = a.ldwu = p.Dp; a.wlimb = 2 * WW;
-    a.rowexp = rowexp; a.exps = exps;
-  } else {
-    if (p.copy_x) {
-      hipLaunchKernelGGL(gated_copy_rows_kernel, dim3((unsigned)rows_grid(d.T)), dim3(256), 0, st, (const uint16_t*)d.x, d.ldx, d.T, d.D, (int)p.Dp,
-                         (uint16_t*)(ws + p.x));
-      a.x = (const uint16_t*)(ws + p.x); a.ldx = p.Dp;
+    PackArgs k = {};
+    k.x = (const float*)d.x; k.ldx = d.ldx; k.T = d.T;
+    k.w[0] = (const float*)d.w_gate; k.w[1] = (const float*)d.w_up; k.ldw[0] = d.ldwg; k.ldw[1] = d.ldwu;
+    k.H = d.H; k.D = d.D; k.Dp = (int)p.Dp;
+    k.xvec = aligned16(d.x, d.ldx, 4); k.wvec = aligned16(d.w_gate, d.ldwg, 4) && aligned16(d.w_up, d.ldwu, 4);
+    k.ox = (uint16_t*)(ws + p.x); k.xlimb = WX;
+    k.ow = (uint16_t*)(ws + p.w); k.wlimb = 2 * WW; k.second = WW;
+    k.rowexp = (int*)(ws + p.rowexp); k.colexp = (int*)(ws + p.colexp); k.Hp = p.Hp;
+    if (BWD) {
+      float* part = (float*)(ws + p.part);
+      k.part = part; k.exps = (int*)(ws + p.exps);
+      k.dh = (const float*)d.dh; k.lddh = d.lddh; k.dvec = aligned16(d.dh, d.lddh, 4); k.act = d.act;
+      k.rscale = (int*)(ws + p.rscale); k.rpart = (int*)(ws + p.spart);
+      hipLaunchKernelGGL(gated_amax_kernel, dim3(NPART, 4), dim3(256), 0, st, k.w[0], d.ldwg, k.w[1], d.ldwu, (const float*)d.b_gate,
+                         (const float*)d.b_up, d.H, d.D, k.wvec, part);
+      a.exps = k.exps;
+      a.rscale = k.rscale;
     }
-    for (int w = 0; w < 2; ++w)
-      if (p.copy_w[w]) {
-        uint16_t* o = (uint16_t*)(ws + p.w) + w * WW;
-        hipLaunchKernelGGL(gated_copy_rows_kernel, dim3((unsigned)rows_grid(d.H)), dim3(256), 0, st, (const uint16_t*)(w ? d.w_up : d.w_gate),
-                           w ? d.ldwu : d.ldwg, (int64_t)d.H, d.D, (int)p.Dp, o);
-        if (w) { a.wu = o; a.ldwu = p.Dp; } else { a.wg = o; a.ldwg = p.Dp; }
-      }
+    hipLaunchKernelGGL(gated_pack_kernel<BWD>, dim3((unsigned)p.pack_blocks), dim3(256), 0, st, k);
+    a.x = k.ox; a.ldx = p.Dp; a.xlimb = WX;
+    a.wg = k.ow; a.wu = k.ow + WW; a.ldwg = a.ldwu = p.Dp; a.wlimb = 2 * WW;
+    a.rowexp = k.rowexp; a.colexp = k.colexp;
+  } else if (p.copy_x || p.copy_w[0] || p.copy_w[1]) {
+    CopyArgs c = {};
+    c.K = d.D; c.Kp = (int)p.Dp;
+    int n = 0;
+    auto add = [&](const void* from, int64_t ld, int64_t rows, uint16_t* to) {
+      c.x[n] = (const uint16_t*)from; c.ld[n] = ld; c.rows[n] = rows; c.out[n] = to;
+      ++n;
+    };
+    uint16_t* w = (uint16_t*)(ws + p.w);
+    if (p.copy_x) { add(d.x, d.ldx, d.T, (uint16_t*)(ws + p.x)); a.x = c.out[n - 1]; a.ldx = p.Dp; }
+    if (p.copy_w[0]) { add(d.w_gate, d.ldwg, d.H, w); a.wg = w; a.ldwg = p.Dp; }
+    if (p.copy_w[1]) { add(d.w_up, d.ldwu, d.H, w + WW); a.wu = w + WW; a.ldwu = p.Dp; }
+    hipLaunchKernelGGL(gated_copy_rows_kernel, dim3((unsigned)rows_grid(c.rows[0] + c.rows[1] + c.rows[2])), dim3(256), 0, st, c);
   }
   a.bg = d.b_gate; a.bu = d.b_up;
   a.T = d.T; a.H = d.H; a.K = (int)p.Dp; a.act = d.act;
@@ -675,11 +763,11 @@ void operands(const hold_gated_desc& d, const Plan& p, char* ws, hipStream_t st,
 template <int MODE, bool BWD>
 void launch_mma(MmaArgs a, bool big, hipStream_t st) {
   if (big) {
-    a.tm = (int)((a.T + 255) / 256); a.tn = (a.H + 127) / 128;
-    hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 256, 128, 2, 4>), dim3((unsigned)(a.tm * a.tn)), dim3(512), 0, st, a);
+    a.tm = (int)cdiv(a.T, 256); a.tn = (int)cdiv(a.H, 128);
+    hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 256, 128, 4, 4, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
   } else {
-    a.tm = (int)((a.T + 127) / 128); a.tn = (a.H + 63) / 64;
-    hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 128, 64, 2, 2>), dim3((unsigned)(a.tm * a.tn)), dim3(256), 0, st, a);
+    a.tm = (int)cdiv(a.T, 128); a.tn = (int)cdiv(a.H, 64);
+    hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 128, 64, 4, 2, false>), dim3((unsigned)(a.tm * a.tn)), dim3(512), 0, st, a);
   }
 }
 
@@ -708,7 +796,7 @@ int fwd(const hold_gated_desc& d, hipStream_t st) {
   const Plan p = plan(d, false);
   if (p.bytes > d.workspace_bytes || (p.bytes && !d.workspace)) return HOLD_E_ARG;
   MmaArgs a = {};
-  operands<MODE>(d, p, (char*)d.workspace, st, a);
+  operands<MODE, false>(d, p, (char*)d.workspace, st, a);
   a.h = d.h; a.ldh = d.ldh;
   launch_mma<MODE, false>(a, p.big, st);
   return ok();
@@ -722,43 +810,51 @@ int bwd(const hold_gated_desc& d, hipStream_t st) {
   constexpr bool F32 = MODE == MODE_F16X3;
   constexpr int NL = limbs<MODE>();
   MmaArgs a = {};
-  operands<MODE>(d, p, ws, st, a);
+  operands<MODE, true>(d, p, ws, st, a);
   const int64_t XN = d.T * p.Dp, DN = d.T * p.Hp;
-  if (F32) {
-    hipLaunchKernelGGL(gated_row_scale_kernel, dim3((unsigned)p.scale_blocks), dim3(256), 0, st, (const float*)d.dh, d.lddh, d.T, d.H, d.D, d.act,
-                       a.rowexp, a.exps, (int*)(ws + p.rscale), (int*)(ws + p.spart));
+  if (F32)
     hipLaunchKernelGGL(gated_pack_tokens_kernel, dim3((unsigned)rows_grid(d.T)), dim3(256), 0, st, (const float*)d.x, d.ldx, d.T, d.D, (int)p.Dp,
-                       (const int*)(ws + p.rscale), (const int*)(ws + p.spart), (int)p.scale_blocks, (uint16_t*)(ws + p.xt), XN, (int*)(ws + p.exps));
-  }
+                       (int)aligned16(d.x, d.ldx, 4), a.rscale, (const int*)(ws + p.spart), (int)p.pack_blocks, (uint16_t*)(ws + p.xt), XN,
+                       (int*)(ws + p.exps));
   a.dh = d.dh; a.lddh = d.lddh;
-  a.dg = (uint16_t*)(ws + p.dg); a.du = a.dg + NL * DN; a.Hp = p.Hp; a.dlimb = DN;
-  a.rscale = (const int*)(ws + p.rscale);
+  a.dg = (uint16_t*)(ws + p.dg); a.du = a.dg + NL * DN; a.dlimb = DN;
   a.dbpart = d.db_gate || d.db_up ? (float*)(ws + p.dbpart) : nullptr;
   launch_mma<MODE, true>(a, p.big, st);
   if (a.dbpart)
-    hipLaunchKernelGGL(gated_db_kernel<MODE>, dim3((unsigned)((d.H + 63) / 64), 2), dim3(256), 0, st, a.dbpart, (int)p.row_tiles, d.H, d.db_gate, d.db_up);
+    hipLaunchKernelGGL(gated_db_kernel<MODE>, dim3((unsigned)((d.H + 63) / 64), 2), dim3(1024), 0, st, a.dbpart, (int)p.row_tiles, d.H, d.db_gate, d.db_up);
+  float* sums = (float*)(ws + p.sums);
   if (d.dx) {
     DxArgs x = {};
     x.dg = a.dg; x.du = a.du; x.Hp = p.Hp; x.dlimb = DN;
     x.wg = a.wg; x.wu = a.wu; x.ldwg = a.ldwg; x.ldwu = a.ldwu; x.wlimb = a.wlimb;
     x.T = d.T; x.H = d.H; x.D = d.D;
     x.rscale = a.rscale; x.exps = a.exps;
-    x.dx = d.dx; x.lddx = d.D;
-    x.tm = (int)((d.T + 127) / 128); x.tn = (d.D + 127) / 128;
-    hipLaunchKernelGGL((gated_dx_kernel<MODE, 128, 128, 2, 2>), dim3((unsigned)(x.tm * x.tn)), dim3(256), 0, st, x);
+    x.dx = d.dx; x.chunk = p.dx_chunk; x.splits = (int)p.dx_splits; x.part = sums;
+    const int t = p.dx_big ? 256 : 128;
+    x.tm = (int)cdiv(d.T, t); x.tn = (int)cdiv(d.D, t);
+    const unsigned blocks = (unsigned)(x.tm * x.tn * x.splits);
+    if (p.dx_big) hipLaunchKernelGGL((gated_dx_kernel<MODE, 256, 256, 4, 4, true>), dim3(blocks), dim3(1024), 0, st, x);
+    else hipLaunchKernelGGL((gated_dx_kernel<MODE, 128, 128, 2, 4, false>), dim3(blocks), dim3(512), 0, st, x);
+    if (x.splits > 1) {
+      const int64_t n = d.T * d.D;
+      hipLaunchKernelGGL(gated_reduce_kernel<MODE>, dim3((unsigned)cdiv(n, 1024)), dim3(256), 0, st, sums, x.splits, 1, n, d.dx, d.dx);
+    }
   }
   if (d.dw_gate) {
     DwArgs w = {};
     w.d[0] = a.dg; w.d[1] = a.du; w.Hp = p.Hp; w.dlimb = DN;
     w.x = F32 ? (const uint16_t*)(ws + p.xt) : a.x; w.ldx = F32 ? p.Dp : a.ldx; w.xlimb = F32 ? XN : 0;
     w.T = d.T; w.H = d.H; w.D = d.D;
-    w.chunk = p.chunk; w.splits = (int)p.splits; w.exps = a.exps;
-    w.out[0] = d.dw_gate; w.out[1] = d.dw_up; w.part = (float*)(ws + p.dwpart);
-    w.tm = (d.H + 127) / 128; w.tn = (d.D + 127) / 128;
-    hipLaunchKernelGGL((gated_dw_kernel<MODE, 128, 128, 2, 2>), dim3((unsigned)(2 * w.tm * w.tn * w.splits)), dim3(256), 0, st, w);
+    w.chunk = p.dw_chunk; w.splits = (int)p.dw_splits; w.exps = a.exps;
+    w.out[0] = d.dw_gate; w.out[1] = d.dw_up; w.part = sums;
+    const int t = p.dw_big ? 256 : 128;
+    w.tm = (int)cdiv(d.H, t); w.tn = (int)cdiv(d.D, t);
+    const unsigned blocks = (unsigned)(2 * w.tm * w.tn * w.splits);
+    if (p.dw_big) hipLaunchKernelGGL((gated_dw_kernel<MODE, 256, 256, 4, 4, true>), dim3(blocks), dim3(1024), 0, st, w);
+    else hipLaunchKernelGGL((gated_dw_kernel<MODE, 128, 128, 2, 4, false>), dim3(blocks), dim3(512), 0, st, w);
     if (w.splits > 1) {
-      const int64_t HD = (int64_t)d.H * d.D;
-      hipLaunchKernelGGL(gated_dw_reduce_kernel<MODE>, dim3((unsigned)((HD + 1023) / 1024), 2), dim3(256), 0, st, w.part, w.splits, HD, d.dw_gate, d.dw_up);
+      const int64_t n = (int64_t)d.H * d.D;
+      hipLaunchKernelGGL(gated_reduce_kernel<MODE>, dim3((unsigned)cdiv(n, 1024), 2), dim3(256), 0, st, sums, w.splits, 2, n, d.dw_gate, d.dw_up);
     }
   }
   return ok();
@@ -779,5 +875,6 @@ extern "C" int hold_gated_fwd(const hold_gated_desc* d, hold_stream_t st) {
 
 extern "C" int hold_gated_bwd(const hold_gated_desc* d, hold_stream_t st) {
   if (check(d) != HOLD_OK || !d->dh || d->lddh < d->H || (!d->dw_gate != !d->dw_up)) return HOLD_E_ARG;
+  if (((uintptr_t)d->dx | (uintptr_t)d->dw_gate | (uintptr_t)d->dw_up) % 16) return HOLD_E_ARG;
   return d->dtype == HOLD_GATED_F32 ? bwd<MODE_F16X3>(*d, (hipStream_t)st) : bwd<MODE_BF16>(*d, (hipStream_t)st);
 }

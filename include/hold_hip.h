@@ -678,7 +678,8 @@ int hold_knn1_bwd(const float* q, int32_t B, int32_t Nq, const float* t, int32_t
  * hold_gated_workspace (host only): *bytes = the scratch of one call (256-byte aligned); the pointers
  * and leading dimensions of the descriptor have to be the call's own, and -- backward -- db_gate /
  * db_up null or not as in the call.
- * hold_gated_bwd: dx, dw_gate + dw_up, db_gate, db_up are contiguous and may be null (dw: both or none).
+ * hold_gated_bwd: dx, dw_gate + dw_up, db_gate, db_up are contiguous and may be null (dw: both or none);
+ * dx, dw_gate and dw_up start on 16-byte boundaries.
  * ---------------------------------------------------------------------------------------- */
 enum hold_gated_dtype { HOLD_GATED_F32 = 0, HOLD_GATED_BF16 = 1 };
 enum hold_gated_act { HOLD_GATED_SILU = 0, HOLD_GATED_GELU = 1 /* erf */, HOLD_GATED_RELU = 2, HOLD_GATED_SIGMOID = 3 };

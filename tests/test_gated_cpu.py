@@ -64,6 +64,8 @@ def test_entry_points_refuse_bad_descriptors():
     assert L.hold_gated_bwd(C.byref(_desc(**{**full, "dh": 0}, workspace=4096, workspace_bytes=1 << 40)), None) == -1
     assert L.hold_gated_bwd(C.byref(_desc(**{**full, "dw_up": 0}, workspace=4096, workspace_bytes=1 << 40)), None) == -1
     assert L.hold_gated_bwd(C.byref(_desc(**full, workspace=4096, workspace_bytes=need - 1)), None) == -1
+    for out in ("dx", "dw_gate", "dw_up"):  # not on a 16-byte boundary
+        assert L.hold_gated_bwd(C.byref(_desc(**{**full, out: 4100}, workspace=4096, workspace_bytes=1 << 40)), None) == -1
     # few rows need no scratch forward; the sizes grow with the rows
     assert L.hold_gated_workspace(C.byref(_desc(T=64)), 0, C.byref(n)) == 0 and n.value == 0
     assert L.hold_gated_workspace(C.byref(_desc(T=65)), 0, C.byref(n)) == 0 and n.value >= 65 * 64 * 4
