@@ -25,20 +25,53 @@ namespace {
 
 enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2, ACT_SIGMOID = 3 };
 
-__device__ __forceinline__ float sigmoid_f(float g) { return 1.f / (1.f + expf(-g)); }
+// e^x by v_exp_f32 (2^x to 1 ulp).  EXACT: the product x log2 e in two parts, 2^-23 relative; else its rounding alone, |x| 2^-24, which is
+// nothing to a result in bf16
+template <bool EXACT>
+__device__ __forceinline__ float exp_of(float x) {
+  const float p = x * 1.44269504088896341f;
+  if (!EXACT) return __builtin_amdgcn_exp2f(p);
+  const float lo = fmaf(x, 1.44269504088896341f, -p) + x * 1.925962989e-8f;  // log2 e = 1.4426950216... + 1.926e-8 in float32
+  const float e = __builtin_amdgcn_exp2f(p);
+  return fabsf(p) < 200.f ? e * fmaf(lo, 0.693147180559945f, 1.f) : e;  // beyond: 0 or infinity
+}
+// 1 / x for x in [1, inf], by v_rcp_f32 (1 ulp) and, EXACT, a Newton step; 1 / inf = 0
+template <bool EXACT>
+__device__ __forceinline__ float recip(float x) {
+  const float r = __builtin_amdgcn_rcpf(x);
+  return EXACT && r > 0.f ? fmaf(fmaf(-x, r, 1.f), r, r) : r;
+}
+// the normal distribution function, 0.5 erfc(-g / sqrt 2).  erfc(z), z >= 0, by W. H. Press et al., "Numerical Recipes" (6.2, erfcc): t e^(-z^2 +
+// P(t)), t = 1 / (1 + z / 2), fractional error below 1.2e-7 everywhere
+template <bool EXACT>
+__device__ __forceinline__ float normal_cdf(float g) {
+  const float z = 0.70710678118654752f * fabsf(g), t = recip<EXACT>(fmaf(0.5f, z, 1.f));
+  float p = 0.17087277f;
+  p = fmaf(p, t, -0.82215223f);
+  p = fmaf(p, t, 1.48851587f);
+  p = fmaf(p, t, -1.13520398f);
+  p = fmaf(p, t, 0.27886807f);
+  p = fmaf(p, t, -0.18628806f);
+  p = fmaf(p, t, 0.09678418f);
+  p = fmaf(p, t, 0.37409196f);
+  p = fmaf(p, t, 1.00002368f);
+  p = fmaf(p, t, -1.26551223f);
+  const float e = 0.5f * t * exp_of<EXACT>(fmaf(-z, z, p));
+  return g > 0.f ? 1.f - e : e;
+}
 
 // act(g) and act'(g)
-template <bool DERIV>
+template <bool DERIV, bool EXACT>
 __device__ __forceinline__ void activate(int act, float g, float& a, float& da) {
   if (act == ACT_RELU) {
     a = g > 0.f ? g : (g == g ? 0.f : g);
     da = g > 0.f ? 1.f : (g == g ? 0.f : g);
   } else if (act == ACT_GELU) {
-    const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
+    const float phi = normal_cdf<EXACT>(g);
     a = g * phi;
-    if (DERIV) da = phi + g * (0.39894228040143268f * expf(-0.5f * g * g));
+    if (DERIV) da = phi + g * (0.39894228040143268f * exp_of<EXACT>(-0.5f * g * g));
   } else {
-    const float s = sigmoid_f(g);
+    const float s = recip<EXACT>(1.f + exp_of<EXACT>(-g));
     if (act == ACT_SIGMOID) {
       a = s;
       if (DERIV) da = s * (1.f - s);
@@ -332,6 +365,17 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
   const bool hvec = BWD ? (a.lddh % 4 == 0 && (uintptr_t)a.dh % (4 * ES) == 0) : (a.ldh % 4 == 0 && (uintptr_t)a.h % (4 * ES) == 0);
   const bool bvec = (uintptr_t)a.bg % (4 * ES) == 0 && (uintptr_t)a.bu % (4 * ES) == 0;
   float* sums = (float*)smem;  // [WM][2][BN]
+  f32x4 dhs[BWD ? Cr::NI : 1][BWD ? Cr::MI : 1];  // all of them requested before the first store
+  if (BWD) {
+#pragma unroll
+    for (int ni = 0; ni < Cr::NI; ++ni)
+#pragma unroll
+      for (int mi = 0; mi < Cr::MI; ++mi) {
+        const int j = n0 + wn * (BN / WN) + 16 * ni + 4 * (lane >> 4), n = a.H - j;
+        const int64_t i = m0 + wm * (BM / WM) + 16 * mi + (lane & 15);
+        dhs[BWD ? ni : 0][BWD ? mi : 0] = i < a.T && n > 0 ? load4<MODE>(a.dh, i * a.lddh + j, n, hvec) : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+  }
 #pragma unroll
   for (int ni = 0; ni < Cr::NI; ++ni) {
     const int jt = wn * (BN / WN) + 16 * ni + 4 * (lane >> 4), j = n0 + jt, n = a.H - j;
@@ -367,18 +411,18 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float s, d;
-          activate<false>(a.act, g[r], s, d);
+          activate<false, MODE == MODE_F16X3>(a.act, g[r], s, d);
           h[r] = s * u[r];
         }
         if (row && n > 0) store4<MODE>(a.h, i * a.ldh + j, n, hvec, h);
       } else {
         f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = dg;
         if (row && n > 0) {
-          const f32x4 dh = load4<MODE>(a.dh, i * a.lddh + j, n, hvec);
+          const f32x4 dh = dhs[ni][mi];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             float s, d;
-            activate<true>(a.act, g[r], s, d);
+            activate<true, MODE == MODE_F16X3>(a.act, g[r], s, d);
             dg[r] = r < n ? dh[r] * u[r] * d : 0.f;
             du[r] = r < n ? dh[r] * s : 0.f;
           }
@@ -612,7 +656,7 @@ __global__ __launch_bounds__(256) void gated_rows_kernel(const void* x, int64_t 
   for (int t = 0; t < NT; ++t)
     if (lane == t && t0 + t < T) {
       float s, d;
-      activate<false>(act, g[t] + vg, s, d);
+      activate<false, MODE == MODE_F16X3>(act, g[t] + vg, s, d);
       store1<MODE>(h, (t0 + t) * ldh + j, s * (u[t] + vu));
     }
 }
