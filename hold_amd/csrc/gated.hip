@@ -616,49 +616,162 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(const float* part, in
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------
-// T <= 64: the weights are read once, by fours of lanes along k; a wave holds 4 output columns (2 of each matrix... see RowsGeom) and
-// all rows' sums.  fp32 arithmetic throughout: 2 T operations a weight element stay below the time of its bytes up to T = 64 in bf16.
+// T <= 64: bound by the weights' bytes, which are read once, 16 a lane, as they are; no product of limbs, fp32 keeps fp32 arithmetic.
 constexpr int ROWS_MAX = 64;
+template <int MODE> constexpr int chunk_k() { return MODE == MODE_BF16 ? 8 : 4; }  // elements in 16 bytes
 
-template <int MODE, int NT>
-__global__ __launch_bounds__(256) void gated_rows_kernel(const void* x, int64_t ldx, const void* wg, int64_t ldwg, const void* wu, int64_t ldwu,
-                                                         const void* bg, const void* bu, int T, int D, int H, int act, void* h, int64_t ldh, int xvec,
-                                                         int wvec) {
-  const int lane = threadIdx.x & 63, j = blockIdx.x * 4 + (threadIdx.x >> 6), t0 = blockIdx.y * NT;
-  if (j >= H) return;
-  float g[NT], u[NT];
+// 16 bytes of a row from element c on, zeros from element K on; `vec`: rows start on 16-byte boundaries
+template <int MODE>
+__device__ __forceinline__ u32x4 chunk16(const void* p, int64_t at, int c, int K, bool vec) {
+  constexpr int N = chunk_k<MODE>();
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (vec && c + N <= K) return MODE == MODE_BF16 ? *(const u32x4*)((const uint16_t*)p + at + c) : *(const u32x4*)((const float*)p + at + c);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) g[t] = u[t] = 0.f;
-  for (int c = lane * 4; c < D; c += 256) {
-    const int n = D - c;
-    const f32x4 a = load4<MODE>(wg, j * ldwg + c, n, wvec), b = load4<MODE>(wu, j * ldwu + c, n, wvec);
+  for (int i = 0; i < N; ++i)
+    if (c + i < K) {
+      if (MODE == MODE_BF16) v[i >> 1] |= (uint32_t)((const uint16_t*)p)[at + c + i] << (16 * (i & 1));
+      else v[i] = ((const uint32_t*)p)[at + c + i];
+    }
+  return v;
+}
+template <int MODE>
+__device__ __forceinline__ float lane_value(u32x4 v, int i) {
+  const uint32_t w = MODE == MODE_BF16 ? v[i >> 1] : v[i];  // a copy: __builtin_bit_cast of a vector's element reads element 0
+  return __builtin_bit_cast(float, MODE == MODE_BF16 ? (i & 1 ? w & 0xffff0000u : w << 16) : w);
+}
+
+struct RowsArgs {
+  const void* x; int64_t ldx;
+  const void* w[2]; int64_t ldw[2];
+  const void* b[2];
+  void* h; int64_t ldh;
+  int T, D, H, act, xvec, wvec;
+};
+
+// T <= 4: dot products, a wave computes NC columns of both projections for all rows, its lanes along k (4 x 4096 -> 8192 in bf16, 134 MB of
+// weights: @@ us; one column a wave reads x as often as the weights and took 56)
+template <int MODE, int NT, int NC>
+__global__ __launch_bounds__(256) void gated_rows_kernel(RowsArgs a) {
+  constexpr int N = chunk_k<MODE>();
+  const int lane = threadIdx.x & 63, j0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * NC;
+  if (j0 >= a.H) return;
+  float s[2][NC][NT];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s[w][n][t] = 0.f;
+  for (int c = lane * N; c < a.D; c += 64 * N) {
+    u32x4 v[2][NC], x[NT];
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) v[w][n] = chunk16<MODE>(a.w[w], (j0 + n < a.H ? j0 + n : a.H - 1) * a.ldw[w], c, a.D, a.wvec);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) x[t] = chunk16<MODE>(a.x, (t < a.T ? t : a.T - 1) * a.ldx, c, a.D, a.xvec);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const float y = lane_value<MODE>(v[w][n], i);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) s[w][n][t] = fmaf(y, lane_value<MODE>(x[t], i), s[w][n][t]);
+        }
+  }
+  float g = 0.f, u = 0.f;  // lane n NT + t keeps column n of row t
+#pragma unroll
+  for (int n = 0; n < NC; ++n)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      if (t0 + t < T) {
-        const f32x4 v = load4<MODE>(x, (t0 + t) * ldx + c, n, xvec);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          g[t] = fmaf(a[r], v[r], g[t]);
-          u[t] = fmaf(b[r], v[r], u[t]);
-        }
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) s[w][n][t] += __shfl_xor(s[w][n][t], o, 64);
+      if (lane == n * NT + t) {
+        g = s[0][n][t];
+        u = s[1][n][t];
       }
     }
+  const int j = j0 + lane / NT, t = lane % NT;
+  if (lane < NC * NT && j < a.H && t < a.T) {
+    if (a.b[0]) g += load1<MODE>(a.b[0], j);
+    if (a.b[1]) u += load1<MODE>(a.b[1], j);
+    float f, d;
+    activate<false, MODE == MODE_F16X3>(a.act, g, f, d);
+    store1<MODE>(a.h, t * a.ldh + j, f * u);
   }
+}
+
+// 4 < T <= 64: 16 columns a block on the matrix cores (bf16: 16x16x32; fp32: 16x16x4, fp32 operands), the weights' chunks going straight from
+// memory into the first operand's registers; the block's four waves take every fourth group of k, their sums meet in LDS.
+// In fp32 a lane's four k's feed four instructions: k runs in another order, the same for both operands.
+template <int MODE, int NB>
+__global__ __launch_bounds__(256) void gated_few_kernel(RowsArgs a) {
+  constexpr int N = chunk_k<MODE>(), STEP = 4 * N, U = 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j0 = blockIdx.x * 16, r = lane & 15, kl = (lane >> 4) * N;
+  const int jr = j0 + r < a.H ? j0 + r : a.H - 1;
+  f32x4 acc[2][NB];
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int w = 0; w < 2; ++w)
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      g[t] += __shfl_xor(g[t], o, 64);
-      u[t] += __shfl_xor(u[t], o, 64);
+    for (int n = 0; n < NB; ++n) acc[w][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k0 = wave * STEP * U; k0 < a.D; k0 += 4 * STEP * U) {
+    u32x4 v[U][2], x[U][NB];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) v[i][w] = chunk16<MODE>(a.w[w], jr * a.ldw[w], k0 + i * STEP + kl, a.D, a.wvec);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) x[i][n] = chunk16<MODE>(a.x, (16 * n + r < a.T ? 16 * n + r : a.T - 1) * a.ldx, k0 + i * STEP + kl, a.D, a.xvec);
     }
-  const float vg = bg ? load1<MODE>(bg, j) : 0.f, vu = bu ? load1<MODE>(bu, j) : 0.f;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-    if (lane == t && t0 + t < T) {
-      float s, d;
-      activate<false, MODE == MODE_F16X3>(act, g[t] + vg, s, d);
-      store1<MODE>(h, (t0 + t) * ldh + j, s * (u[t] + vu));
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (MODE == MODE_BF16) {
+            acc[w][n] = mfma<MODE_BF16>(__builtin_bit_cast(s16x8, v[i][w]), __builtin_bit_cast(s16x8, x[i][n]), acc[w][n]);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              acc[w][n] = __builtin_amdgcn_mfma_f32_16x16x4f32(lane_value<MODE>(v[i][w], q), lane_value<MODE>(x[i][n], q), acc[w][n], 0, 0, 0);
+          }
+        }
+  }
+  __shared__ f32x4 part[3][2][NB][64];
+  if (wave) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) part[wave - 1][w][n][lane] = acc[w][n];
+  }
+  __syncthreads();
+  if (wave) return;
+  const int j = j0 + 4 * (lane >> 4), n4 = a.H - j;  // a lane: four columns of row 16 n + r
+  if (n4 <= 0) return;
+  constexpr int ES = MODE == MODE_BF16 ? 2 : 4;
+  const bool bvec = (uintptr_t)a.b[0] % (4 * ES) == 0 && (uintptr_t)a.b[1] % (4 * ES) == 0, hvec = a.ldh % 4 == 0 && (uintptr_t)a.h % (4 * ES) == 0;
+  f32x4 bias[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) bias[w] = a.b[w] ? load4<MODE>(a.b[w], j, n4, bvec) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int t = 16 * n + r;
+    f32x4 h;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) acc[w][n] = ((acc[w][n] + part[0][w][n][lane]) + part[1][w][n][lane]) + part[2][w][n][lane] + bias[w];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float f, d;
+      activate<false, MODE == MODE_F16X3>(a.act, acc[0][n][q], f, d);
+      h[q] = f * acc[1][n][q];
     }
+    if (t < a.T) store4<MODE>(a.h, t * a.ldh + j, n4, hvec, h);
+  }
 }
 
 inline int ok() { return hipGetLastError() == hipSuccess ? HOLD_OK : HOLD_E_LAUNCH; }
@@ -818,17 +931,26 @@ void launch_mma(MmaArgs a, bool big, hipStream_t st) {
 template <int MODE>
 void rows(const hold_gated_desc& d, hipStream_t st) {
   constexpr int ES = MODE == MODE_BF16 ? 2 : 4;
-  const int xvec = d.ldx % 4 == 0 && (uintptr_t)d.x % (4 * ES) == 0;
-  const int wvec = d.ldwg % 4 == 0 && d.ldwu % 4 == 0 && (uintptr_t)d.w_gate % (4 * ES) == 0 && (uintptr_t)d.w_up % (4 * ES) == 0;
-  const dim3 block(256);
-  const unsigned gx = (unsigned)((d.H + 3) / 4);
-#define HOLD_ROWS(NT) \
-  hipLaunchKernelGGL((gated_rows_kernel<MODE, NT>), dim3(gx, (unsigned)((d.T + NT - 1) / NT)), block, 0, st, d.x, d.ldx, d.w_gate, d.ldwg, d.w_up, \
-                     d.ldwu, d.b_gate, d.b_up, (int)d.T, d.D, d.H, d.act, d.h, d.ldh, xvec, wvec)
-  if (d.T == 1) HOLD_ROWS(1);
-  else if (d.T <= 4) HOLD_ROWS(4);
-  else HOLD_ROWS(16);
+  RowsArgs a = {};
+  a.x = d.x; a.ldx = d.ldx;
+  a.w[0] = d.w_gate; a.w[1] = d.w_up; a.ldw[0] = d.ldwg; a.ldw[1] = d.ldwu;
+  a.b[0] = d.b_gate; a.b[1] = d.b_up;
+  a.h = d.h; a.ldh = d.ldh;
+  a.T = (int)d.T; a.D = d.D; a.H = d.H; a.act = d.act;
+  a.xvec = aligned16(d.x, d.ldx, ES);
+  a.wvec = aligned16(d.w_gate, d.ldwg, ES) && aligned16(d.w_up, d.ldwu, ES);
+  // four columns a wave where that still leaves two waves a SIMD, one elsewhere
+#define HOLD_ROWS(NT, NC) hipLaunchKernelGGL((gated_rows_kernel<MODE, NT, NC>), dim3((unsigned)cdiv(d.H, 4 * NC)), dim3(256), 0, st, a)
+#define HOLD_FEW(NB) hipLaunchKernelGGL((gated_few_kernel<MODE, NB>), dim3((unsigned)cdiv(d.H, 16)), dim3(256), 0, st, a)
+  const bool wide = d.H >= 4096;
+  if (d.T == 1) { if (wide) HOLD_ROWS(1, 4); else HOLD_ROWS(1, 1); }
+  else if (d.T == 2) { if (wide) HOLD_ROWS(2, 4); else HOLD_ROWS(2, 1); }
+  else if (d.T <= 4) { if (wide) HOLD_ROWS(4, 4); else HOLD_ROWS(4, 1); }
+  else if (d.T <= 16) HOLD_FEW(1);
+  else if (d.T <= 32) HOLD_FEW(2);
+  else HOLD_FEW(4);
 #undef HOLD_ROWS
+#undef HOLD_FEW
 }
 
 template <int MODE>

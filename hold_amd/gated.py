@@ -6,8 +6,8 @@ is a second projection's gate.  ``gated_linear`` takes weights in ``nn.Linear``'
 
 Arithmetic: float32 tensors through two-limb fp16 products with float32 accumulation (errors of float32's own size), bfloat16 tensors
 through bf16 products with float32 accumulation, rounded once at the end; in the backward pass of bfloat16, dL/dg and dL/du are rounded
-to bfloat16 once as operands of the next products.  Results do not depend on the other rows of a batch, except that above 64 rows
-another kernel (of the same accuracy) computes them.  The backward pass computes the projections again instead of keeping them: a call
+to bfloat16 once as operands of the next products.  Results do not depend on the other rows of a batch, except that up to 4 and up to
+64 rows other kernels (of the same accuracy) compute them.  The backward pass computes the projections again instead of keeping them: a call
 keeps its inputs only.  All sums have a fixed order.
 """
 from __future__ import annotations
@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import GatedDesc, check, ptr, stream_ptr
+from ._lib import GatedDesc, check, stream_ptr
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -26,35 +26,60 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 def _rows(t):
     """[..., n] as [rows, n] with a unit inner stride and a positive row stride of at least n (copied where it is not so already)"""
-    t = t.reshape(-1, t.shape[-1])
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        t = t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if not t.is_contiguous():
+        rows, n = t.shape
+        ld, inner = t.stride()
+        if n > 1 and inner != 1 or rows > 1 and ld < n:
+            t = t.contiguous()
     return t
 
 
-def _ld(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _descriptor(x, w_gate, w_up, b_gate, b_up, act):
+def _call(act, x, w_gate, w_up, b_gate, b_up, h, dh, out):
+    """one launch sequence on the current stream: the forward pass into ``h``, or the backward pass from ``dh`` into ``out``"""
+    x, w_gate, w_up = _rows(x), _rows(w_gate), _rows(w_up)
+    T, D = x.shape
+    H = w_gate.shape[0]
     d = GatedDesc()
-    d.x, d.ldx = ptr(x), _ld(x)
-    d.w_gate, d.ldwg, d.w_up, d.ldwu = ptr(w_gate), _ld(w_gate), ptr(w_up), _ld(w_up)
-    d.b_gate, d.b_up = ptr(b_gate), ptr(b_up)
-    d.T, d.D, d.H, d.dtype, d.act = x.shape[0], x.shape[1], w_gate.shape[0], _DTYPES[x.dtype], act
-    return d
+    d.x, d.w_gate, d.w_up = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
+    d.ldx, d.ldwg, d.ldwu = x.stride(0) if T > 1 else D, w_gate.stride(0) if H > 1 else D, w_up.stride(0) if H > 1 else D
+    if b_gate is not None:
+        b_gate = b_gate.contiguous()
+        d.b_gate = b_gate.data_ptr()
+    if b_up is not None:
+        b_up = b_up.contiguous()
+        d.b_up = b_up.data_ptr()
+    d.T, d.D, d.H, d.dtype, d.act = T, D, H, _DTYPES[x.dtype], act
+    if dh is None:
+        d.h, d.ldh = h.data_ptr(), H
+    else:
+        dh = _rows(dh)
+        d.dh, d.lddh = dh.data_ptr(), dh.stride(0) if T > 1 else H
+        d.dx, d.dw_gate, d.dw_up, d.db_gate, d.db_up = (None if t is None else t.data_ptr() for t in out)
+    L, n, what = _lib.lib(), C.c_int64(), "gated_linear" if dh is None else "gated_linear (backward)"
+    if L.hold_gated_workspace(C.byref(d), 0 if dh is None else 1, C.byref(n)) != 0:
+        raise ValueError(f"{what}: a size is out of range (T = {T}, D = {D}, H = {H}, strides {d.ldx}, {d.ldwg}, {d.ldwu})")
+    if n.value:
+        # from the allocator's pool of the current stream (of a capture's while one is recorded): calls share no scratch
+        ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), n.value
+    check((L.hold_gated_fwd if dh is None else L.hold_gated_bwd)(C.byref(d), stream_ptr()), what)
 
 
-def _launch(d, backward, device, what):
-    L = _lib.lib()
-    n = C.c_int64()
-    if L.hold_gated_workspace(C.byref(d), 1 if backward else 0, C.byref(n)) != 0:
-        raise ValueError(f"{what}: a size is out of range (T = {d.T}, D = {d.D}, H = {d.H}, strides {d.ldx}, {d.ldwg}, {d.ldwu})")
-    # of the allocator's own pool for the current stream (and of a capture's pool while one is recorded): calls share no scratch
-    ws = torch.empty(max(n.value, 1), dtype=torch.uint8, device=device)
-    d.workspace, d.workspace_bytes = ptr(ws), n.value
-    fn = L.hold_gated_bwd if backward else L.hold_gated_fwd
-    check(fn(C.byref(d), stream_ptr()), what)
+def _on(device, *args):
+    """_call with the tensors' device as the current one"""
+    if device.index == torch.cuda.current_device():
+        return _call(*args)
+    with torch.cuda.device(device):
+        return _call(*args)
+
+
+def _forward(x, w_gate, w_up, b_gate, b_up, act):
+    h = torch.empty(*x.shape[:-1], w_gate.shape[0], dtype=x.dtype, device=x.device)
+    if h.numel():
+        _on(x.device, act, x, w_gate, w_up, b_gate, b_up, h, None, None)
+    return h
 
 
 class _GatedFn(torch.autograd.Function):
@@ -62,38 +87,22 @@ class _GatedFn(torch.autograd.Function):
     def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
         ctx.save_for_backward(x, w_gate, w_up, b_gate, b_up)
         ctx.act = act
-        H = w_gate.shape[0]
-        h = torch.empty(*x.shape[:-1], H, dtype=x.dtype, device=x.device)
-        if h.numel():
-            x2, wg, wu = _rows(x), _rows(w_gate), _rows(w_up)
-            bg, bu = (None if b is None else b.contiguous() for b in (b_gate, b_up))
-            with torch.cuda.device(x.device):
-                d = _descriptor(x2, wg, wu, bg, bu, act)
-                d.h, d.ldh = ptr(h), H
-                _launch(d, False, x.device, "gated_linear")
-        return h
+        return _forward(x, w_gate, w_up, b_gate, b_up, act)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
-        x, w_gate, w_up, b_gate, b_up = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dw = need[1] or need[2]
-        new = lambda t, wanted: torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and wanted else None  # noqa: E731
-        out = [new(x, need[0]), new(w_gate, dw), new(w_up, dw), new(b_gate, need[3]), new(b_up, need[4])]
+        given = ctx.saved_tensors
+        need = list(ctx.needs_input_grad[:5])
+        need[1] = need[2] = need[1] or need[2]  # the weights' gradients come together
+        out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip(given, need)]
         if dh.numel():
-            x2, wg, wu, dh2 = _rows(x), _rows(w_gate), _rows(w_up), _rows(dh)
-            bg, bu = (None if b is None else b.contiguous() for b in (b_gate, b_up))
-            with torch.cuda.device(x.device):
-                d = _descriptor(x2, wg, wu, bg, bu, ctx.act)
-                d.dh, d.lddh = ptr(dh2), _ld(dh2)
-                d.dx, d.dw_gate, d.dw_up, d.db_gate, d.db_up = (ptr(t) for t in out)
-                _launch(d, True, x.device, "gated_linear (backward)")
+            _on(dh.device, ctx.act, *given, None, dh, out)
         else:
             for t in out:
                 if t is not None:
                     t.zero_()
-        return out[0], out[1] if need[1] else None, out[2] if need[2] else None, out[3], out[4], None
+        return (*(t if n else None for t, n in zip(out, ctx.needs_input_grad)), None)
 
 
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
@@ -101,21 +110,24 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
 
     All tensors on one GPU and of one type, float32 or bfloat16.  Differentiable once in every tensor.  Up to 64 rows go through a
     kernel for few rows that reads the weights as they are, once; more through the matrix cores."""
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"gated_linear: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
-    if x.dim() < 1 or w_gate.dim() != 2 or w_up.shape != w_gate.shape or x.shape[-1] != w_gate.shape[1]:
-        raise ValueError(f"gated_linear: x [..., D] and two weights [H, D] are wanted, got {tuple(x.shape)}, {tuple(w_gate.shape)}, {tuple(w_up.shape)}")
-    if w_gate.shape[1] == 0:
+    shape, dtype, device = w_gate.shape, x.dtype, x.device
+    if x.dim() < 1 or len(shape) != 2 or w_up.shape != shape or x.shape[-1] != shape[1]:
+        raise ValueError(f"gated_linear: x [..., D] and two weights [H, D] are wanted, got {tuple(x.shape)}, {tuple(shape)}, {tuple(w_up.shape)}")
+    if shape[1] == 0:
         raise ValueError("gated_linear: at least one input feature is wanted")
-    given = {"x": x, "w_gate": w_gate, "w_up": w_up, "b_gate": b_gate, "b_up": b_up}
-    for name, t in given.items():
-        if t is None:
-            continue
-        if name.startswith("b_") and tuple(t.shape) != (w_gate.shape[0],):
-            raise ValueError(f"gated_linear: {name} must have shape ({w_gate.shape[0]},), got {tuple(t.shape)}")
-        if t.dtype != x.dtype or t.dtype not in _DTYPES:
-            raise TypeError(f"gated_linear: float32 or bfloat16 throughout is wanted, got {name} of {t.dtype} beside x of {x.dtype}")
-    for name, t in given.items():
-        if t is not None and (t.device != x.device or not t.is_cuda):
-            raise ValueError(f"gated_linear: all tensors have to be on one GPU, got {name} on {t.device}, x on {x.device}")
-    return _GatedFn.apply(x, w_gate, w_up, b_gate, b_up, ACTIVATIONS[activation])
+    tensors = [x, w_gate, w_up]
+    for name, b in (("b_gate", b_gate), ("b_up", b_up)):
+        if b is not None:
+            if b.shape != shape[:1]:
+                raise ValueError(f"gated_linear: {name} must have shape ({shape[0]},), got {tuple(b.shape)}")
+            tensors.append(b)
+    if dtype not in _DTYPES or any(t.dtype is not dtype for t in tensors):
+        raise TypeError(f"gated_linear: float32 or bfloat16 throughout is wanted, got {[str(t.dtype) for t in tensors]}")
+    if device.type != "cuda" or any(t.device != device for t in tensors):
+        raise ValueError(f"gated_linear: all tensors have to be on one GPU, got {[str(t.device) for t in tensors]}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return _GatedFn.apply(x, w_gate, w_up, b_gate, b_up, act)
+    return _forward(x, w_gate, w_up, b_gate, b_up, act)
