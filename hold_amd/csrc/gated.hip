@@ -92,36 +92,65 @@ __device__ __forceinline__ void store1(void* p, int64_t i, float v) {
   if (MODE == MODE_BF16) ((uint16_t*)p)[i] = bf16_bits(v);
   else ((float*)p)[i] = v;
 }
-// four consecutive elements of which the first n exist; VEC: all four do and the address is a multiple of their size
+// four consecutive elements of which the first n exist; rows may start anywhere (the memory takes 16 bytes on any element's boundary)
 template <int MODE>
-__device__ __forceinline__ f32x4 load4(const void* p, int64_t i, int n, bool vec) {
+__device__ __forceinline__ f32x4 load4(const void* p, int64_t i, int n) {
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (vec && n >= 4) {
+  if (n >= 4) {
     if (MODE == MODE_BF16) {
-      const u32x2 w = *(const u32x2*)((const uint16_t*)p + i);
-      v = f32x4{bf16_value((uint16_t)w[0]), bf16_value((uint16_t)(w[0] >> 16)), bf16_value((uint16_t)w[1]), bf16_value((uint16_t)(w[1] >> 16))};
+      u32x2 w;
+      __builtin_memcpy(&w, (const uint16_t*)p + i, 8);
+      const uint32_t w0 = w[0], w1 = w[1];
+      v = f32x4{bf16_value((uint16_t)w0), bf16_value((uint16_t)(w0 >> 16)), bf16_value((uint16_t)w1), bf16_value((uint16_t)(w1 >> 16))};
     } else {
-      v = *(const f32x4*)((const float*)p + i);
+      __builtin_memcpy(&v, (const float*)p + i, 16);
     }
   } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 3; ++r)
       if (r < n) v[r] = load1<MODE>(p, i + r);
   }
   return v;
 }
 template <int MODE>
-__device__ __forceinline__ void store4(void* p, int64_t i, int n, bool vec, f32x4 v) {
-  if (vec && n >= 4) {
-    if (MODE == MODE_BF16)
-      *(u32x2*)((uint16_t*)p + i) = u32x2{(uint32_t)bf16_bits(v[0]) | (uint32_t)bf16_bits(v[1]) << 16, (uint32_t)bf16_bits(v[2]) | (uint32_t)bf16_bits(v[3]) << 16};
-    else
-      *(f32x4*)((float*)p + i) = v;
+__device__ __forceinline__ void store4(void* p, int64_t i, int n, f32x4 v) {
+  if (n >= 4) {
+    if (MODE == MODE_BF16) {
+      const u32x2 w = {(uint32_t)bf16_bits(v[0]) | (uint32_t)bf16_bits(v[1]) << 16, (uint32_t)bf16_bits(v[2]) | (uint32_t)bf16_bits(v[3]) << 16};
+      __builtin_memcpy((uint16_t*)p + i, &w, 8);
+    } else {
+      __builtin_memcpy((float*)p + i, &v, 16);
+    }
   } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 3; ++r)
       if (r < n) store1<MODE>(p, i + r, v[r]);
   }
+}
+
+template <int MODE> constexpr int chunk_k() { return MODE == MODE_BF16 ? 8 : 4; }  // elements in 16 bytes
+
+// 16 bytes of a row from element c on, zeros from element K on
+template <int MODE>
+__device__ __forceinline__ u32x4 chunk16(const void* p, int64_t at, int c, int K) {
+  constexpr int N = chunk_k<MODE>();
+  u32x4 v = {0u, 0u, 0u, 0u};
+  if (c + N <= K) {
+    __builtin_memcpy(&v, (const char*)p + (at + c) * (16 / N), 16);
+    return v;
+  }
+#pragma unroll
+  for (int i = 0; i < N - 1; ++i)
+    if (c + i < K) {
+      if (MODE == MODE_BF16) v[i >> 1] |= (uint32_t)((const uint16_t*)p)[at + c + i] << (16 * (i & 1));
+      else v[i] = ((const uint32_t*)p)[at + c + i];
+    }
+  return v;
+}
+template <int MODE>
+__device__ __forceinline__ float lane_value(u32x4 v, int i) {
+  const uint32_t w = MODE == MODE_BF16 ? v[i >> 1] : v[i];  // a copy: __builtin_bit_cast of a vector's element reads element 0
+  return __builtin_bit_cast(float, MODE == MODE_BF16 ? (i & 1 ? w & 0xffff0000u : w << 16) : w);
 }
 
 template <int K>
@@ -145,14 +174,14 @@ constexpr int NPART = 256;  // blocks that look for the weights' maxima
 constexpr int NONE = -100000;
 __device__ __forceinline__ int exp_or_none(float m) { return m > 0.f ? exp_above(m) : NONE; }
 
-// a wave's rows: 4 consecutive elements a lane, 256 a piece; `vec`: rows on 16-byte boundaries
-__device__ __forceinline__ f32x4 row4(const float* p, int c, int K, bool vec) { return load4<MODE_F16X3>(p, c, K - c, vec); }
+// a wave's rows: 4 consecutive elements a lane, 256 a piece
+__device__ __forceinline__ f32x4 row4(const float* p, int c, int K) { return load4<MODE_F16X3>(p, c, K - c); }
 
-__device__ __forceinline__ float row_max(const float* p, int K, bool vec) {
+__device__ __forceinline__ float row_max(const float* p, int K) {
   const int lane = threadIdx.x & 63;
   float m = 0.f;
   for (int c = 4 * lane; c < K; c += 256) {
-    const f32x4 v = row4(p, c, K, vec);
+    const f32x4 v = row4(p, c, K);
 #pragma unroll
     for (int r = 0; r < 4; ++r) m = fmaxf(m, finite_abs(v[r]));
   }
@@ -161,13 +190,13 @@ __device__ __forceinline__ float row_max(const float* p, int K, bool vec) {
 
 // largest finite magnitude of the weights and biases, per block of the grid: part[which][block]
 __global__ __launch_bounds__(256) void gated_amax_kernel(const float* wg, int64_t ldg, const float* wu, int64_t ldu, const float* bg,
-                                                         const float* bu, int H, int D, int vec, float* part) {
+                                                         const float* bu, int H, int D, float* part) {
   const int which = blockIdx.y;
   float m = 0.f;
   if (which < 2) {
     const float* p = which ? wu : wg;
     const int64_t ld = which ? ldu : ldg;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < H; r += gridDim.x * 4) m = fmaxf(m, row_max(p + r * ld, D, vec));
+    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < H; r += gridDim.x * 4) m = fmaxf(m, row_max(p + r * ld, D));
   } else {
     const float* p = which == 2 ? bg : bu;
     if (p)
@@ -196,16 +225,16 @@ __device__ __forceinline__ void put_limbs(uint16_t* o, int64_t limb, f32x4 v, in
   *(u32x2*)(o + limb) = u32x2{y[0].lo | (uint32_t)y[1].lo << 16, y[2].lo | (uint32_t)y[3].lo << 16};
 }
 // one row to limbs by 2^k
-__device__ __forceinline__ void pack_row(const float* p, int K, int Kp, bool vec, int k, uint16_t* o, int64_t limb) {
+__device__ __forceinline__ void pack_row(const float* p, int K, int Kp, int k, uint16_t* o, int64_t limb) {
   const int lane = threadIdx.x & 63;
-  for (int c = 4 * lane; c < Kp; c += 256) put_limbs(o + c, limb, row4(p, c, K, vec), k);
+  for (int c = 4 * lane; c < Kp; c += 256) put_limbs(o + c, limb, row4(p, c, K), k);
 }
 
 struct PackArgs {
   const float* x; int64_t ldx, T;
   const float* w[2]; int64_t ldw[2];
-  int H, D, Dp, xvec, wvec;
-  uint16_t* ox; int64_t xlimb;
+  int H, D, Dp;
+  uint16_t* ox; int64_t xlimb;  // null: x's rows are only measured
   uint16_t* ow; int64_t wlimb, second;
   int* rowexp;       // [T]
   int* colexp;       // [2][Hp]: the exponent of a weight row's scale
@@ -213,7 +242,7 @@ struct PackArgs {
   // backward
   const float* part; // the weights' maxima: one scale a matrix, and the exponents below
   int* exps;
-  const float* dh; int64_t lddh; int dvec, act;
+  const float* dh; int64_t lddh; int act;
   int* rscale; int* rpart;
 };
 
@@ -243,27 +272,27 @@ __global__ __launch_bounds__(256) void gated_pack_kernel(PackArgs a) {
       const float* p = a.w[w] + j * a.ldw[w];
       int ex = BWD ? ws[w] : 0;
       if (!BWD) {
-        ex = exp_or_none(row_max(p, a.D, a.wvec));
+        ex = exp_or_none(row_max(p, a.D));
         ex = ex == NONE ? 15 : ex;
       }
       if (lane == 0) a.colexp[w * a.Hp + j] = ex;
-      pack_row(p, a.D, a.Dp, a.wvec, 15 - ex, a.ow + w * a.second + (int64_t)j * a.Dp, a.wlimb);
+      pack_row(p, a.D, a.Dp, 15 - ex, a.ow + w * a.second + (int64_t)j * a.Dp, a.wlimb);
       continue;
     }
     const float* p = a.x + r * a.ldx;
     uint16_t* o = a.ox + r * a.Dp;
     int ex;
     if (a.Dp <= 256) {  // the row stays in registers
-      const f32x4 v = row4(p, 4 * lane, a.D, a.xvec);
+      const f32x4 v = row4(p, 4 * lane, a.D);
       ex = exp_or_none(wave_fmax(fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3])))));
-      if (4 * lane < a.Dp) put_limbs(o + 4 * lane, a.xlimb, v, ex == NONE ? 0 : 15 - ex);
+      if (4 * lane < a.Dp && a.ox) put_limbs(o + 4 * lane, a.xlimb, v, ex == NONE ? 0 : 15 - ex);
     } else {
-      ex = exp_or_none(row_max(p, a.D, a.xvec));
-      pack_row(p, a.D, a.Dp, a.xvec, ex == NONE ? 0 : 15 - ex, o, a.xlimb);
+      ex = exp_or_none(row_max(p, a.D));
+      if (a.ox) pack_row(p, a.D, a.Dp, ex == NONE ? 0 : 15 - ex, o, a.xlimb);
     }
     if (lane == 0) a.rowexp[r] = ex;
     if (BWD) {
-      const int ed = exp_or_none(row_max(a.dh + r * a.lddh, a.H, a.dvec));
+      const int ed = exp_or_none(row_max(a.dh + r * a.lddh, a.H));
       auto proj = [&](int w) {  // exponent above a projection's magnitude
         const int m = (ex == NONE || e[w] == NONE) ? NONE : ex + e[w] + ld2, b = e[2 + w];
         return (m > b ? m : b) == NONE ? NONE : (m > b ? m : b) + 1;
@@ -290,7 +319,7 @@ __global__ __launch_bounds__(256) void gated_pack_kernel(PackArgs a) {
 }
 
 // x_t 2^(R - r_t) as limbs for the sum over tokens; rows without a gradient are zeros (where finite).  exps[4] = R
-__global__ __launch_bounds__(256) void gated_pack_tokens_kernel(const float* x, int64_t ld, int64_t T, int D, int Dp, int vec, const int* rscale,
+__global__ __launch_bounds__(256) void gated_pack_tokens_kernel(const float* x, int64_t ld, int64_t T, int D, int Dp, const int* rscale,
                                                                 const int* part, int nparts, uint16_t* out, int64_t limb, int* exps) {
   const int lane = threadIdx.x & 63;
   int top = NONE;
@@ -301,7 +330,7 @@ __global__ __launch_bounds__(256) void gated_pack_tokens_kernel(const float* x, 
   for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < T; r += (int64_t)gridDim.x * 4) {
     const int k = rscale[r];
     for (int c = 4 * lane; c < Dp; c += 256) {
-      f32x4 v = row4(x + r * ld, c, D, vec);
+      f32x4 v = row4(x + r * ld, c, D);
       if (k == NONE) v *= 0.f;
       put_limbs(out + r * Dp + c, limb, v, k == NONE ? 0 : R - k);
     }
@@ -322,10 +351,7 @@ __global__ __launch_bounds__(256) void gated_copy_rows_kernel(CopyArgs a) {
     const int64_t r = q - (w > 0 ? a.rows[0] : 0) - (w > 1 ? a.rows[1] : 0);
     const uint16_t* p = a.x[w] + r * a.ld[w];
     uint16_t* o = a.out[w] + r * a.Kp;
-    for (int c = 2 * lane; c < a.Kp; c += 128) {
-      const uint32_t u = c < a.K ? p[c] : 0, v = c + 1 < a.K ? p[c + 1] : 0;
-      *(uint32_t*)(o + c) = u | v << 16;
-    }
+    for (int c = 8 * lane; c < a.Kp; c += 512) *(u32x4*)(o + c) = chunk16<MODE_BF16>(p, 0, c, a.K);
   }
 }
 
@@ -361,9 +387,6 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const int shift = MODE == MODE_F16X3 && BWD ? a.exps[6] - a.exps[5] : 0;
-  constexpr int ES = MODE == MODE_BF16 ? 2 : 4;
-  const bool hvec = BWD ? (a.lddh % 4 == 0 && (uintptr_t)a.dh % (4 * ES) == 0) : (a.ldh % 4 == 0 && (uintptr_t)a.h % (4 * ES) == 0);
-  const bool bvec = (uintptr_t)a.bg % (4 * ES) == 0 && (uintptr_t)a.bu % (4 * ES) == 0;
   float* sums = (float*)smem;  // [WM][2][BN]
   f32x4 dhs[BWD ? Cr::NI : 1][BWD ? Cr::MI : 1];  // all of them requested before the first store
   if (BWD) {
@@ -373,15 +396,15 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
       for (int mi = 0; mi < Cr::MI; ++mi) {
         const int j = n0 + wn * (BN / WN) + 16 * ni + 4 * (lane >> 4), n = a.H - j;
         const int64_t i = m0 + wm * (BM / WM) + 16 * mi + (lane & 15);
-        dhs[BWD ? ni : 0][BWD ? mi : 0] = i < a.T && n > 0 ? load4<MODE>(a.dh, i * a.lddh + j, n, hvec) : f32x4{0.f, 0.f, 0.f, 0.f};
+        dhs[BWD ? ni : 0][BWD ? mi : 0] = i < a.T && n > 0 ? load4<MODE>(a.dh, i * a.lddh + j, n) : f32x4{0.f, 0.f, 0.f, 0.f};
       }
   }
 #pragma unroll
   for (int ni = 0; ni < Cr::NI; ++ni) {
     const int jt = wn * (BN / WN) + 16 * ni + 4 * (lane >> 4), j = n0 + jt, n = a.H - j;
     f32x4 bg = {0.f, 0.f, 0.f, 0.f}, bu = {0.f, 0.f, 0.f, 0.f};
-    if (a.bg && n > 0) bg = load4<MODE>(a.bg, j, n, bvec);
-    if (a.bu && n > 0) bu = load4<MODE>(a.bu, j, n, bvec);
+    if (a.bg && n > 0) bg = load4<MODE>(a.bg, j, n);
+    if (a.bu && n > 0) bu = load4<MODE>(a.bu, j, n);
     int eg[4] = {0, 0, 0, 0}, eu[4] = {0, 0, 0, 0};
     if (MODE == MODE_F16X3 && n > 0) {
 #pragma unroll
@@ -414,7 +437,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
           activate<false, MODE == MODE_F16X3>(a.act, g[r], s, d);
           h[r] = s * u[r];
         }
-        if (row && n > 0) store4<MODE>(a.h, i * a.ldh + j, n, hvec, h);
+        if (row && n > 0) store4<MODE>(a.h, i * a.ldh + j, n, h);
       } else {
         f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = dg;
         if (row && n > 0) {
@@ -432,8 +455,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
         if (row && j < a.Hp) {  // Hp is a multiple of 8: all four columns are inside, the ones behind H as zeros
           const int64_t o = i * a.Hp + j;
           if (MODE == MODE_BF16) {
-            store4<MODE>(a.dg, o, 4, true, dg);
-            store4<MODE>(a.du, o, 4, true, du);
+            store4<MODE>(a.dg, o, 4, dg);
+            store4<MODE>(a.du, o, 4, du);
           } else {
             const int k = a.rscale[i] == NONE ? 0 : a.rscale[i], ku = a.rscale[i] == NONE ? 0 : k + shift;
             uint16_t hg[4], lg[4], hu[4], lu[4];
@@ -476,6 +499,224 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
         a.dbpart[((int64_t)tm * 2 + w) * a.H + n0 + j] = v;
       }
     }
+  }
+}
+
+// ---- short rows: D <= 256 ------------------------------------------------------------------------------------------------------------------
+// With a sum this short a tile is mostly its start and its end, and the limbs' way through memory costs as much as the layer.  So: a block
+// keeps 64 columns of both weight matrices in LDS for its whole life, as fragments in the order of their reads, and its eight waves run
+// over rows without meeting again: a wave loads 16 MI whole rows as they are (128 bytes of a row at a time), finds their scales and splits
+// them in registers, multiplies, and stores.  One launch, x read once a panel, nothing written but the result.
+// 131072 x 256 -> 256 in fp32: packing and tiles 180 us, this @@ us; bound by @@.
+constexpr int PANEL = 64, SHORT_WAVES = 8;
+
+struct ShortArgs {
+  const void* x; int64_t ldx;
+  const void* w[2]; int64_t ldw[2];
+  const void* b[2];
+  int64_t T, chunk;          // rows of a block: chunk, a multiple of 16 MI waves
+  int D, H, act, panels, parts;
+  void* h; int64_t ldh;      // forward
+  const void* dh; int64_t lddh;  // backward, as MmaArgs
+  uint16_t* dg; uint16_t* du; int64_t Hp, dlimb;
+  const int* rscale; const int* exps;
+  float* dbpart;             // [parts waves][2][H], or null
+};
+
+// 16 rows x 32 KS of k as fragments: a lane holds row lane % 16 (clamped to the last), 8 k's of every 32.  fp32: scaled to [2^14, 2^15), `e` = the
+// row's exponent, limbs; the largest magnitude ignores NaN, and a row with an infinity, scaled by 1, keeps infinities or NaN
+// FULL: D = 32 KS, no chunk ends inside a row
+template <int MODE, int KS, bool FULL>
+__device__ __forceinline__ void short_rows(const void* p, int64_t ld, int64_t row, int64_t rows, int D, s16x8 (&f)[KS][limbs<MODE>()], int& e) {
+  const int lane = threadIdx.x & 63, kl = 8 * (lane >> 4);
+  int64_t r = row + (lane & 15);
+  r = r < rows ? r : rows - 1;
+  if constexpr (MODE == MODE_BF16) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) f[k][0] = __builtin_bit_cast(s16x8, chunk16<MODE_BF16>(p, r * ld, 32 * k + kl, FULL ? 32 * KS + 8 : D));
+    e = 0;
+  } else {
+    u32x4 v[KS][2];
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) v[k][q] = chunk16<MODE_F16X3>(p, r * ld, 32 * k + kl + 4 * q, FULL ? 32 * KS + 8 : D);
+    float m = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(lane_value<MODE_F16X3>(v[k][q], i)));
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    e = m > 0.f && m < __builtin_inff() ? exp_above(m) : 15;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      u32x4 hi, lo;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float a = ldexpf(lane_value<MODE_F16X3>(v[k][q >> 1], 2 * (q & 1)), 15 - e), b = ldexpf(lane_value<MODE_F16X3>(v[k][q >> 1], 2 * (q & 1) + 1), 15 - e);
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        const f16x2 h = __builtin_convertvector(f32x2{a, b}, f16x2);
+        const f16x2 l = __builtin_convertvector(f32x2{a - (float)h[0], b - (float)h[1]}, f16x2);
+        hi[q] = __builtin_bit_cast(uint32_t, h);
+        lo[q] = __builtin_bit_cast(uint32_t, l);
+      }
+      f[k][0] = __builtin_bit_cast(s16x8, hi);
+      f[k][1] = __builtin_bit_cast(s16x8, lo);
+    }
+  }
+}
+
+template <int MODE, bool BWD, int KS, int MI, bool FULL>
+__global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs a) {
+  constexpr int NL = limbs<MODE>(), NF = PANEL / 16;
+  __shared__ __align__(16) s16x8 panel[KS][2 * NF][NL][64];
+  __shared__ __align__(16) int colexp[2][PANEL];
+  __shared__ __align__(16) float bias[2][PANEL];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  // all panels of a part's rows on one XCD (blocks go to the XCDs in turn): its L2 serves the rows after the first
+  const int x8 = blockIdx.x % 8, i8 = blockIdx.x / 8;
+  const bool even = a.parts % 8 == 0;
+  const int part = even ? x8 + 8 * (i8 / a.panels) : (int)blockIdx.x / a.panels, pan = even ? i8 % a.panels : (int)blockIdx.x % a.panels;
+  const int n0 = pan * PANEL;
+  {  // a wave: 16 columns of one of the matrices
+    const int w = wave / NF, q = wave % NF;
+    s16x8 f[KS][NL];
+    int e;
+    short_rows<MODE, KS, FULL>(a.w[w], a.ldw[w], n0 + 16 * q, a.H, a.D, f, e);
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int l = 0; l < NL; ++l) panel[k][wave][l][lane] = f[k][l];
+    if (lane < 16) {
+      const int j = n0 + 16 * q + lane;
+      colexp[w][16 * q + lane] = e - 15;
+      bias[w][16 * q + lane] = a.b[w] && j < a.H ? load1<MODE>(a.b[w], j) : 0.f;
+    }
+  }
+  static_assert(SHORT_WAVES == 2 * NF, "a wave for each 16 columns of the panel");
+  __syncthreads();
+  const int jl = 4 * (lane >> 4);  // of 16 columns the lane's four
+  f32x4 sum[2][BWD ? NF : 1];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int f = 0; f < (BWD ? NF : 1); ++f) sum[w][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int shift = MODE == MODE_F16X3 && BWD ? a.exps[6] - a.exps[5] : 0;
+  const int64_t begin = part * a.chunk, end = begin + a.chunk < a.T ? begin + a.chunk : a.T;
+  for (int64_t row = begin + wave * 16 * MI; row < end; row += SHORT_WAVES * 16 * MI) {
+    s16x8 x[MI][KS][NL];
+    int ex[MI];
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+      short_rows<MODE, KS, FULL>(a.x, a.ldx, row + 16 * m, a.T, a.D, x[m], ex[m]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    f32x4 acc[2][MI][NF];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) acc[w][m][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    asm volatile("" ::: "memory");  // the panel is the same for every round: it would be hoisted out of the loop, into scratch
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        __builtin_amdgcn_sched_barrier(0);  // and read a matrix at a time
+        s16x8 b[NF][NL];
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+          for (int l = 0; l < NL; ++l) b[f][l] = panel[k][w * NF + f][l][lane];
+#pragma unroll
+        for (int p = NL == 2 ? 0 : 2; p < 3; ++p)
+#pragma unroll
+          for (int m = 0; m < MI; ++m)
+#pragma unroll
+            for (int f = 0; f < NF; ++f) acc[w][m][f] = mfma<MODE>(b[f][p == 0 ? NL - 1 : 0], x[m][k][p == 1 ? NL - 1 : 0], acc[w][m][f]);
+      }
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+      const int64_t i = row + 16 * m + (lane & 15);
+      const bool live = i < a.T;
+      f32x4 dhs[BWD ? NF : 1];
+      int rs = 0;
+      if (BWD) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          const int j = n0 + 16 * f + jl;
+          dhs[BWD ? f : 0] = live && j < a.H ? load4<MODE>(a.dh, i * a.lddh + j, a.H - j) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        if (MODE == MODE_F16X3) rs = live ? a.rscale[i] : NONE;
+      }
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const int j = n0 + 16 * f + jl, n = a.H - j;
+        f32x4 g = acc[0][m][f], u = acc[1][m][f];
+        if (MODE == MODE_F16X3) {
+          const int4 cg = *(const int4*)&colexp[0][16 * f + jl], cu = *(const int4*)&colexp[1][16 * f + jl];
+          const int e0 = ex[m] - 15;
+          g = f32x4{ldexpf(g[0], e0 + cg.x), ldexpf(g[1], e0 + cg.y), ldexpf(g[2], e0 + cg.z), ldexpf(g[3], e0 + cg.w)};
+          u = f32x4{ldexpf(u[0], e0 + cu.x), ldexpf(u[1], e0 + cu.y), ldexpf(u[2], e0 + cu.z), ldexpf(u[3], e0 + cu.w)};
+        }
+        g += *(const f32x4*)&bias[0][16 * f + jl];
+        u += *(const f32x4*)&bias[1][16 * f + jl];
+        if (!BWD) {
+          f32x4 h;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float s, d;
+            activate<false, MODE == MODE_F16X3>(a.act, g[r], s, d);
+            h[r] = s * u[r];
+          }
+          if (live && n > 0) store4<MODE>(a.h, i * a.ldh + j, n, h);
+        } else {
+          f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = dg;
+          if (live) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float s, d;
+              activate<true, MODE == MODE_F16X3>(a.act, g[r], s, d);
+              if (r < n) {
+                dg[r] = dhs[BWD ? f : 0][r] * u[r] * d;
+                du[r] = dhs[BWD ? f : 0][r] * s;
+              }
+            }
+          }
+          sum[0][BWD ? f : 0] += dg;
+          sum[1][BWD ? f : 0] += du;
+          if (live && j < a.Hp) {  // as the tiles' epilogue
+            const int64_t o = i * a.Hp + j;
+            if (MODE == MODE_BF16) {
+              store4<MODE>(a.dg, o, 4, dg);
+              store4<MODE>(a.du, o, 4, du);
+            } else {
+              put_limbs(a.dg + o, a.dlimb, dg, rs == NONE ? 0 : rs);
+              put_limbs(a.du + o, a.dlimb, du, rs == NONE ? 0 : rs + shift);
+            }
+          }
+        }
+      }
+    }
+  }
+  if (BWD && a.dbpart) {  // a wave's own column sums, over the 16 lanes of equal columns
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        f32x4 v = sum[w][BWD ? f : 0];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) v[r] += __shfl_xor(v[r], o, 64);
+        const int j = n0 + 16 * f + jl;
+        if ((lane & 15) == 0 && j < a.H) store4<MODE_F16X3>(a.dbpart, (((int64_t)part * SHORT_WAVES + wave) * 2 + w) * a.H + j, a.H - j, v);
+      }
   }
 }
 
@@ -533,7 +774,6 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dx_kernel(DxArgs a) {
   }
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const int ew = MODE == MODE_F16X3 ? a.exps[5] - 15 : 0;
-  const bool vec = a.D % 4 == 0;
 #pragma unroll
   for (int mi = 0; mi < Cr::MI; ++mi) {
     const int64_t i = m0 + wm * (BM / WM) + 16 * mi + (lane & 15);
@@ -547,8 +787,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dx_kernel(DxArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], k);
       if (j >= a.D) continue;
-      if (a.splits == 1) store4<MODE>(a.dx, i * a.D + j, a.D - j, vec, v);
-      else store4<MODE_F16X3>(a.part, (sp * a.T + i) * a.D + j, a.D - j, vec, v);
+      if (a.splits == 1) store4<MODE>(a.dx, i * a.D + j, a.D - j, v);
+      else store4<MODE_F16X3>(a.part, (sp * a.T + i) * a.D + j, a.D - j, v);
     }
   }
 }
@@ -582,7 +822,6 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dw_kernel(DwArgs a) {
   else Cr::run(smem, A, B, acc);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   const int e = MODE == MODE_F16X3 ? -a.exps[4] - (w ? a.exps[6] - a.exps[5] : 0) : 0;
-  const bool vec = a.D % 4 == 0;
 #pragma unroll
   for (int mi = 0; mi < Cr::MI; ++mi) {
     const int i = m0 + wm * (BM / WM) + 16 * mi + (lane & 15);
@@ -595,8 +834,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dw_kernel(DwArgs a) {
       if (MODE == MODE_F16X3)
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], e);
-      if (a.splits == 1) store4<MODE>(a.out[w], (int64_t)i * a.D + j, a.D - j, vec, v);
-      else store4<MODE_F16X3>(a.part, (((int64_t)sp * 2 + w) * a.H + i) * a.D + j, a.D - j, vec, v);
+      if (a.splits == 1) store4<MODE>(a.out[w], (int64_t)i * a.D + j, a.D - j, v);
+      else store4<MODE_F16X3>(a.part, (((int64_t)sp * 2 + w) * a.H + i) * a.D + j, a.D - j, v);
     }
   }
 }
@@ -608,44 +847,21 @@ __global__ __launch_bounds__(256) void gated_reduce_kernel(const float* part, in
   const int w = blockIdx.y;
   if (i >= n) return;
   const int m = n - i < 4 ? (int)(n - i) : 4;
-  const bool vec = n % 4 == 0;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < splits; ++s) v += load4<MODE_F16X3>(part, ((int64_t)s * sets + w) * n + i, m, vec);
-  store4<MODE>(w ? out1 : out0, i, m, true, v);
+  for (int s = 0; s < splits; ++s) v += load4<MODE_F16X3>(part, ((int64_t)s * sets + w) * n + i, m);
+  store4<MODE>(w ? out1 : out0, i, m, v);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------
 // T <= 64: bound by the weights' bytes, which are read once, 16 a lane, as they are; no product of limbs, fp32 keeps fp32 arithmetic.
 constexpr int ROWS_MAX = 64;
-template <int MODE> constexpr int chunk_k() { return MODE == MODE_BF16 ? 8 : 4; }  // elements in 16 bytes
-
-// 16 bytes of a row from element c on, zeros from element K on; `vec`: rows start on 16-byte boundaries
-template <int MODE>
-__device__ __forceinline__ u32x4 chunk16(const void* p, int64_t at, int c, int K, bool vec) {
-  constexpr int N = chunk_k<MODE>();
-  u32x4 v = {0u, 0u, 0u, 0u};
-  if (vec && c + N <= K) return MODE == MODE_BF16 ? *(const u32x4*)((const uint16_t*)p + at + c) : *(const u32x4*)((const float*)p + at + c);
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (c + i < K) {
-      if (MODE == MODE_BF16) v[i >> 1] |= (uint32_t)((const uint16_t*)p)[at + c + i] << (16 * (i & 1));
-      else v[i] = ((const uint32_t*)p)[at + c + i];
-    }
-  return v;
-}
-template <int MODE>
-__device__ __forceinline__ float lane_value(u32x4 v, int i) {
-  const uint32_t w = MODE == MODE_BF16 ? v[i >> 1] : v[i];  // a copy: __builtin_bit_cast of a vector's element reads element 0
-  return __builtin_bit_cast(float, MODE == MODE_BF16 ? (i & 1 ? w & 0xffff0000u : w << 16) : w);
-}
-
 struct RowsArgs {
   const void* x; int64_t ldx;
   const void* w[2]; int64_t ldw[2];
   const void* b[2];
   void* h; int64_t ldh;
-  int T, D, H, act, xvec, wvec;
+  int T, D, H, act;
 };
 
 // T <= 4: dot products, a wave computes NC columns of both projections for all rows, its lanes along k (4 x 4096 -> 8192 in bf16, 134 MB of
@@ -667,9 +883,9 @@ __global__ __launch_bounds__(256) void gated_rows_kernel(RowsArgs a) {
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
-      for (int w = 0; w < 2; ++w) v[w][n] = chunk16<MODE>(a.w[w], (j0 + n < a.H ? j0 + n : a.H - 1) * a.ldw[w], c, a.D, a.wvec);
+      for (int w = 0; w < 2; ++w) v[w][n] = chunk16<MODE>(a.w[w], (j0 + n < a.H ? j0 + n : a.H - 1) * a.ldw[w], c, a.D);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) x[t] = chunk16<MODE>(a.x, (t < a.T ? t : a.T - 1) * a.ldx, c, a.D, a.xvec);
+    for (int t = 0; t < NT; ++t) x[t] = chunk16<MODE>(a.x, (t < a.T ? t : a.T - 1) * a.ldx, c, a.D);
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -723,9 +939,9 @@ __global__ __launch_bounds__(256) void gated_few_kernel(RowsArgs a) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
 #pragma unroll
-      for (int w = 0; w < 2; ++w) v[i][w] = chunk16<MODE>(a.w[w], jr * a.ldw[w], k0 + i * STEP + kl, a.D, a.wvec);
+      for (int w = 0; w < 2; ++w) v[i][w] = chunk16<MODE>(a.w[w], jr * a.ldw[w], k0 + i * STEP + kl, a.D);
 #pragma unroll
-      for (int n = 0; n < NB; ++n) x[i][n] = chunk16<MODE>(a.x, (16 * n + r < a.T ? 16 * n + r : a.T - 1) * a.ldx, k0 + i * STEP + kl, a.D, a.xvec);
+      for (int n = 0; n < NB; ++n) x[i][n] = chunk16<MODE>(a.x, (16 * n + r < a.T ? 16 * n + r : a.T - 1) * a.ldx, k0 + i * STEP + kl, a.D);
     }
 #pragma unroll
     for (int i = 0; i < U; ++i)
@@ -753,11 +969,9 @@ __global__ __launch_bounds__(256) void gated_few_kernel(RowsArgs a) {
   if (wave) return;
   const int j = j0 + 4 * (lane >> 4), n4 = a.H - j;  // a lane: four columns of row 16 n + r
   if (n4 <= 0) return;
-  constexpr int ES = MODE == MODE_BF16 ? 2 : 4;
-  const bool bvec = (uintptr_t)a.b[0] % (4 * ES) == 0 && (uintptr_t)a.b[1] % (4 * ES) == 0, hvec = a.ldh % 4 == 0 && (uintptr_t)a.h % (4 * ES) == 0;
   f32x4 bias[2];
 #pragma unroll
-  for (int w = 0; w < 2; ++w) bias[w] = a.b[w] ? load4<MODE>(a.b[w], j, n4, bvec) : f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int w = 0; w < 2; ++w) bias[w] = a.b[w] ? load4<MODE>(a.b[w], j, n4) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     const int t = 16 * n + r;
@@ -770,7 +984,7 @@ __global__ __launch_bounds__(256) void gated_few_kernel(RowsArgs a) {
       activate<false, MODE == MODE_F16X3>(a.act, acc[0][n][q], f, d);
       h[q] = f * acc[1][n][q];
     }
-    if (t < a.T) store4<MODE>(a.h, t * a.ldh + j, n4, hvec, h);
+    if (t < a.T) store4<MODE>(a.h, t * a.ldh + j, n4, h);
   }
 }
 
@@ -797,7 +1011,8 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // where everything of one call lies in its workspace (bytes; every part starts on a multiple of 256)
 struct Plan {
   bool copy_x, copy_w[2];
-  bool big, dx_big, dw_big;
+  bool brief, big, dx_big, dw_big;  // brief: the kernel for short rows
+  int64_t parts, part_rows;
   int64_t Dp, Hp, row_tiles, pack_blocks;
   int64_t dx_splits, dx_chunk, dw_splits, dw_chunk;
   int64_t x, w, dg, xt, part, exps, rowexp, colexp, rscale, dbpart, sums, spart, bytes;
@@ -825,10 +1040,18 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
   p.copy_w[1] = f32 || d.D % 8 || !aligned16(d.w_up, d.ldwu, 2);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o += up(bytes, 256); return at; };
+  p.brief = d.D <= 256;
+  // some 256 blocks; a part's rows are whole rounds of its waves, and all panels of a part go to one XCD where the parts divide
+  const int64_t panels = cdiv(d.H, PANEL), round = SHORT_WAVES * 16 * (bwd ? 1 : 2), rounds = cdiv(d.T, round);
+  int64_t parts = cdiv(256, panels);
+  parts = parts > rounds ? rounds : parts >= 8 ? (parts + 7) / 8 * 8 : parts;
+  p.part_rows = cdiv(rounds, parts) * round;
+  p.parts = cdiv(d.T, p.part_rows);
   p.big = large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64), cdiv(p.Dp, step));
-  p.row_tiles = cdiv(d.T, p.big ? 256 : 128);
+  p.row_tiles = p.brief ? p.parts * SHORT_WAVES : cdiv(d.T, p.big ? 256 : 128);
   p.pack_blocks = rows_grid(d.T + 2 * (int64_t)d.H);
-  p.x = p.copy_x ? take(d.T * p.Dp * 2 * nl) : 0;
+  if (p.brief && !bwd) return p;  // takes everything as it is
+  p.x = p.copy_x && !(p.brief && f32) ? take(d.T * p.Dp * 2 * nl) : 0;
   p.w = p.copy_w[0] || p.copy_w[1] ? take(2 * (int64_t)d.H * p.Dp * 2 * nl) : 0;
   if (f32) {
     p.rowexp = take(d.T * 4);
@@ -881,17 +1104,16 @@ void operands(const hold_gated_desc& d, const Plan& p, char* ws, hipStream_t st,
     k.x = (const float*)d.x; k.ldx = d.ldx; k.T = d.T;
     k.w[0] = (const float*)d.w_gate; k.w[1] = (const float*)d.w_up; k.ldw[0] = d.ldwg; k.ldw[1] = d.ldwu;
     k.H = d.H; k.D = d.D; k.Dp = (int)p.Dp;
-    k.xvec = aligned16(d.x, d.ldx, 4); k.wvec = aligned16(d.w_gate, d.ldwg, 4) && aligned16(d.w_up, d.ldwu, 4);
-    k.ox = (uint16_t*)(ws + p.x); k.xlimb = WX;
+    k.ox = p.brief ? nullptr : (uint16_t*)(ws + p.x); k.xlimb = WX;
     k.ow = (uint16_t*)(ws + p.w); k.wlimb = 2 * WW; k.second = WW;
     k.rowexp = (int*)(ws + p.rowexp); k.colexp = (int*)(ws + p.colexp); k.Hp = p.Hp;
     if (BWD) {
       float* part = (float*)(ws + p.part);
       k.part = part; k.exps = (int*)(ws + p.exps);
-      k.dh = (const float*)d.dh; k.lddh = d.lddh; k.dvec = aligned16(d.dh, d.lddh, 4); k.act = d.act;
+      k.dh = (const float*)d.dh; k.lddh = d.lddh; k.act = d.act;
       k.rscale = (int*)(ws + p.rscale); k.rpart = (int*)(ws + p.spart);
       hipLaunchKernelGGL(gated_amax_kernel, dim3(NPART, 4), dim3(256), 0, st, k.w[0], d.ldwg, k.w[1], d.ldwu, (const float*)d.b_gate,
-                         (const float*)d.b_up, d.H, d.D, k.wvec, part);
+                         (const float*)d.b_up, d.H, d.D, part);
       a.exps = k.exps;
       a.rscale = k.rscale;
     }
@@ -918,8 +1140,36 @@ void operands(const hold_gated_desc& d, const Plan& p, char* ws, hipStream_t st,
 }
 
 template <int MODE, bool BWD>
-void launch_mma(MmaArgs a, bool big, hipStream_t st) {
-  if (big) {
+void launch_short(const hold_gated_desc& d, const MmaArgs& m, const Plan& p, hipStream_t st) {
+  ShortArgs a = {};
+  a.x = d.x; a.ldx = d.ldx;
+  a.w[0] = d.w_gate; a.w[1] = d.w_up; a.ldw[0] = d.ldwg; a.ldw[1] = d.ldwu;
+  a.b[0] = d.b_gate; a.b[1] = d.b_up;
+  a.T = d.T; a.chunk = p.part_rows; a.D = d.D; a.H = d.H; a.act = d.act;
+  a.panels = (int)cdiv(d.H, PANEL); a.parts = (int)p.parts;
+  a.h = m.h; a.ldh = m.ldh;
+  a.dh = m.dh; a.lddh = m.lddh;
+  a.dg = m.dg; a.du = m.du; a.Hp = p.Hp; a.dlimb = m.dlimb;
+  a.rscale = m.rscale; a.exps = m.exps; a.dbpart = m.dbpart;
+  const dim3 grid((unsigned)(a.panels * p.parts)), block(64 * SHORT_WAVES);
+  constexpr int MI = BWD ? 1 : 2;
+  const int ks = (d.D + 31) / 32;
+  const bool full = d.D % 64 == 0;
+#define HOLD_SHORT(KS)                                                                                             \
+  if (full) hipLaunchKernelGGL((gated_short_kernel<MODE, BWD, KS, MI, true>), grid, block, 0, st, a);               \
+  else hipLaunchKernelGGL((gated_short_kernel<MODE, BWD, KS, MI, false>), grid, block, 0, st, a)
+  if (ks <= 2) { HOLD_SHORT(2); }
+  else if (ks <= 4) { HOLD_SHORT(4); }
+  else if (ks <= 6) { HOLD_SHORT(6); }
+  else { HOLD_SHORT(8); }
+#undef HOLD_SHORT
+}
+
+template <int MODE, bool BWD>
+void launch_mma(const hold_gated_desc& d, MmaArgs a, const Plan& p, hipStream_t st) {
+  if (p.brief) {
+    launch_short<MODE, BWD>(d, a, p, st);
+  } else if (p.big) {
     a.tm = (int)cdiv(a.T, 256); a.tn = (int)cdiv(a.H, 128);
     hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 256, 128, 4, 4, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
   } else {
@@ -930,15 +1180,12 @@ void launch_mma(MmaArgs a, bool big, hipStream_t st) {
 
 template <int MODE>
 void rows(const hold_gated_desc& d, hipStream_t st) {
-  constexpr int ES = MODE == MODE_BF16 ? 2 : 4;
   RowsArgs a = {};
   a.x = d.x; a.ldx = d.ldx;
   a.w[0] = d.w_gate; a.w[1] = d.w_up; a.ldw[0] = d.ldwg; a.ldw[1] = d.ldwu;
   a.b[0] = d.b_gate; a.b[1] = d.b_up;
   a.h = d.h; a.ldh = d.ldh;
   a.T = (int)d.T; a.D = d.D; a.H = d.H; a.act = d.act;
-  a.xvec = aligned16(d.x, d.ldx, ES);
-  a.wvec = aligned16(d.w_gate, d.ldwg, ES) && aligned16(d.w_up, d.ldwu, ES);
   // four columns a wave where that still leaves two waves a SIMD, one elsewhere
 #define HOLD_ROWS(NT, NC) hipLaunchKernelGGL((gated_rows_kernel<MODE, NT, NC>), dim3((unsigned)cdiv(d.H, 4 * NC)), dim3(256), 0, st, a)
 #define HOLD_FEW(NB) hipLaunchKernelGGL((gated_few_kernel<MODE, NB>), dim3((unsigned)cdiv(d.H, 16)), dim3(256), 0, st, a)
@@ -962,9 +1209,9 @@ int fwd(const hold_gated_desc& d, hipStream_t st) {
   const Plan p = plan(d, false);
   if (p.bytes > d.workspace_bytes || (p.bytes && !d.workspace)) return HOLD_E_ARG;
   MmaArgs a = {};
-  operands<MODE, false>(d, p, (char*)d.workspace, st, a);
+  if (!p.brief) operands<MODE, false>(d, p, (char*)d.workspace, st, a);
   a.h = d.h; a.ldh = d.ldh;
-  launch_mma<MODE, false>(a, p.big, st);
+  launch_mma<MODE, false>(d, a, p, st);
   return ok();
 }
 
@@ -980,12 +1227,12 @@ int bwd(const hold_gated_desc& d, hipStream_t st) {
   const int64_t XN = d.T * p.Dp, DN = d.T * p.Hp;
   if (F32)
     hipLaunchKernelGGL(gated_pack_tokens_kernel, dim3((unsigned)rows_grid(d.T)), dim3(256), 0, st, (const float*)d.x, d.ldx, d.T, d.D, (int)p.Dp,
-                       (int)aligned16(d.x, d.ldx, 4), a.rscale, (const int*)(ws + p.spart), (int)p.pack_blocks, (uint16_t*)(ws + p.xt), XN,
+                       a.rscale, (const int*)(ws + p.spart), (int)p.pack_blocks, (uint16_t*)(ws + p.xt), XN,
                        (int*)(ws + p.exps));
   a.dh = d.dh; a.lddh = d.lddh;
   a.dg = (uint16_t*)(ws + p.dg); a.du = a.dg + NL * DN; a.dlimb = DN;
   a.dbpart = d.db_gate || d.db_up ? (float*)(ws + p.dbpart) : nullptr;
-  launch_mma<MODE, true>(a, p.big, st);
+  launch_mma<MODE, true>(d, a, p, st);
   if (a.dbpart)
     hipLaunchKernelGGL(gated_db_kernel<MODE>, dim3((unsigned)((d.H + 63) / 64), 2), dim3(1024), 0, st, a.dbpart, (int)p.row_tiles, d.H, d.db_gate, d.db_up);
   float* sums = (float*)(ws + p.sums);

@@ -203,9 +203,31 @@ __global__ __launch_bounds__(256) void ns_load_kernel(Items a, Firsts t, Step s,
   const int64_t b = mat * it.stride;
   const float f = it.m ? grad_scale(s) : 1.f;
   const int r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;  // the tile's place in the source
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int r = e >> 6, c = e & 63;
-    s_tile[r][c] = r0 + r < it.rows && c0 + c < it.cols ? update_of(it, s, f, b, r0 + r, c0 + c) : 0.f;
+  const bool whole = r0 + 64 <= it.rows && c0 + 64 <= it.cols && s.dtype == HOLD_MUON_F32 &&
+                     (((uintptr_t)it.g | (uintptr_t)it.m | (uint64_t)(4 * b)) % 16 | (uint32_t)(it.ldg | (it.m ? it.ldm : 0)) % 4) == 0;
+  if (whole) {  // 16 bytes a lane, all of a thread's loads requested together
+    const float* gp = (const float*)it.g + b + c0;
+    const float* mp = (const float*)it.m + b + c0;
+    f32x4 g[4], m[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int r = r0 + q * 16 + (threadIdx.x >> 4), c = 4 * (threadIdx.x & 15);
+      g[q] = *(const f32x4*)(gp + (int64_t)r * it.ldg + c);
+      if (it.m) m[q] = *(const f32x4*)(mp + (int64_t)r * it.ldm + c);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float u = !it.m ? g[q][i] : s.nesterov ? s.rest * (g[q][i] * f) + s.mu * m[q][i] : m[q][i];
+        s_tile[q * 16 + (threadIdx.x >> 4)][4 * (threadIdx.x & 15) + i] = u;
+      }
+  } else {
+#pragma unroll 4
+    for (int e = threadIdx.x; e < 4096; e += 256) {
+      const int r = e >> 6, c = e & 63;
+      s_tile[r][c] = r0 + r < it.rows && c0 + c < it.cols ? update_of(it, s, f, b, r0 + r, c0 + c) : 0.f;
+    }
   }
   __syncthreads();
   const double inv = ldexp(1. / (sqrt((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])) + (double)s.eps), xs);
@@ -300,9 +322,21 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
     A = Operand{s.l + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
     B[0] = Operand{s.x + xo + j0, s.xlimb, np, np - j0, mp};
   }
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+  // the small tiles' launches are latencies: POLY's own tile of A is requested before the products, not behind them
+  constexpr bool EARLY = KIND == POLY && T <= 64;
+  f32x4 early[EARLY ? Cr::MI : 1][EARLY ? Cr::NI : 1];
+  if (EARLY) {
+#pragma unroll
+    for (int mi = 0; mi < Cr::MI; ++mi)
+#pragma unroll
+      for (int ni = 0; ni < Cr::NI; ++ni) {
+        const int i = i0 + wm * (T / WM) + 16 * mi + (lane & 15), j = j0 + wn * (T / WN) + 16 * ni + 4 * (lane >> 4);
+        early[EARLY ? mi : 0][EARLY ? ni : 0] = i < mp && j < mp ? load_limbs(s.l + co + (int64_t)i * mp + j, s.climb) : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+  }
   if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
   else Cr::run(smem, A, B, acc);
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   uint16_t* sym = s.o + co;
   uint16_t* turn = (uint16_t*)smem;
 #pragma unroll
@@ -319,7 +353,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
         if (in) store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
       } else if (KIND == POLY) {
         if (in) {
-          const f32x4 u = load_limbs(s.l + co + (int64_t)i * mp + j, s.climb);
+          const f32x4 u = EARLY ? early[EARLY ? mi : 0][EARLY ? ni : 0] : load_limbs(s.l + co + (int64_t)i * mp + j, s.climb);
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = fmaf(s.c, v[r], s.b * u[r]) + (i == j + r ? s.a : 0.f);
           store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
@@ -515,6 +549,8 @@ int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStre
   if (best == 0) launch_tiles<KIND, 256, 4, 4, 2, true, LAST>(cl, s, st, a, n, stream);
   else if (best == 1) launch_tiles<KIND, 192, 3, 4, 2, false, LAST>(cl, s, st, a, n, stream);
   else if (best == 2) launch_tiles<KIND, 128, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
+  // with a block to itself a unit has the whole LDS: all of 256 k's in flight at once (one 256 x 256: 7.1 -> @@ us a launch)
+  else if (n <= 256) launch_tiles<KIND, 64, 2, 2, 8, false, LAST>(cl, s, st, a, n, stream);
   else launch_tiles<KIND, 64, 2, 2, 4, false, LAST>(cl, s, st, a, n, stream);
   return HOLD_OK;
 }

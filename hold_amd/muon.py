@@ -11,6 +11,7 @@ with them.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -96,10 +97,23 @@ def update_scale(rows, cols, scale):
     raise ValueError(f'muon_step: scale must be "spectral", "rms" or a number, got {scale!r}')
 
 
+def _row_stride(t, rows, cols):
+    if t.is_contiguous():
+        return cols
+    step, inner = t.stride()
+    if rows == 1:
+        step = cols
+    if cols > 1 and inner != 1 or not cols <= step < 1 << 31:
+        raise ValueError(f"muon_step: contiguous rows are wanted, got strides {t.stride()} of shape {tuple(t.shape)}")
+    return step
+
+
 def _spans_overlap(spans):
     """spans: (first byte, end, only read, rows, columns, row stride) of float32 matrices.  Column slices of one wider matrix interleave
     without sharing memory: they are told apart where their row strides agree."""
     spans.sort()
+    if all(a[1] <= b[0] for a, b in zip(spans, spans[1:])):
+        return False
     for i, (lo, hi, read, rows, cols, ld) in enumerate(spans):
         for j in range(i + 1, len(spans)):
             lo2, _, read2, rows2, cols2, ld2 = spans[j]
@@ -148,40 +162,37 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
     device, every = params[0].device, params + grads + momenta
     if {t.dtype for t in every} != {torch.float32}:
         raise TypeError(f"{what}: float32 matrices are wanted, got {sorted({str(t.dtype) for t in every})}")
-    items, spans = [], []
-    for three in zip(params, grads, momenta):
-        shape = three[0].shape
-        if len(shape) != 2 or three[1].shape != shape or three[2].shape != shape:
-            raise ValueError(f"{what}: a parameter, its gradient and its momentum are 2-D and of one shape, got {[tuple(t.shape) for t in three]}")
+    flat, spans, gains = [], [], {}
+    for p, g, m in zip(params, grads, momenta):
+        shape = p.shape
+        if len(shape) != 2 or g.shape != shape or m.shape != shape:
+            raise ValueError(f"{what}: a parameter, its gradient and its momentum are 2-D and of one shape, got {[tuple(t.shape) for t in (p, g, m)]}")
         rows, cols = shape
-        gain = update_scale(rows, cols, scale) if rows and cols else 0.0
         if not (rows and cols):
             continue
-        if rows > MAX_DIM or cols > MAX_DIM:
-            raise ValueError(f"{what}: a matrix of {tuple(shape)} is larger than {MAX_DIM} on a side")
-        at, ld = [], []
-        for k, t in enumerate(three):
-            step, inner = t.stride()
-            if rows == 1:
-                step = cols
-            if cols > 1 and inner != 1 or not cols <= step < 1 << 31:
-                raise ValueError(f"{what}: contiguous rows are wanted, got strides {t.stride()} of shape {tuple(shape)}")
-            lo = t.data_ptr()
-            at.append(lo)
-            ld.append(step)
-            spans.append((lo, lo + 4 * ((rows - 1) * step + cols), k == 1, rows, cols, step))
-        items.append((at[0], at[1], at[2], rows, cols, ld[0], ld[1], ld[2], gain))
-    if len({t.device for t in every}) > 1 or not params[0].is_cuda:
+        gain = gains.get(shape)
+        if gain is None:
+            if rows > MAX_DIM or cols > MAX_DIM:
+                raise ValueError(f"{what}: a matrix of {tuple(shape)} is larger than {MAX_DIM} on a side")
+            gain = gains[shape] = update_scale(rows, cols, scale)
+        ldp, ldg, ldm = _row_stride(p, rows, cols), _row_stride(g, rows, cols), _row_stride(m, rows, cols)
+        ap, ag, am = p.data_ptr(), g.data_ptr(), m.data_ptr()
+        flat += (ap, ag, am, rows, cols, ldp, ldg, ldm, gain)
+        rows -= 1
+        spans += ((ap, ap + 4 * (rows * ldp + cols), False, rows + 1, cols, ldp), (ag, ag + 4 * (rows * ldg + cols), True, rows + 1, cols, ldg),
+                  (am, am + 4 * (rows * ldm + cols), False, rows + 1, cols, ldm))
+    if not params[0].is_cuda or len({t.get_device() for t in every}) > 1:
         raise ValueError(f"{what}: all tensors have to be on one GPU, got {sorted({str(t.device) for t in every})}")
     if _spans_overlap(spans):
         raise ValueError(f"{what}: a parameter or momentum shares memory with another tensor of the call")
     if sumsq is not None and (sumsq.numel() != 1 or sumsq.dtype != torch.float32 or sumsq.device != device):
         raise ValueError(f"{what}: sumsq is one float32 value on {device}")
-    if not items:
+    if not flat:
         return
     d = MuonDesc()
-    array = (MuonItem * len(items))(*items)  # a tuple an item, in the structure's order
-    d.items, d.n_items = C.cast(array, C.POINTER(MuonItem)), len(items)
+    d.n_items = len(flat) // 9
+    array = bytearray(struct.pack("<" + "QQQiiiiif" * d.n_items, *flat))  # MuonItem, laid out in one call
+    d.items = C.cast((C.c_char * len(array)).from_buffer(array), C.POINTER(MuonItem))
     d.coef, d.steps, d.nesterov = C.cast(coef, C.POINTER(C.c_float)), steps, 1 if nesterov else 0
     d.lr, d.momentum, d.weight_decay, d.grad_mul, d.clip_norm, d.eps = float(lr), float(momentum), float(weight_decay), float(grad_mul), float(clip_norm), eps
     d.sumsq = ptr(sumsq)
@@ -190,7 +201,7 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         if L.hold_muon_workspace(C.byref(d), C.byref(n)) != 0:
             raise _diverges(what)
         ws = torch.empty(n.value, dtype=torch.uint8, device=device)
-        d.workspace, d.workspace_bytes = ptr(ws), n.value
+        d.workspace, d.workspace_bytes = ws.data_ptr(), n.value
         code = L.hold_muon_step(C.byref(d), stream_ptr())
         if code == -1:
             raise _diverges(what)
