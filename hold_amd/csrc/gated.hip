@@ -615,6 +615,20 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
       short_rows<MODE, KS, FULL>(a.x, a.ldx, row + 16 * m, a.T, a.D, x[m], ex[m]);
       __builtin_amdgcn_sched_barrier(0);
     }
+    f32x4 dhs[MI][BWD ? NF : 1];  // on their way while the products run
+    int rs[MI];
+    if (BWD) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const int64_t i = row + 16 * m + (lane & 15);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          const int j = n0 + 16 * f + jl;
+          dhs[m][BWD ? f : 0] = i < a.T && j < a.H ? load4<MODE>(a.dh, i * a.lddh + j, a.H - j) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        rs[m] = MODE == MODE_F16X3 ? (i < a.T ? a.rscale[i] : NONE) : 0;
+      }
+    }
     f32x4 acc[2][MI][NF];
 #pragma unroll
     for (int w = 0; w < 2; ++w)
@@ -644,16 +658,6 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
     for (int m = 0; m < MI; ++m) {
       const int64_t i = row + 16 * m + (lane & 15);
       const bool live = i < a.T;
-      f32x4 dhs[BWD ? NF : 1];
-      int rs = 0;
-      if (BWD) {
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          const int j = n0 + 16 * f + jl;
-          dhs[BWD ? f : 0] = live && j < a.H ? load4<MODE>(a.dh, i * a.lddh + j, a.H - j) : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        if (MODE == MODE_F16X3) rs = live ? a.rscale[i] : NONE;
-      }
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
         const int j = n0 + 16 * f + jl, n = a.H - j;
@@ -683,8 +687,8 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
               float s, d;
               activate<true, MODE == MODE_F16X3>(a.act, g[r], s, d);
               if (r < n) {
-                dg[r] = dhs[BWD ? f : 0][r] * u[r] * d;
-                du[r] = dhs[BWD ? f : 0][r] * s;
+                dg[r] = dhs[m][BWD ? f : 0][r] * u[r] * d;
+                du[r] = dhs[m][BWD ? f : 0][r] * s;
               }
             }
           }
@@ -696,8 +700,8 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
               store4<MODE>(a.dg, o, 4, dg);
               store4<MODE>(a.du, o, 4, du);
             } else {
-              put_limbs(a.dg + o, a.dlimb, dg, rs == NONE ? 0 : rs);
-              put_limbs(a.du + o, a.dlimb, du, rs == NONE ? 0 : rs + shift);
+              put_limbs(a.dg + o, a.dlimb, dg, rs[m] == NONE ? 0 : rs[m]);
+              put_limbs(a.du + o, a.dlimb, du, rs[m] == NONE ? 0 : rs[m] + shift);
             }
           }
         }
