@@ -1072,7 +1072,7 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
     }
     if (d.db_gate || d.db_up) p.dbpart = take(p.row_tiles * 2 * d.H * 4);
     const int64_t x256 = cdiv(d.T, 256) * cdiv(d.D, 256), x128 = cdiv(d.T, 128) * cdiv(d.D, 128);
-    p.dx_big = x256 >= 200 && large_tiles(x256, x128, cdiv(p.Hp, step));
+    p.dx_big = x256 >= 200 && large_tiles(x256, x128, 2 * cdiv(p.Hp, step));
     split_sum(p.dx_big ? 512 : x128, p.Hp, 512, p.dx_splits, p.dx_chunk);
     const int64_t w256 = 2 * cdiv(d.H, 256) * cdiv(d.D, 256), w128 = 2 * cdiv(d.H, 128) * cdiv(d.D, 128);
     p.dw_big = w256 >= 200 && large_tiles(w256, w128, cdiv(d.T, step));
