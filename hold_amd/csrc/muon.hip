@@ -405,6 +405,195 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
   }
 }
 
+// ---- small matrices: a block each, the whole iteration in LDS ----------------------------------------------------------------------------------
+// X and A as limbs in LDS; 16 waves take 32 x 32 blocks of each product, results wait in registers until everyone has read.  One launch instead of 2 + 3 a step, which for a 64 x 64
+// matrix are 66 us of launches; @@.
+constexpr int SMALL_STEPS = 8, SMALL_LDS = 160 * 1024 - 1024, SMALL_BLOCKS = 32;
+struct SmallSteps {
+  float a[SMALL_STEPS], b[SMALL_STEPS], c[SMALL_STEPS];
+  int gram[SMALL_STEPS], apply[SMALL_STEPS], n, xs;
+};
+inline int up32(int v) { return (v + 31) / 32 * 32; }
+// A row's pitch in elements and the exchange of its 16-byte chunks, so that neither a fragment by rows nor one by k meets a bank twice: rows of
+// multiples of 256 bytes exchange eight pairs of chunks; others are an odd multiple of 64 bytes long, which spreads 4 rows over the banks, and
+// exchange fours
+__host__ __device__ __forceinline__ int small_pitch(int n32) { return n32 % 128 == 0 ? n32 : (n32 / 32 | 1) * 32; }
+__device__ __forceinline__ int small_swz(int pitch, int r) { return pitch % 128 == 0 ? ((r & 3) | ((r >> 1) & 4)) << 4 : (-(r >> 2) & 3) << 3; }
+__device__ __forceinline__ int small_at(int pitch, int r, int c) { return r * pitch + (c ^ small_swz(pitch, r)); }
+// elements of the two arrays (one limb); what fits: both limbs of both in LDS, at most two blocks of X a wave
+bool small(const Item& it, int steps) {
+  const int64_t m = it.rows < it.cols ? it.rows : it.cols, n = it.rows < it.cols ? it.cols : it.rows;
+  if (steps > SMALL_STEPS || m > 128 || n > 2048) return false;
+  const int64_t mp = up32((int)m), np = up32((int)n);
+  return 4 * mp * (small_pitch((int)np) + small_pitch((int)mp)) <= SMALL_LDS && (mp / 32) * (np / 32) <= SMALL_BLOCKS;
+}
+
+// acc[mi][ni] of a 32 x 32 block: sum over K of A(i, k) B(j, k); A by rows, B by rows (LB = KC) or by k (KS).  The exchange of chunks depends on
+// a row's place among 16 alone: it is the same for every 16 rows and every 32 k's
+template <int LB>
+__device__ __forceinline__ void small_block(const uint16_t* a, int pa, int la, const uint16_t* b, int pb, int lb, int i0, int j0, int K, f32x4 (&acc)[2][2]) {
+  const int lane = threadIdx.x & 63, row = lane & 15, kl = 8 * (lane >> 4), kr = kl + (row >> 2), xa = small_swz(pa, row), xb = small_swz(pb, row);
+  const uint16_t* ap = a + (i0 + row) * pa;
+  const uint16_t* bp = LB == KC ? b + (j0 + row) * pb : b + kr * pb;
+  const int x0 = small_swz(pb, kr), x1 = small_swz(pb, kr + 4), c = j0 + 4 * (lane & 3);
+  const int o[2][2] = {{c ^ x0, 4 * pb + (c ^ x1)}, {(c + 16) ^ x0, 4 * pb + ((c + 16) ^ x1)}};  // KS: the two halves of two 16-column fragments
+#pragma unroll 1
+  for (int k = 0; k < K; k += 32) {
+    s16x8 fa[2][2], fb[2][2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int l = 0; l < 2; ++l) {
+        fa[q][l] = *(const s16x8*)(ap + l * la + 16 * q * pa + ((k + kl) ^ xa));
+        if (LB == KC) {
+          fb[q][l] = *(const s16x8*)(bp + l * lb + 16 * q * pb + ((k + kl) ^ xb));
+        } else {
+          const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(bp + l * lb + o[q][0]));
+          const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(bp + l * lb + o[q][1]));
+          fb[q][l] = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+      }
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+      for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 2; ++ni) acc[mi][ni] = mfma<MODE_F16X3>(fb[ni][p == 0], fa[mi][p == 1], acc[mi][ni]);
+    if (LB == KS) bp += 32 * pb;
+  }
+}
+
+__global__ __launch_bounds__(1024) void ns_small_kernel(Items a, Firsts t, Step s, SmallSteps st) {
+  __shared__ __align__(16) uint16_t lds[SMALL_LDS / 2];
+  __shared__ double red[16];
+  const int k = last_below(a.n, blockIdx.x, [&](int i) { return t.first[i]; });
+  const Item& it = a.it[k];
+  const int64_t base = (int64_t)(blockIdx.x - t.first[k]) * it.stride;
+  const bool tall = it.rows > it.cols;
+  const int m = tall ? it.cols : it.rows, n = tall ? it.rows : it.cols, mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
+  const int px = small_pitch(np), pa = small_pitch(mp), lx = mp * px, la = mp * pa;
+  uint16_t* X = lds;
+  uint16_t* A = lds + 2 * lx;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const float f = it.m ? grad_scale(s) : 1.f;
+  // momentum and the norm, then X0 from the same thread's elements
+  const int count = it.rows * it.cols;
+  double sum = 0.;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < count; e += 1024) {
+    const int r = e / it.cols, c = e - r * it.cols;
+    const float g = value(it.g, base + (int64_t)r * it.ldg + c, s.dtype);
+    float u = g;
+    if (it.m) {
+      float* p = (float*)it.m + base + (int64_t)r * it.ldm + c;
+      const float gf = g * f, mm = s.mu * *p + s.rest * gf;
+      *p = mm;
+      u = s.nesterov ? s.rest * gf + s.mu * mm : mm;
+    }
+    sum += (double)u * u;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) red[wave] = sum;
+  for (int e = threadIdx.x; e < lx; e += 1024) ((uint32_t*)X)[e] = 0u;  // both limbs, also behind the last row and column
+  __syncthreads();
+  sum = 0.;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) sum += red[w];
+  const double inv = ldexp(1. / (sqrt(sum) + (double)s.eps), st.xs);
+#pragma unroll 4
+  for (int e = threadIdx.x; e < count; e += 1024) {
+    const int r = e / it.cols, c = e - r * it.cols;
+    const Split y = split16((float)(update_of(it, s, f, base, r, c) * inv));
+    uint16_t* x = X + (tall ? small_at(px, c, r) : small_at(px, r, c));
+    x[0] = y.hi;
+    x[lx] = y.lo;
+  }
+  __syncthreads();
+  const int tm = mp / 32, tn = np / 32;
+  auto each = [&](const f32x4 (&acc)[2][2], int i0, int j0, auto put4) {
+#pragma unroll
+    for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+      for (int ni = 0; ni < 2; ++ni) put4(i0 + 16 * mi + (lane & 15), j0 + 16 * ni + 4 * (lane >> 4), acc[mi][ni]);
+  };
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4 x[2][2][2];  // X's blocks of the wave, up to two
+#pragma unroll 1
+  for (int q = 0; q < st.n; ++q) {
+    f32x4 acc[2][2] = {{zero, zero}, {zero, zero}};
+    const int ai = wave / tm * 32, aj = wave % tm * 32;  // tm^2 <= 16 blocks of A
+    if (wave < tm * tm) {
+      small_block<KC>(X, px, lx, X, px, lx, ai, aj, np, acc);
+      each(acc, ai, aj, [&](int i, int j, f32x4 v) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], st.gram[q]);
+        store_limbs(A + small_at(pa, i, j), la, v);
+      });
+    }
+    __syncthreads();
+    f32x4 c[2][2] = {{zero, zero}, {zero, zero}};
+    if (wave < tm * tm) small_block<KC>(A, pa, la, A, pa, la, ai, aj, mp, c);
+    if (wave < tm * tm) {
+#pragma unroll
+      for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 2; ++ni) {
+          const int i = ai + 16 * mi + (lane & 15), j = aj + 16 * ni + 4 * (lane >> 4);
+          const f32x4 u = load_limbs(A + small_at(pa, i, j), la);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) c[mi][ni][r] = fmaf(st.c[q], c[mi][ni][r], st.b[q] * u[r]) + (i == j + r ? st.a[q] : 0.f);
+        }
+    }
+    __syncthreads();
+    if (wave < tm * tm) each(c, ai, aj, [&](int i, int j, f32x4 v) { store_limbs(A + small_at(pa, i, j), la, v); });
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int b = wave + 16 * h;
+#pragma unroll
+      for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 2; ++ni) x[h][mi][ni] = zero;
+      if (b < tm * tn) small_block<KS>(A, pa, la, X, px, lx, b / tn * 32, b % tn * 32, mp, x[h]);
+    }
+    if (q + 1 == st.n) break;
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int b = wave + 16 * h;
+      if (b < tm * tn)
+        each(x[h], b / tn * 32, b % tn * 32, [&](int i, int j, f32x4 v) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], st.apply[q]);
+          store_limbs(X + small_at(px, i, j), lx, v);
+        });
+    }
+    __syncthreads();
+  }
+  const int shift = st.apply[st.n - 1];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int b = wave + 16 * h;
+    if (b < tm * tn)
+      each(x[h], b / tn * 32, b % tn * 32, [&](int i, int j, f32x4 v) {
+        if (i >= m) return;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (j + r >= n) continue;
+          const int64_t at = base + (tall ? (int64_t)(j + r) * it.ldp + i : (int64_t)i * it.ldp + j + r);
+          const float y = ldexpf(v[r], shift);
+          if (it.m) {
+            float* p = (float*)it.p + at;
+            *p = *p * s.decay - it.gain * y;
+          } else {
+            put(it.p, at, s.dtype, y);
+          }
+        }
+      });
+  }
+}
+
 inline int ok() { return hipGetLastError() == hipSuccess ? HOLD_OK : HOLD_E_LAUNCH; }
 
 // The bounds of the singular values of X, and of the entries of A and C, through the iteration; false: they leave the range of the limbs
@@ -526,32 +715,40 @@ void launch_tiles(const Classes& cl, const NsArgs& s, const Step& st, const Item
   }
 }
 
-// The tile size by the time of the launch in units of one 256 x 256 tile per compute unit: rounds of blocks over the 256 units times a
-// block's share.  256 and 192: one block a unit; 128: two, 64: four; the smaller tiles' lower rates (more LDS reads and loads a product)
-// are measured on 4096^3: 1310 / 1400 (192, counted without its idle units) / 1135 / 620 TFLOP/s of limb products.
+// The tile size by the launch's time, rounds of blocks over the 256 compute units at (per k + fixed) microseconds.  256 and 192: one block a
+// unit; 128: two; 64 (three stages of LDS): three; a last round that leaves units with fewer blocks is shorter.  Fitted to launches alone
+// on single matrices of 1500 .. 4096 and batches of 256 .. 1024 rows, each with every tile size: 4096^3 takes 255 us in 256 x 256
+// tiles, 2 x 154 in 128, 5.3 x 119 in 64; 36 matrices of 256 x 256 in 64 8 us a product, 14 in 128.
+struct TileCost {
+  int size, units;                   // rows; blocks of a full round
+  double full[2], two[2], alone[2];  // a round: full, of up to 512 blocks (64), of up to 256
+};
+const TileCost COST[4] = {{256, 256, {.0535, 36.}, {.0535, 36.}, {.0535, 36.}},
+                          {192, 256, {.0535, 6.}, {.0535, 6.}, {.0535, 6.}},
+                          {128, 512, {.034, 15.}, {.034, 15.}, {.026, 13.}},
+                          {64, 768, {.025, 3.}, {.016, 4.}, {.012, 4.}}};
+
 template <int KIND, bool LAST>
 int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStream_t stream) {
-  const int T[4] = {256, 192, 128, 64}, at_once[4] = {256, 256, 512, 1024};
-  const double cost[4] = {1., 0.55, 0.58, 0.55};  // of a full round
+  double K = 0.;  // the longest sum
+  for (int k = 0; k < cl.n; ++k) K = fmax(K, KIND == GRAM ? cl.k[k].np : cl.k[k].mp);
   int best = -1;
   double least = 0.;
   for (int k = 0; k < 4; ++k) {
-    const int64_t n = count_tiles<KIND>(cl, T[k]);
+    const TileCost& c = COST[k];
+    const int64_t n = count_tiles<KIND>(cl, c.size);
     if (n < 0) continue;
-    const int64_t rounds = (n + at_once[k] - 1) / at_once[k], per_unit = (n + 255) / 256;
-    // a round that does not fill the units' places is as long as its blocks alone, half of a full one for 128, a third for 64
-    double t = cost[k] * (double)rounds;
-    if (rounds == 1 && k >= 2) t = cost[k] * (0.35 + 0.65 * (double)per_unit / (k == 2 ? 2. : 4.));
+    const int64_t rest = n % c.units;
+    const double* last = rest <= 256 ? c.alone : rest <= 512 ? c.two : c.full;
+    const double t = (double)(n / c.units) * (K * c.full[0] + c.full[1]) + (rest ? K * last[0] + last[1] : 0.);
     if (best < 0 || t < least) { best = k; least = t; }
   }
   if (best < 0) return HOLD_E_ARG;
-  const unsigned n = (unsigned)count_tiles<KIND>(cl, T[best]);
+  const unsigned n = (unsigned)count_tiles<KIND>(cl, COST[best].size);
   if (best == 0) launch_tiles<KIND, 256, 4, 4, 2, true, LAST>(cl, s, st, a, n, stream);
   else if (best == 1) launch_tiles<KIND, 192, 3, 4, 2, false, LAST>(cl, s, st, a, n, stream);
   else if (best == 2) launch_tiles<KIND, 128, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
-  // with a block to itself a unit has the whole LDS: all of 256 k's in flight at once (one 256 x 256: 7.1 -> @@ us a launch)
-  else if (n <= 256) launch_tiles<KIND, 64, 2, 2, 8, false, LAST>(cl, s, st, a, n, stream);
-  else launch_tiles<KIND, 64, 2, 2, 4, false, LAST>(cl, s, st, a, n, stream);
+  else launch_tiles<KIND, 64, 2, 2, 3, false, LAST>(cl, s, st, a, n, stream);
   return HOLD_OK;
 }
 
@@ -652,6 +849,34 @@ int run_group(Items& a, bool join, const Step& st, const float* coef, int steps,
   return rc == HOLD_OK ? ok() : rc;
 }
 
+int run_small(const Items& a, const Step& st, const float* coef, int steps, hipStream_t stream) {
+  Bounds bo;
+  if (!follow(coef, steps, bo)) return HOLD_E_ARG;
+  SmallSteps ss = {};
+  ss.n = steps;
+  ss.xs = bo.xs[0];
+  for (int k = 0; k < steps; ++k) {
+    ss.gram[k] = bo.as[k] - 2 * bo.xs[k];
+    ss.a[k] = (float)ldexp((double)coef[3 * k], bo.cs[k]);
+    ss.b[k] = (float)ldexp((double)coef[3 * k + 1], bo.cs[k] - bo.as[k]);
+    ss.c[k] = (float)ldexp((double)coef[3 * k + 2], bo.cs[k] - 2 * bo.as[k]);
+    ss.apply[k] = (k + 1 == steps ? 0 : bo.xs[k + 1]) - bo.cs[k] - bo.xs[k];
+  }
+  Firsts t = {};
+  int64_t n = 0;
+  for (int k = 0; k < a.n; ++k) {
+    t.first[k] = (int)n;
+    n += a.it[k].count;
+    if (n > (1 << 30)) return HOLD_E_ARG;
+  }
+  hipLaunchKernelGGL(ns_small_kernel, dim3((unsigned)n), dim3(1024), 0, stream, a, t, st, ss);
+  return ok();
+}
+
+// how an item is computed: in one block's LDS, step by step, or with steps joined
+enum { SMALL = 0, PLAIN = 1, JOIN = 2 };
+int way_of(const Item& it, bool exact, int steps) { return small(it, steps) ? SMALL : joined(it, exact) ? JOIN : PLAIN; }
+
 bool sizes_ok(int64_t rows, int64_t cols, int64_t count) {
   return rows >= 1 && cols >= 1 && count >= 1 && rows <= (1 << 20) && cols <= (1 << 20) && count <= (1 << 24);
 }
@@ -676,23 +901,23 @@ bool read_item(const hold_muon_desc* d, int k, Item& it) {
   it.gain = (float)(d->lr * i.scale);
   return true;
 }
-// calls f(items, join) for the groups of a step: those whose steps are joined, then the others, up to MAXI a group; false: a bad item
+// calls f(items, way) for the groups of a step, up to MAXI items that are computed alike; false: a bad item
 template <class F>
 bool groups_of(const hold_muon_desc* d, F f) {
-  for (int join = 1; join >= 0; --join) {
+  for (int way = JOIN; way >= SMALL; --way) {
     Items a;
     a.n = 0;
     for (int k = 0; k < d->n_items; ++k) {
       Item it;
       if (!read_item(d, k, it)) return false;
-      if (joined(it, false) != (join != 0)) continue;
+      if (way_of(it, false, d->steps) != way) continue;
       a.it[a.n++] = it;
       if (a.n == MAXI) {
-        if (!f(a, join != 0)) return false;
+        if (!f(a, way)) return false;
         a.n = 0;
       }
     }
-    if (a.n && !f(a, join != 0)) return false;
+    if (a.n && !f(a, way)) return false;
   }
   return true;
 }
@@ -703,7 +928,8 @@ extern "C" int hold_orthogonalize_workspace(const hold_ortho_desc* d, int64_t* b
   Items a;
   Classes cl;
   if (!one_item(d, a) || !bytes) return HOLD_E_ARG;
-  *bytes = room(a, cl, joined(a.it[0], d->dtype == HOLD_MUON_F32)).bytes;
+  const int way = way_of(a.it[0], d->dtype == HOLD_MUON_F32, d->steps);
+  *bytes = way == SMALL ? 256 : room(a, cl, way == JOIN).bytes;
   return HOLD_OK;
 }
 
@@ -717,15 +943,18 @@ extern "C" int hold_orthogonalize(const hold_ortho_desc* d, hold_stream_t stream
   Step st = {};
   st.eps = d->eps;
   st.dtype = d->dtype;
-  return run_group(a, joined(a.it[0], d->dtype == HOLD_MUON_F32), st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+  const int way = way_of(a.it[0], d->dtype == HOLD_MUON_F32, d->steps);
+  if (way == SMALL) return run_small(a, st, d->coef, d->steps, (hipStream_t)stream);
+  return run_group(a, way == JOIN, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
 }
 
 extern "C" int hold_muon_workspace(const hold_muon_desc* d, int64_t* bytes) {
   if (!d || !bytes || d->n_items < 1 || !d->items) return HOLD_E_ARG;
-  *bytes = 0;
-  return groups_of(d, [&](Items& a, bool join) {
+  *bytes = 256;
+  return groups_of(d, [&](Items& a, int way) {
+    if (way == SMALL) return true;
     Classes cl;
-    const int64_t n = room(a, cl, join).bytes;
+    const int64_t n = room(a, cl, way == JOIN).bytes;
     if (n > *bytes) *bytes = n;
     return true;
   }) ? HOLD_OK : HOLD_E_ARG;
@@ -749,8 +978,9 @@ extern "C" int hold_muon_step(const hold_muon_desc* d, hold_stream_t stream) {
   st.clip = d->clip_norm;
   st.sumsq = d->sumsq;
   int rc = HOLD_OK;  // groups share the workspace: they run one after the other
-  groups_of(d, [&](Items& a, bool join) {
-    rc = run_group(a, join, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+  groups_of(d, [&](Items& a, int way) {
+    rc = way == SMALL ? run_small(a, st, d->coef, d->steps, (hipStream_t)stream)
+                      : run_group(a, way == JOIN, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
     return rc == HOLD_OK;
   });
   return rc;

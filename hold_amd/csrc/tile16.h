@@ -304,17 +304,21 @@ struct Core {
     // loads a wave issues per stage: the same for every wave, or S == 2
     constexpr int LPS = NL * (Loader<LA, BM, BK, NW>::N + NB * Loader<LB, BN, BK, NW>::N), AHEAD = (S - 2) * LPS;
     static_assert(S == 2 || (Loader<LA, BM, BK, NW>::EVEN && Loader<LB, BN, BK, NW>::EVEN && AHEAD < 63), "countable loads");
+    const bool all = S > 2 && nk <= S;  // a sum that fits: one wait for everything
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
       if (i < nk) stage(i, smem + i * STAGE);
+    if (all && nk == S) stage(S - 1, smem + (S - 1) * STAGE);
     int at = 0, to = S - 1;  // the stage that is read, the stage that is filled
     for (int kt = 0; kt < nk; ++kt) {
       const char* s = smem + at * STAGE;
-      if (S == 2 || kt + S - 1 > nk) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (kt + S - 1 < nk) stage(kt + S - 1, smem + to * STAGE);
+      if (!all || kt == 0) {
+        if (S == 2 || all || kt + S - 1 > nk) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      if (!all && kt + S - 1 < nk) stage(kt + S - 1, smem + to * STAGE);
       at = at + 1 == S ? 0 : at + 1;
       to = to + 1 == S ? 0 : to + 1;
       const char* sa = s;

@@ -77,7 +77,7 @@ def _ortho(**kw):
     coef = (C.c_float * 96)(*([3.4445, -4.7750, 2.0315] * 32))
     d = OrthoDesc()
     d.x, d.out, d.coef, d.workspace, d.workspace_bytes = 4096, 8192, C.cast(coef, C.POINTER(C.c_float)), 0, 0  # never a launch: no workspace
-    d.batch, d.rows, d.cols, d.dtype, d.steps, d.eps = 2, 20, 30, 0, 5, 1e-7
+    d.batch, d.rows, d.cols, d.dtype, d.steps, d.eps = 2, 200, 300, 0, 5, 1e-7
     for k, v in kw.items():
         setattr(d, k, v)
     d._keep = coef
@@ -88,7 +88,7 @@ def test_entry_points_refuse_bad_descriptors():
     from hold_amd import _lib, build
     build.build()
     L, n = _lib.lib(), C.c_int64()
-    assert L.hold_orthogonalize_workspace(C.byref(_ortho()), C.byref(n)) == 0 and n.value > 2 * 20 * 30 * 8
+    assert L.hold_orthogonalize_workspace(C.byref(_ortho()), C.byref(n)) == 0 and n.value > 2 * 200 * 300 * 8
     need = n.value
     for bad in (dict(batch=0), dict(rows=0), dict(cols=0), dict(rows=(1 << 20) + 1), dict(batch=(1 << 24) + 1)):
         assert L.hold_orthogonalize_workspace(C.byref(_ortho(**bad)), C.byref(n)) == -1

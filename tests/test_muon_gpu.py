@@ -59,8 +59,10 @@ def joins(x):
     return n >= 1.5 * m and m * m * n * (x.numel() // (m * n)) >= 1e9 and x.dtype != torch.float32
 
 
+# the borders of the kernel for small matrices among them: (128, 160) and (32, 1024) are its largest, (128, 161), (129, 129) and (31, 1025) are not its
 SHAPES = [(1, 1), (1, 7), (9, 1), (2, 3), (8, 8), (5, 64), (33, 47), (64, 64), (65, 64), (72, 130), (257, 63), (256, 256), (256, 84), (256, 304),
-          (3, 31, 40), (2, 2, 100, 36), (5, 1, 1), (24, 130, 129)]
+          (3, 31, 40), (2, 2, 100, 36), (5, 1, 1), (24, 130, 129), (128, 128), (160, 128), (128, 161), (129, 129), (32, 1024), (31, 1025), (2, 96, 250),
+          (64, 512), (513, 64), (300, 17, 50)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -135,7 +137,7 @@ def test_singular_values_come_near_one():
 def test_steps_and_coefficients():
     from hold_amd.muon import orthogonalize
     x = make(70, 90)
-    for steps in (1, 2, 7):
+    for steps in (1, 2, 7, 8, 9):  # nine are too many for the kernel for small matrices
         assert off(orthogonalize(x, steps=steps), iterate(x.double(), steps=steps)) <= allowed(x, steps=steps)
     cubic = (1.5, -0.5, 0.0)
     assert off(orthogonalize(x, steps=12, coefficients=cubic), iterate(x.double(), 12, cubic)) <= allowed(x, steps=12, coefficients=cubic)
