@@ -7,7 +7,7 @@
 // KERNELS.  gated_mma_kernel: both projections of a tile share the x tile in LDS, the epilogue applies bias, activation and product
 // (forward) or forms dg, du from dh and the recomputed g, u (backward), with the column sums for the bias gradients from the
 // unrounded values.  gated_dx_kernel: [dg | du] times [Wg; Wu] as one sum.  gated_dw_kernel: both weight gradients, the sum over
-// tokens split over blocks into fp32 partial tiles that gated_dw_reduce_kernel adds in a fixed order.  gated_rows_kernel: T <= 64 rows.
+// tokens split over blocks into fp32 partial tiles that gated_finish_kernel adds in a fixed order.  gated_rows_kernel: T <= 64 rows.
 //
 // ROUNDINGS.  bf16: dg and du are rounded to bf16 once, as the operands of the next matrix instructions; everything before is fp32.
 // fp32: every operand is split into two fp16 limbs (tile16.h) after an exact power-of-two scale: a row of x by its own largest
@@ -370,9 +370,9 @@ struct MmaArgs {
   int tm, tn;
 };
 
-template <int MODE, bool BWD, int BM, int BN, int WM, int WN, bool PHASED>
+template <int MODE, bool BWD, int BM, int BN, int WM, int WN, bool PHASED, int S = 2>
 __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
-  using Cr = Core<MODE, KC, KC, BM, BN, 2, WM, WN>;
+  using Cr = Core<MODE, KC, KC, BM, BN, 2, WM, WN, S>;
   __shared__ __align__(1024) char smem[Cr::LDS];
   int tm, tn;
   tile_of(blockIdx.x, gridDim.x, a.tm, a.tn, 8, tm, tn);
@@ -724,26 +724,6 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
   }
 }
 
-// db[w][j] = sum over the row tiles, in 16 interleaved chains per column joined in a fixed order
-template <int MODE>
-__global__ __launch_bounds__(1024) void gated_db_kernel(const float* part, int tiles, int H, void* dbg, void* dbu) {
-  const int w = blockIdx.y, c = threadIdx.x & 63, j = blockIdx.x * 64 + c, q = threadIdx.x >> 6;
-  __shared__ float s[16][64];
-  float v = 0.f;
-  if (j < H)
-    for (int t = q; t < tiles; t += 16) v += part[((int64_t)t * 2 + w) * H + j];
-  s[q][c] = v;
-  __syncthreads();
-  void* out = w ? dbu : dbg;
-  if (q == 0 && j < H && out) {
-#pragma unroll
-    for (int k = 8; k > 0; k >>= 1)
-#pragma unroll
-      for (int i = 0; i < k; ++i) s[i][c] += s[i + k][c];
-    store1<MODE>(out, j, s[0][c]);
-  }
-}
-
 // ---- dx = dg Wg + du Wu -----------------------------------------------------------------------------------------------------------------
 struct DxArgs {
   const uint16_t* dg; const uint16_t* du; int64_t Hp, dlimb;
@@ -844,17 +824,44 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dw_kernel(DwArgs a) {
   }
 }
 
-// the sum of the splits' parts in their order; `sets` results lie side by side in a split's part
+// ---- what is left: the parts of dx and dW in the order of their splits, the column sums of the bias gradients -----------------------------------
+struct FinishArgs {
+  const float* part[2]; int splits[2], sets[2]; int64_t n[2];  // dx, dW: `sets` results of n lie side by side in a split's part
+  void* out[2][2];
+  const float* db; int tiles, H;                               // [tiles][2][H]
+  void* dbg; void* dbu;
+  int first[3];                                                // first block of dW, of db; blocks
+};
 template <int MODE>
-__global__ __launch_bounds__(256) void gated_reduce_kernel(const float* part, int splits, int sets, int64_t n, void* out0, void* out1) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  const int w = blockIdx.y;
+__global__ __launch_bounds__(256) void gated_finish_kernel(FinishArgs a) {
+  const int id = blockIdx.x;
+  if (id >= a.first[1]) {  // 16 columns, 16 interleaved chains each, joined in a fixed order
+    const int cols = (a.H + 15) / 16, q = id - a.first[1], w = q / cols, c = threadIdx.x & 15, j = q % cols * 16 + c, t0 = threadIdx.x >> 4;
+    __shared__ float s[16][16];
+    float v = 0.f;
+    if (j < a.H)
+#pragma unroll 4
+      for (int t = t0; t < a.tiles; t += 16) v += a.db[((int64_t)t * 2 + w) * a.H + j];
+    s[t0][c] = v;
+    __syncthreads();
+    void* out = w ? a.dbu : a.dbg;
+    if (t0 == 0 && j < a.H && out) {
+#pragma unroll
+      for (int k = 8; k > 0; k >>= 1)
+#pragma unroll
+        for (int i = 0; i < k; ++i) s[i][c] += s[i + k][c];
+      store1<MODE>(out, j, s[0][c]);
+    }
+    return;
+  }
+  const int r = id >= a.first[0];
+  const int64_t n = a.n[r], per = (n + 1023) / 1024, q = id - (r ? a.first[0] : 0), w = q / per, i = (q % per * 256 + threadIdx.x) * 4;
   if (i >= n) return;
   const int m = n - i < 4 ? (int)(n - i) : 4;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < splits; ++s) v += load4<MODE_F16X3>(part, ((int64_t)s * sets + w) * n + i, m);
-  store4<MODE>(w ? out1 : out0, i, m, v);
+  for (int s = 0; s < a.splits[r]; ++s) v += load4<MODE_F16X3>(a.part[r], ((int64_t)s * a.sets[r] + w) * n + i, m);
+  store4<MODE>(a.out[r][w], i, m, v);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------
@@ -1015,11 +1022,11 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // where everything of one call lies in its workspace (bytes; every part starts on a multiple of 256)
 struct Plan {
   bool copy_x, copy_w[2];
-  bool brief, big, dx_big, dw_big;  // brief: the kernel for short rows
+  bool brief, big, little, dx_big, dw_big;  // brief: the kernel for short rows; big, little: tiles of 256 and of 64 rows
   int64_t parts, part_rows;
   int64_t Dp, Hp, row_tiles, pack_blocks;
   int64_t dx_splits, dx_chunk, dw_splits, dw_chunk;
-  int64_t x, w, dg, xt, part, exps, rowexp, colexp, rscale, dbpart, sums, spart, bytes;
+  int64_t x, w, dg, xt, part, exps, rowexp, colexp, rscale, dbpart, dx_sums, dw_sums, spart, bytes;
 };
 
 bool aligned16(const void* p, int64_t ld, int es) { return (uintptr_t)p % 16 == 0 && (ld * es) % 16 == 0; }
@@ -1052,7 +1059,10 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
   p.part_rows = cdiv(rounds, parts) * round;
   p.parts = cdiv(d.T, p.part_rows);
   p.big = large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64), cdiv(p.Dp, step));
-  p.row_tiles = p.brief ? p.parts * SHORT_WAVES : cdiv(d.T, p.big ? 256 : 128);
+  // less than a block a unit of 128 x (64 + 64): tiles a quarter of that, four stages deep, their loads three steps ahead
+  // (2019 x 2816 -> 32 in fp32: @@ -> @@ us; 1237 x 517 -> 1021 in bf16: @@ -> @@)
+  p.little = !p.big && cdiv(d.T, 128) * cdiv(d.H, 64) <= 64;
+  p.row_tiles = p.brief ? p.parts * SHORT_WAVES : cdiv(d.T, p.big ? 256 : p.little ? 64 : 128);
   p.pack_blocks = rows_grid(d.T + 2 * (int64_t)d.H);
   if (p.brief && !bwd) return p;  // takes everything as it is
   p.x = p.copy_x && !(p.brief && f32) ? take(d.T * p.Dp * 2 * nl) : 0;
@@ -1077,10 +1087,8 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
     const int64_t w256 = 2 * cdiv(d.H, 256) * cdiv(d.D, 256), w128 = 2 * cdiv(d.H, 128) * cdiv(d.D, 128);
     p.dw_big = w256 >= 200 && large_tiles(w256, w128, cdiv(d.T, step));
     split_sum(p.dw_big ? 512 : w128, d.T, 512, p.dw_splits, p.dw_chunk);
-    int64_t sums = p.dx_splits > 1 ? p.dx_splits * d.T * d.D * 4 : 0;  // dx's parts are added before dW's are written
-    const int64_t more = p.dw_splits > 1 ? p.dw_splits * 2 * (int64_t)d.H * d.D * 4 : 0;
-    sums = more > sums ? more : sums;
-    if (sums) p.sums = take(sums);
+    if (p.dx_splits > 1) p.dx_sums = take(p.dx_splits * d.T * d.D * 4);
+    if (p.dw_splits > 1) p.dw_sums = take(p.dw_splits * 2 * (int64_t)d.H * d.D * 4);
   }
   p.bytes = o;
   return p;
@@ -1176,6 +1184,9 @@ void launch_mma(const hold_gated_desc& d, MmaArgs a, const Plan& p, hipStream_t 
   } else if (p.big) {
     a.tm = (int)cdiv(a.T, 256); a.tn = (int)cdiv(a.H, 128);
     hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 256, 128, 4, 4, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
+  } else if (p.little) {
+    a.tm = (int)cdiv(a.T, 64); a.tn = (int)cdiv(a.H, 32);
+    hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 64, 32, 2, 1, false, 4>), dim3((unsigned)(a.tm * a.tn)), dim3(128), 0, st, a);
   } else {
     a.tm = (int)cdiv(a.T, 128); a.tn = (int)cdiv(a.H, 64);
     hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 128, 64, 4, 2, false>), dim3((unsigned)(a.tm * a.tn)), dim3(512), 0, st, a);
@@ -1237,24 +1248,23 @@ int bwd(const hold_gated_desc& d, hipStream_t st) {
   a.dg = (uint16_t*)(ws + p.dg); a.du = a.dg + NL * DN; a.dlimb = DN;
   a.dbpart = d.db_gate || d.db_up ? (float*)(ws + p.dbpart) : nullptr;
   launch_mma<MODE, true>(d, a, p, st);
-  if (a.dbpart)
-    hipLaunchKernelGGL(gated_db_kernel<MODE>, dim3((unsigned)((d.H + 63) / 64), 2), dim3(1024), 0, st, a.dbpart, (int)p.row_tiles, d.H, d.db_gate, d.db_up);
-  float* sums = (float*)(ws + p.sums);
+  FinishArgs f = {};
   if (d.dx) {
     DxArgs x = {};
     x.dg = a.dg; x.du = a.du; x.Hp = p.Hp; x.dlimb = DN;
     x.wg = a.wg; x.wu = a.wu; x.ldwg = a.ldwg; x.ldwu = a.ldwu; x.wlimb = a.wlimb;
     x.T = d.T; x.H = d.H; x.D = d.D;
     x.rscale = a.rscale; x.exps = a.exps;
-    x.dx = d.dx; x.chunk = p.dx_chunk; x.splits = (int)p.dx_splits; x.part = sums;
+    x.dx = d.dx; x.chunk = p.dx_chunk; x.splits = (int)p.dx_splits; x.part = (float*)(ws + p.dx_sums);
     const int t = p.dx_big ? 256 : 128;
     x.tm = (int)cdiv(d.T, t); x.tn = (int)cdiv(d.D, t);
     const unsigned blocks = (unsigned)(x.tm * x.tn * x.splits);
     if (p.dx_big) hipLaunchKernelGGL((gated_dx_kernel<MODE, 256, 256, 4, 4, true>), dim3(blocks), dim3(1024), 0, st, x);
     else hipLaunchKernelGGL((gated_dx_kernel<MODE, 128, 128, 2, 4, false>), dim3(blocks), dim3(512), 0, st, x);
     if (x.splits > 1) {
-      const int64_t n = d.T * d.D;
-      hipLaunchKernelGGL(gated_reduce_kernel<MODE>, dim3((unsigned)cdiv(n, 1024)), dim3(256), 0, st, sums, x.splits, 1, n, d.dx, d.dx);
+      f.part[0] = x.part; f.splits[0] = x.splits; f.sets[0] = 1; f.n[0] = d.T * d.D;
+      f.out[0][0] = d.dx;
+      f.first[0] = (int)cdiv(f.n[0], 1024);
     }
   }
   if (d.dw_gate) {
@@ -1263,17 +1273,24 @@ int bwd(const hold_gated_desc& d, hipStream_t st) {
     w.x = F32 ? (const uint16_t*)(ws + p.xt) : a.x; w.ldx = F32 ? p.Dp : a.ldx; w.xlimb = F32 ? XN : 0;
     w.T = d.T; w.H = d.H; w.D = d.D;
     w.chunk = p.dw_chunk; w.splits = (int)p.dw_splits; w.exps = a.exps;
-    w.out[0] = d.dw_gate; w.out[1] = d.dw_up; w.part = sums;
+    w.out[0] = d.dw_gate; w.out[1] = d.dw_up; w.part = (float*)(ws + p.dw_sums);
     const int t = p.dw_big ? 256 : 128;
     w.tm = (int)cdiv(d.H, t); w.tn = (int)cdiv(d.D, t);
     const unsigned blocks = (unsigned)(2 * w.tm * w.tn * w.splits);
     if (p.dw_big) hipLaunchKernelGGL((gated_dw_kernel<MODE, 256, 256, 4, 4, true>), dim3(blocks), dim3(1024), 0, st, w);
     else hipLaunchKernelGGL((gated_dw_kernel<MODE, 128, 128, 2, 4, false>), dim3(blocks), dim3(512), 0, st, w);
     if (w.splits > 1) {
-      const int64_t n = (int64_t)d.H * d.D;
-      hipLaunchKernelGGL(gated_reduce_kernel<MODE>, dim3((unsigned)cdiv(n, 1024), 2), dim3(256), 0, st, sums, w.splits, 2, n, d.dw_gate, d.dw_up);
+      f.part[1] = w.part; f.splits[1] = w.splits; f.sets[1] = 2; f.n[1] = (int64_t)d.H * d.D;
+      f.out[1][0] = d.dw_gate; f.out[1][1] = d.dw_up;
     }
   }
+  f.first[1] = f.first[0] + (int)(2 * cdiv(f.n[1], 1024));
+  f.first[2] = f.first[1];
+  if (a.dbpart) {
+    f.db = a.dbpart; f.tiles = (int)p.row_tiles; f.H = d.H; f.dbg = d.db_gate; f.dbu = d.db_up;
+    f.first[2] += (int)(2 * cdiv(d.H, 16));
+  }
+  if (f.first[2]) hipLaunchKernelGGL(gated_finish_kernel<MODE>, dim3((unsigned)f.first[2]), dim3(256), 0, st, f);
   return ok();
 }
 

@@ -274,7 +274,7 @@ struct NsArgs {
   const uint16_t* r;
   uint16_t* o;        // m x m result of GRAM, POLY and PROD
   int64_t xlimb, climb;
-  float a, b, c;      // POLY, already in the scales of its operands and its result
+  float a, b, c;      // POLY, already in the scales of its operands and its result; APPLY: a, where C comes without a I
   int shift;          // exponent from the accumulated sum to the stored limbs
 };
 
@@ -309,6 +309,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
     j0 = (tile - bi * (bi + 1) / 2) * T;
   }
   const int64_t xo = c.x + (int64_t)mat * mp * np, co = c.c + (int64_t)mat * mp * mp;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
   typename Cr::Acc acc;
   Cr::zero(acc);
   Operand A, B[1];
@@ -322,9 +323,14 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
     A = Operand{s.l + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
     B[0] = Operand{s.x + xo + j0, s.xlimb, np, np - j0, mp};
   }
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  // the small tiles' launches are latencies: POLY's own tile of A is requested before the products, not behind them
-  constexpr bool EARLY = KIND == POLY && T <= 64;
+  // POLY adds b A, APPLY a X (where C comes without a I: X itself, in one rounding, instead of the limbs of a diagonal that is large against
+  // the rest of C; in front of the sum every addition would round at its size).  The small tiles' launches are latencies: there the own tile
+  // is requested before the products, not behind them
+  constexpr bool EARLY = (KIND == POLY || KIND == APPLY) && T <= 64;
+  const uint16_t* own = KIND == POLY ? s.l + co : s.x + xo;
+  const int64_t olimb = KIND == POLY ? s.climb : s.xlimb;
+  const int opitch = KIND == APPLY ? np : mp;
+  const bool adds = KIND == POLY || (KIND == APPLY && s.a != 0.f);
   f32x4 early[EARLY ? Cr::MI : 1][EARLY ? Cr::NI : 1];
   if (EARLY) {
 #pragma unroll
@@ -332,7 +338,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
 #pragma unroll
       for (int ni = 0; ni < Cr::NI; ++ni) {
         const int i = i0 + wm * (T / WM) + 16 * mi + (lane & 15), j = j0 + wn * (T / WN) + 16 * ni + 4 * (lane >> 4);
-        early[EARLY ? mi : 0][EARLY ? ni : 0] = i < mp && j < mp ? load_limbs(s.l + co + (int64_t)i * mp + j, s.climb) : f32x4{0.f, 0.f, 0.f, 0.f};
+        early[EARLY ? mi : 0][EARLY ? ni : 0] = adds && i < mp && j < opitch ? load_limbs(own + (int64_t)i * opitch + j, olimb) : f32x4{0.f, 0.f, 0.f, 0.f};
       }
   }
   if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
@@ -353,12 +359,13 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
         if (in) store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
       } else if (KIND == POLY) {
         if (in) {
-          const f32x4 u = EARLY ? early[EARLY ? mi : 0][EARLY ? ni : 0] : load_limbs(s.l + co + (int64_t)i * mp + j, s.climb);
+          const f32x4 u = EARLY ? early[EARLY ? mi : 0][EARLY ? ni : 0] : load_limbs(own + (int64_t)i * opitch + j, olimb);
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = fmaf(s.c, v[r], s.b * u[r]) + (i == j + r ? s.a : 0.f);
           store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
         }
       } else {
+        if (adds && in) v += s.a * (EARLY ? early[EARLY ? mi : 0][EARLY ? ni : 0] : load_limbs(own + (int64_t)i * opitch + j, olimb));
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], s.shift);
         if constexpr (!LAST) {
@@ -539,10 +546,8 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(Items a, Firsts t, Step 
       for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
         for (int ni = 0; ni < 2; ++ni) {
-          const int i = ai + 16 * mi + (lane & 15), j = aj + 16 * ni + 4 * (lane >> 4);
-          const f32x4 u = load_limbs(A + small_at(pa, i, j), la);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) c[mi][ni][r] = fmaf(st.c[q], c[mi][ni][r], st.b[q] * u[r]) + (i == j + r ? st.a[q] : 0.f);
+          for (int r = 0; r < 4; ++r) c[mi][ni][r] = fmaf(st.c[q], c[mi][ni][r], st.b[q] * ldexpf(acc[mi][ni][r], st.gram[q]));  // C - a I; A before its limbs
         }
     }
     __syncthreads();
@@ -555,7 +560,14 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(Items a, Firsts t, Step 
       for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
         for (int ni = 0; ni < 2; ++ni) x[h][mi][ni] = zero;
-      if (b < tm * tn) small_block<KS>(A, pa, la, X, px, lx, b / tn * 32, b % tn * 32, mp, x[h]);
+      if (b < tm * tn) {
+        small_block<KS>(A, pa, la, X, px, lx, b / tn * 32, b % tn * 32, mp, x[h]);
+#pragma unroll
+        for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+          for (int ni = 0; ni < 2; ++ni)
+            x[h][mi][ni] += st.a[q] * load_limbs(X + small_at(px, b / tn * 32 + 16 * mi + (lane & 15), b % tn * 32 + 16 * ni + 4 * (lane >> 4)), lx);
+      }
     }
     if (q + 1 == st.n) break;
     __syncthreads();
@@ -612,8 +624,8 @@ bool follow(const float* coef, int steps, Bounds& o) {
     const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2], S = r * r;
     if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
     auto P = [&](double s) { return fabs(a + b * s + c * s * s); };
-    double top = fmax(P(0.), P(S));
-    if (c != 0. && -b / (2. * c) > 0. && -b / (2. * c) < S) top = fmax(top, P(-b / (2. * c)));
+    double top = fmax(fmax(P(0.), P(S)), fabs(b * S + c * S * S));  // of C with and without a I
+    if (c != 0. && -b / (2. * c) > 0. && -b / (2. * c) < S) top = fmax(fmax(top, P(-b / (2. * c))), fabs(b * b / (4. * c)));
     if (!(top < 1e9) || !(top > 1e-9)) return false;
     o.cb[k] = (int)ceil(log2(top));
     o.cs[k] = 14 - o.cb[k];
@@ -785,10 +797,10 @@ int run_group(Items& a, bool join, const Step& st, const float* coef, int steps,
     s.shift = bo.as[k] - 2 * bo.xs[k];
     if (rc == HOLD_OK) rc = launch<GRAM, false>(cl, s, st, a, stream);
   };
-  auto poly = [&](int k, uint16_t* o) {
+  auto poly = [&](int k, uint16_t* o, bool whole) {  // whole: with a I
     s.l = mm[0];
     s.o = o;
-    s.a = (float)ldexp((double)coef[3 * k], bo.cs[k]);
+    s.a = whole ? (float)ldexp((double)coef[3 * k], bo.cs[k]) : 0.f;
     s.b = (float)ldexp((double)coef[3 * k + 1], bo.cs[k] - bo.as[k]);
     s.c = (float)ldexp((double)coef[3 * k + 2], bo.cs[k] - 2 * bo.as[k]);
     if (rc == HOLD_OK) rc = launch<POLY, false>(cl, s, st, a, stream);
@@ -800,7 +812,8 @@ int run_group(Items& a, bool join, const Step& st, const float* coef, int steps,
     s.shift = shift;
     if (rc == HOLD_OK) rc = launch<PROD, false>(cl, s, st, a, stream);
   };
-  auto apply = [&](const uint16_t* c, int cs, int from, int to) {  // X of step `from` -> X before step `to`
+  auto apply = [&](const uint16_t* c, int cs, int from, int to, float own) {  // X of step `from` -> X before step `to`
+    s.a = own;
     s.l = c;
     s.x = x;
     s.y = y;
@@ -813,8 +826,8 @@ int run_group(Items& a, bool join, const Step& st, const float* coef, int steps,
   if (!join) {
     for (int k = 0; k < steps; ++k) {
       gram(k);
-      poly(k, mm[1]);
-      apply(mm[1], bo.cs[k], k, k + 1);
+      poly(k, mm[1], false);
+      apply(mm[1], bo.cs[k], k, k + 1, (float)ldexp((double)coef[3 * k], bo.cs[k]));
     }
   } else {
     const int groups = (steps + 2) / 3;
@@ -826,11 +839,11 @@ int run_group(Items& a, bool join, const Step& st, const float* coef, int steps,
       for (; k < end; ++k) {
         const uint16_t* c = C;
         if (k == first) {
-          poly(k, Q);
+          poly(k, Q, true);
           c = Q;
           qb = bo.cb[k];
         } else {
-          poly(k, C);
+          poly(k, C, true);
           qb += bo.cb[k];
           prod(C, Q, T, 14 - qb - bo.cs[k] - (14 - (qb - bo.cb[k])));
           uint16_t* z = Q;
@@ -843,7 +856,7 @@ int run_group(Items& a, bool join, const Step& st, const float* coef, int steps,
           prod(T, c, A, bo.as[k + 1] - ts - bo.cs[k]);
         }
       }
-      apply(Q, 14 - qb, first, end);
+      apply(Q, 14 - qb, first, end, 0.f);
     }
   }
   return rc == HOLD_OK ? ok() : rc;
