@@ -507,7 +507,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
 // keeps 64 columns of both weight matrices in LDS for its whole life, as fragments in the order of their reads, and its eight waves run
 // over rows without meeting again: a wave loads 16 MI whole rows as they are (128 bytes of a row at a time), finds their scales and splits
 // them in registers, multiplies, and stores.  One launch, x read once a panel, nothing written but the result.
-// 131072 x 256 -> 256 in fp32: packing and tiles 180 us, this @@ us; bound by @@.
+// 131072 x 256 -> 256 in fp32: packing and tiles 177 us, this 124: 278 TFLOP/s (three products a term) and
+// 2.2 TB/s, neither near its bound -- a wave's splits, products and activations take turns, and two waves share a SIMD.
 constexpr int PANEL = 64, SHORT_WAVES = 8;
 
 struct ShortArgs {
@@ -876,7 +877,7 @@ struct RowsArgs {
 };
 
 // T <= 4: dot products, a wave computes NC columns of both projections for all rows, its lanes along k (4 x 4096 -> 8192 in bf16, 134 MB of
-// weights: @@ us; one column a wave reads x as often as the weights and took 56)
+// weights: 26 us; one column a wave reads x as often as the weights and took 56)
 template <int MODE, int NT, int NC>
 __global__ __launch_bounds__(256) void gated_rows_kernel(RowsArgs a) {
   constexpr int N = chunk_k<MODE>();
@@ -1007,16 +1008,17 @@ inline int64_t rows_grid(int64_t rows) {
 }
 
 // Tiles of 256 rows, one block a compute unit, or of 128, two a unit: by the time of the launch in rounds over the 256 units.  The small
-// tiles' lower rate (1135 against 1310 TFLOP/s at 4096^3, more LDS reads and loads a product) counts little against a part-filled round;
-// and where the sum is short a block is mostly its epilogue, which two blocks a unit hide behind each other's products
-// (131072 x 256 -> 256 in fp32: @@ against @@ us).
-bool large_tiles(int64_t n256, int64_t n128, int64_t steps) {
-  if (steps <= 16) return false;
+// tiles' lower rate (1135 against 1310 TFLOP/s at 4096^3, more LDS reads and loads a product) counts little against a part-filled round.
+// Sums of 5 to 16 steps: 65536 x 384 -> 512 in fp32 200 against 219 us, 65536 x 1024 -> 2048 in bf16 493 against 574.
+bool large_tiles(int64_t n256, int64_t n128) {
   const double large = (double)((n256 + 255) / 256);
   double small = 0.58 * (double)((n128 + 511) / 512);
   if (n128 <= 512) small = 0.58 * (n128 <= 256 ? 0.68 : 1.);
   return large <= small;
 }
+// in the backward pass, whose epilogues are longer, two blocks a unit hide them behind each other's products where the sum is short
+// (65536 x 384 -> 512 in fp32, the whole step: 1117 against 1146 us)
+constexpr int64_t SHORT_SUM = 16;
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // where everything of one call lies in its workspace (bytes; every part starts on a multiple of 256)
@@ -1058,9 +1060,9 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
   parts = parts > rounds ? rounds : parts >= 8 ? (parts + 7) / 8 * 8 : parts;
   p.part_rows = cdiv(rounds, parts) * round;
   p.parts = cdiv(d.T, p.part_rows);
-  p.big = large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64), cdiv(p.Dp, step));
+  p.big = !(bwd && cdiv(p.Dp, step) <= SHORT_SUM) && large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64));
   // less than a block a unit of 128 x (64 + 64): tiles a quarter of that, four stages deep, their loads three steps ahead
-  // (2019 x 2816 -> 32 in fp32: @@ -> @@ us; 1237 x 517 -> 1021 in bf16: @@ -> @@)
+  // (2019 x 2816 -> 32 in fp32: 80.9 -> 57.0 us; 1000 x 2048 -> 512 in bf16: 24.4 -> 16.9)
   p.little = !p.big && cdiv(d.T, 128) * cdiv(d.H, 64) <= 64;
   p.row_tiles = p.brief ? p.parts * SHORT_WAVES : cdiv(d.T, p.big ? 256 : p.little ? 64 : 128);
   p.pack_blocks = rows_grid(d.T + 2 * (int64_t)d.H);
@@ -1082,10 +1084,10 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
     }
     if (d.db_gate || d.db_up) p.dbpart = take(p.row_tiles * 2 * d.H * 4);
     const int64_t x256 = cdiv(d.T, 256) * cdiv(d.D, 256), x128 = cdiv(d.T, 128) * cdiv(d.D, 128);
-    p.dx_big = x256 >= 200 && large_tiles(x256, x128, 2 * cdiv(p.Hp, step));
+    p.dx_big = x256 >= 200 && 2 * cdiv(p.Hp, step) > SHORT_SUM && large_tiles(x256, x128);
     split_sum(p.dx_big ? 512 : x128, p.Hp, 512, p.dx_splits, p.dx_chunk);
     const int64_t w256 = 2 * cdiv(d.H, 256) * cdiv(d.D, 256), w128 = 2 * cdiv(d.H, 128) * cdiv(d.D, 128);
-    p.dw_big = w256 >= 200 && large_tiles(w256, w128, cdiv(d.T, step));
+    p.dw_big = w256 >= 200 && cdiv(d.T, step) > SHORT_SUM && large_tiles(w256, w128);
     split_sum(p.dw_big ? 512 : w128, d.T, 512, p.dw_splits, p.dw_chunk);
     if (p.dx_splits > 1) p.dx_sums = take(p.dx_splits * d.T * d.D * 4);
     if (p.dw_splits > 1) p.dw_sums = take(p.dw_splits * 2 * (int64_t)d.H * d.D * 4);

@@ -9,9 +9,10 @@
 // WIDE MATRICES (n columns, m rows, n >= 1.5 m) spend most of a step on X's two products.  C is a polynomial of A, so A of the next step is
 // C A C, and k steps on X are one with Q = C_k .. C_1: of the steps' products k - 1 GRAMs and APPLYs turn into three symmetric m x m
 // products each (PROD), which for 5 steps of 1024 x 4096 in groups of 2 and 3 leaves 38 of 65 units of m^3.  Groups stay short because A's
-// rounding errors grow by a^2 = 12 a step where X's grow by a.  The result is 4 times less exact than step by step (9e-6 against 2.4e-6
-// of the norm, float32's own plain evaluation: 2.4e-6, at 736 x 1408): nothing to a weight's update or to a result in 16 bits, and done
-// for those only.
+// rounding errors grow by a^2 = 12 a step where X's grow by a.  For a spectrum as narrow as a random matrix's that costs nothing
+// (1024 x 2048: 2.6e-6 of the norm against 2.3e-6 step by step and 3.4e-6 for float32's plain evaluation), for one spread over two
+// decades 2.0e-5 against 2.1e-6, for rank 64 and noise 1.0e-4 against 1.5e-5: nothing to a weight's update or to a result in 16 bits,
+// and done for those only.
 //
 // ARITHMETIC.  Small singular values grow by a^steps (485 with the usual coefficients), and with them every rounding of X relative to
 // the largest one; bf16's 2^-9 would be the result there.  So X, A and C = a I + b A + c A A are kept as two fp16 limbs (tile16.h,
@@ -413,8 +414,8 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
 }
 
 // ---- small matrices: a block each, the whole iteration in LDS ----------------------------------------------------------------------------------
-// X and A as limbs in LDS; 16 waves take 32 x 32 blocks of each product, results wait in registers until everyone has read.  One launch instead of 2 + 3 a step, which for a 64 x 64
-// matrix are 66 us of launches; @@.
+// X and A as limbs in LDS; 16 waves take 32 x 32 blocks of each product, results wait in registers until everyone has read.  One launch
+// instead of 2 + 3 a step: a 64 x 64 matrix takes 25 us instead of 66, most of it the barriers between products of a few hundred cycles.
 constexpr int SMALL_STEPS = 8, SMALL_LDS = 160 * 1024 - 1024, SMALL_BLOCKS = 32;
 struct SmallSteps {
   float a[SMALL_STEPS], b[SMALL_STEPS], c[SMALL_STEPS];
@@ -654,7 +655,7 @@ inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 struct Room {
   int64_t part, x, y, mm[4], xn, cn, bytes;
 };
-// Whether an item's steps are joined: measured on 6 x 1024 x 4096 (1.77 -> 1.22 ms) and 3 x 1531 x 517 (294 -> 259 us); with less
+// Whether an item's steps are joined: measured on 6 x 1024 x 4096 (1.57 -> 1.05 ms) and 3 x 1531 x 517 (274 -> 249 us); with less
 // work launches are what counts, and a result in float32 keeps float32's exactness
 bool joined(const Item& it, bool exact) {
   if (exact) return false;
