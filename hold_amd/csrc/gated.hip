@@ -1100,9 +1100,11 @@ int check(const hold_gated_desc* d) {
   if (!d || !d->x || !d->w_gate || !d->w_up || d->T < 1 || d->D < 1 || d->H < 1 || d->act < 0 || d->act > 3) return HOLD_E_ARG;
   if (d->dtype != HOLD_GATED_F32 && d->dtype != HOLD_GATED_BF16) return HOLD_E_ARG;
   if (d->ldx < d->D || d->ldwg < d->D || d->ldwu < d->D) return HOLD_E_ARG;
-  // the tile loads' 32-bit offsets: 256 rows of an operand, 64 rows of dg, and the tile grids
+  // the tile loads' 32-bit offsets: 256 rows of an operand, 64 rows of dg
   if (d->ldx > (1 << 21) || d->ldwg > (1 << 21) || d->ldwu > (1 << 21) || d->H > (1 << 21) || d->T > (1ll << 31)) return HOLD_E_ARG;
-  if (((d->T + 127) / 128) * (((d->H > d->D ? d->H : d->D) + 63) / 64) > (1ll << 29)) return HOLD_E_ARG;
+  // a launch has less than 2^32 threads: 512 a tile of 128 x 64 of h or dx, or of 128 x 128 of both weights' gradients
+  if (((d->T + 127) / 128) * (((d->H > d->D ? d->H : d->D) + 63) / 64) >= (1ll << 23)) return HOLD_E_ARG;
+  if (((int64_t)d->H + 127) / 128 * (((int64_t)d->D + 127) / 128) >= (1ll << 22)) return HOLD_E_ARG;
   return HOLD_OK;
 }
 

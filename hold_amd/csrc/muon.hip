@@ -915,6 +915,12 @@ bool read_item(const hold_muon_desc* d, int k, Item& it) {
   it.gain = (float)(d->lr * i.scale);
   return true;
 }
+// a launch has less than 2^32 threads: a batch that would pass 2^21 blocks goes in parts, one after the other in the same workspace
+int32_t part_of(const Item& it, int way) {
+  if (way == SMALL) return 1 << 21;
+  const int64_t blocks = ((int64_t)it.rows + 71) / 64 * (((int64_t)it.cols + 71) / 64) + 512, n = (1 << 21) / blocks;
+  return n < 1 ? 1 : (int32_t)n;
+}
 // calls f(items, way) for the groups of a step, up to MAXI items that are computed alike; false: a bad item
 template <class F>
 bool groups_of(const hold_muon_desc* d, F f) {
@@ -943,6 +949,8 @@ extern "C" int hold_orthogonalize_workspace(const hold_ortho_desc* d, int64_t* b
   Classes cl;
   if (!one_item(d, a) || !bytes) return HOLD_E_ARG;
   const int way = way_of(a.it[0], d->dtype == HOLD_MUON_F32, d->steps);
+  const int32_t part = part_of(a.it[0], way);
+  if (a.it[0].count > part) a.it[0].count = part;
   *bytes = way == SMALL ? 256 : room(a, cl, way == JOIN).bytes;
   return HOLD_OK;
 }
@@ -952,14 +960,23 @@ extern "C" int hold_orthogonalize(const hold_ortho_desc* d, hold_stream_t stream
   int64_t need = 0;
   if (hold_orthogonalize_workspace(d, &need) != HOLD_OK || !d->workspace || need > d->workspace_bytes || !one_item(d, a)) return HOLD_E_ARG;
   if (!d->x || !d->out || !d->coef || d->steps < 1 || d->steps > 32 || d->dtype < 0 || d->dtype > 2 || !(d->eps >= 0.f)) return HOLD_E_ARG;
-  a.it[0].g = d->x;
-  a.it[0].p = d->out;
   Step st = {};
   st.eps = d->eps;
   st.dtype = d->dtype;
-  const int way = way_of(a.it[0], d->dtype == HOLD_MUON_F32, d->steps);
-  if (way == SMALL) return run_small(a, st, d->coef, d->steps, (hipStream_t)stream);
-  return run_group(a, way == JOIN, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+  const Item whole = a.it[0];
+  const int way = way_of(whole, d->dtype == HOLD_MUON_F32, d->steps);
+  const int64_t bytes = whole.stride * (d->dtype == HOLD_MUON_F32 ? 4 : 2);
+  const int32_t part = part_of(whole, way);
+  for (int32_t k = 0; k < d->batch; k += part) {
+    Item& it = a.it[0] = whole;
+    it.g = (const char*)d->x + k * bytes;
+    it.p = (char*)d->out + k * bytes;
+    it.count = d->batch - k < part ? d->batch - k : part;
+    const int rc = way == SMALL ? run_small(a, st, d->coef, d->steps, (hipStream_t)stream)
+                                : run_group(a, way == JOIN, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+    if (rc != HOLD_OK) return rc;
+  }
+  return HOLD_OK;
 }
 
 extern "C" int hold_muon_workspace(const hold_muon_desc* d, int64_t* bytes) {

@@ -22,6 +22,7 @@ from ._lib import GatedDesc, check, stream_ptr
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+MAX_WIDTH = 1 << 21
 
 
 def _rows(t):
@@ -109,15 +110,17 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """``act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)``: x [..., D], w_gate and w_up [H, D], biases [H] or None -> [..., H].
 
     All tensors on one GPU and of one type, float32 or bfloat16.  Differentiable once in every tensor.  Up to 64 rows go through a
-    kernel for few rows that reads the weights as they are, once; more through the matrix cores."""
+    kernel for few rows that reads the weights as they are, once; more through the tiled ones.  A captured training step takes its
+    gradients by ``torch.autograd.grad``, or by ``backward`` while no eager graph of the same leaves lives (autograd would
+    otherwise make the capture wait for the eager graph's stream)."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"gated_linear: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
     shape, dtype, device = w_gate.shape, x.dtype, x.device
     if x.dim() < 1 or len(shape) != 2 or w_up.shape != shape or x.shape[-1] != shape[1]:
         raise ValueError(f"gated_linear: x [..., D] and two weights [H, D] are wanted, got {tuple(x.shape)}, {tuple(shape)}, {tuple(w_up.shape)}")
-    if shape[1] == 0:
-        raise ValueError("gated_linear: at least one input feature is wanted")
+    if shape[1] == 0 or max(shape) > MAX_WIDTH:
+        raise ValueError(f"gated_linear: 1 to {MAX_WIDTH} input features and at most as many results are taken, got weights of {tuple(shape)}")
     tensors = [x, w_gate, w_up]
     for name, b in (("b_gate", b_gate), ("b_up", b_up)):
         if b is not None:

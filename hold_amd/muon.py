@@ -21,7 +21,7 @@ from ._lib import MuonDesc, MuonItem, OrthoDesc, check, ptr, stream_ptr
 #: (a, b, c) of  s -> a s + b s^3 + c s^5
 QUINTIC = (3.4445, -4.7750, 2.0315)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-MAX_STEPS, MAX_DIM = 32, 1 << 20
+MAX_STEPS, MAX_DIM, MAX_BATCH = 32, 1 << 20, 1 << 24
 
 
 def _coefficients(coefficients, steps, what):
@@ -43,8 +43,8 @@ def _eps(eps, what):
 
 
 def _diverges(what):
-    return ValueError(f"{what}: a size or the coefficients are out of range (the bound on the largest singular value has to stay "
-                      "between 1e-9 and 1e9 through the steps)")
+    return ValueError(f"{what}: the coefficients are out of range (the bound on the largest singular value has to stay between 1e-9 and "
+                      "1e9 through the steps)")
 
 
 @torch.no_grad()
@@ -61,6 +61,10 @@ def orthogonalize(x, steps=5, coefficients=QUINTIC, eps=1e-7):
     if x.dtype not in _DTYPES:
         raise TypeError(f"{what}: float32, bfloat16 or float16 is wanted, got {x.dtype}")
     eps = _eps(eps, what)
+    rows, cols = x.shape[-2:]
+    batch = x.numel() // max(rows * cols, 1)
+    if rows > MAX_DIM or cols > MAX_DIM or batch > MAX_BATCH:
+        raise ValueError(f"{what}: at most {MAX_BATCH} matrices of at most {MAX_DIM} on a side are taken, got shape {tuple(x.shape)}")
     if not x.is_cuda:
         raise ValueError(f"{what}: the tensor has to be on a GPU, got {x.device}")
     x = x.detach().contiguous()
@@ -69,8 +73,7 @@ def orthogonalize(x, steps=5, coefficients=QUINTIC, eps=1e-7):
         return out
     d = OrthoDesc()
     d.x, d.out, d.coef = ptr(x), ptr(out), C.cast(coef, C.POINTER(C.c_float))
-    d.rows, d.cols = x.shape[-2:]
-    d.batch = x.numel() // (d.rows * d.cols)
+    d.rows, d.cols, d.batch = rows, cols, batch
     d.dtype, d.steps, d.eps = _DTYPES[x.dtype], steps, eps
     L, n = _lib.lib(), C.c_int64()
     with torch.cuda.device(x.device):

@@ -24,6 +24,7 @@ def _t(*shape, dtype=torch.float32):
     (dict(b_gate=_t(8, dtype=torch.bfloat16)), TypeError),
     (dict(x=_t(3, 4, dtype=torch.float64), w_gate=_t(8, 4, dtype=torch.float64), w_up=_t(8, 4, dtype=torch.float64)), TypeError),
     (dict(x=_t(3, 4, dtype=torch.float16), w_gate=_t(8, 4, dtype=torch.float16), w_up=_t(8, 4, dtype=torch.float16)), TypeError),
+    (dict(w_gate=_t(1, 4).expand((1 << 21) + 1, 4), w_up=_t(1, 4).expand((1 << 21) + 1, 4)), ValueError),
     (dict(), ValueError),                                   # on the CPU: there is no fallback
 ])
 def test_gated_linear_refuses(kw, error):
@@ -53,19 +54,21 @@ def test_entry_points_refuse_bad_descriptors():
     assert L.hold_gated_workspace(C.byref(_desc()), 1, C.byref(n)) == 0 and n.value > 0
     need = n.value
     for bad in (dict(T=0), dict(T=-1), dict(D=0), dict(H=0), dict(dtype=2), dict(act=4), dict(act=-1), dict(x=0), dict(w_gate=0), dict(w_up=0),
-                dict(ldx=63), dict(ldwg=63), dict(ldwu=63), dict(ldx=(1 << 21) + 1), dict(H=(1 << 21) + 1), dict(T=(1 << 31) + 1)):
+                dict(ldx=63), dict(ldwg=63), dict(ldwu=63), dict(ldx=(1 << 21) + 1), dict(H=(1 << 21) + 1), dict(T=(1 << 31) + 1),
+                dict(T=1 << 30), dict(H=1 << 20, D=1 << 20, ldx=1 << 20, ldwg=1 << 20, ldwu=1 << 20)):
         assert L.hold_gated_workspace(C.byref(_desc(**bad)), 1, C.byref(n)) == -1, bad
         assert L.hold_gated_fwd(C.byref(_desc(**{"h": 4096, "ldh": 1 << 22, **bad})), None) == -1, bad
     assert L.hold_gated_workspace(C.byref(_desc()), 1, None) == -1
     assert L.hold_gated_fwd(C.byref(_desc(workspace=4096, workspace_bytes=1 << 40)), None) == -1                  # no result
     assert L.hold_gated_fwd(C.byref(_desc(h=4096, ldh=47, workspace=4096, workspace_bytes=1 << 40)), None) == -1  # rows overlap
-    assert L.hold_gated_fwd(C.byref(_desc(h=4096, ldh=48)), None) == -1                                           # no workspace
+    assert L.hold_gated_fwd(C.byref(_desc(h=4096, ldh=48, D=300)), None) == -1                                    # no workspace
     full = dict(dh=4096, lddh=48, dx=4096, dw_gate=4096, dw_up=4096)
     assert L.hold_gated_bwd(C.byref(_desc(**{**full, "dh": 0}, workspace=4096, workspace_bytes=1 << 40)), None) == -1
     assert L.hold_gated_bwd(C.byref(_desc(**{**full, "dw_up": 0}, workspace=4096, workspace_bytes=1 << 40)), None) == -1
     assert L.hold_gated_bwd(C.byref(_desc(**full, workspace=4096, workspace_bytes=need - 1)), None) == -1
     for out in ("dx", "dw_gate", "dw_up"):  # not on a 16-byte boundary
         assert L.hold_gated_bwd(C.byref(_desc(**{**full, out: 4100}, workspace=4096, workspace_bytes=1 << 40)), None) == -1
-    # few rows need no scratch forward; the sizes grow with the rows
-    assert L.hold_gated_workspace(C.byref(_desc(T=64)), 0, C.byref(n)) == 0 and n.value == 0
-    assert L.hold_gated_workspace(C.byref(_desc(T=65)), 0, C.byref(n)) == 0 and n.value >= 65 * 64 * 4
+    # few rows and short ones need no scratch forward; the sizes grow with the rows
+    assert L.hold_gated_workspace(C.byref(_desc()), 0, C.byref(n)) == 0 and n.value == 0
+    assert L.hold_gated_workspace(C.byref(_desc(T=64, D=300)), 0, C.byref(n)) == 0 and n.value == 0
+    assert L.hold_gated_workspace(C.byref(_desc(T=65, D=300)), 0, C.byref(n)) == 0 and n.value >= 65 * 300 * 4

@@ -30,9 +30,9 @@ def act64(g, act):
     return s if act == "sigmoid" else g * s
 
 
-def reference(x, wg, wu, bg, bu, act, dh=None):
+def reference(x, wg, wu, bg, bu, act, dh=None, at="cpu"):
     """(h, its bound), [(gradient, its bound) or None]"""
-    t = [None if v is None else v.detach().cpu().double() for v in (x, wg, wu, bg, bu)]
+    t = [None if v is None else v.detach().to(at).double() for v in (x, wg, wu, bg, bu)]
     low = x.dtype == torch.bfloat16
     d, r, q = 2.0 ** -18, 2.0 ** -8 if low else 2.0 ** -24, 2.0 ** -8 if low else 2.0 ** -22
     x_, wg_, wu_ = t[:3]
@@ -51,7 +51,7 @@ def reference(x, wg, wu, bg, bu, act, dh=None):
     eh = (ada + kink) * eg * u.abs() + a.abs() * eu + (1 + ada + kink) * eg * eu + (d + r) * h.abs()
     if dh is None:
         return (h, eh), None
-    dh = dh.detach().cpu().double()
+    dh = dh.detach().to(at).double()
     dg, du = dh * u * da, dh * a
     fg = dh.abs() * (ada * eu + u.abs() * ((0 if act == "relu" else 1) * eg + kink) + kink * eu) + d * dg.abs()
     fu = dh.abs() * (ada + kink) * eg + d * du.abs()
@@ -70,14 +70,16 @@ def make(T, D, H, dtype, bias, seed=0):
 
 
 def close(got, want, what=""):
-    a, (b, bound) = got.detach().cpu().double(), want
+    b, bound = want
+    a = got.detach().to(b.device).double()
     assert a.shape == b.shape and bool(torch.isfinite(a).all()), what
     over = (a - b).abs() - bound * (1 + 1e-6)
     assert not bool((over > 0).any()), (what, float(over.max()), float(((a - b).abs() / bound.clamp(min=1e-300)).max()))
 
 
-SIZES = [(128, 264, 40), (100, 300, 24), (1, 1, 1), (1, 256, 256), (3, 7, 5), (4, 129, 66), (16, 64, 200), (17, 33, 9), (64, 260, 31), (65, 8, 8), (65, 40, 72), (127, 64, 64),
-         (129, 65, 63), (130, 256, 256), (300, 136, 520), (257, 31, 1), (200, 1, 130), (1000, 72, 24)]
+SIZES = [(1, 1, 1), (1, 256, 256), (3, 7, 5), (4, 129, 66), (16, 64, 200), (17, 33, 9), (64, 260, 31), (65, 8, 8), (65, 40, 72), (127, 64, 64),
+         (129, 65, 63), (130, 256, 256), (300, 136, 520), (257, 31, 1), (200, 1, 130), (1000, 72, 24), (100, 300, 24), (128, 264, 40),
+         (700, 257, 1500)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -98,14 +100,28 @@ def test_matches_the_formula(T, D, H, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_large_tiles_and_split_sums(dtype):
-    """the 256-row tiles (256 of them and more), sums over tokens split between blocks, a ragged end in every direction"""
+def test_many_short_rows_and_split_sums(dtype):
+    """rows of up to 256 elements through many blocks, sums over tokens split between blocks, a ragged end in every direction"""
     from hold_amd.gated import gated_linear
     for T, D, H, act in ((33000, 72, 257, "silu"), (8321, 200, 1032, "gelu")):
         args, dh = make(T, D, H, dtype, bias=True)
         leaves = [v.requires_grad_(True) for v in args]
         h = gated_linear(*leaves, activation=act)
         want, grads = reference(*args, act, dh)
+        close(h, want, "h")
+        for name, a, w in zip("x w_gate w_up b_gate b_up".split(), torch.autograd.grad(h, leaves, dh), grads):
+            close(a, w, name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_tiles(dtype):
+    """the tiles of 256 rows of every product with ragged ends: h (short and long sums), dg and du, dx, and the weights' gradients"""
+    from hold_amd.gated import gated_linear
+    for T, D, H, act in ((32700, 263, 380, "relu"), (16300, 1020, 1019, "silu"), (2000, 2563, 2570, "gelu")):
+        args, dh = make(T, D, H, dtype, bias=D == 1020)
+        leaves = [v.requires_grad_(True) for v in args if v is not None]
+        h = gated_linear(*leaves, activation=act)
+        want, grads = reference(*args, act, dh, at=DEV)
         close(h, want, "h")
         for name, a, w in zip("x w_gate w_up b_gate b_up".split(), torch.autograd.grad(h, leaves, dh), grads):
             close(a, w, name)

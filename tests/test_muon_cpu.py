@@ -19,6 +19,8 @@ from parity_common import ROOT  # noqa: F401
     (torch.zeros(4, 4), dict(steps=2, coefficients=[(1.0, 2.0, 3.0), (1.0, 2.0)]), ValueError),
     (torch.zeros(4, 4), dict(eps=-1.0), ValueError),
     (torch.zeros(4, 4), dict(eps=float("nan")), ValueError),
+    (torch.zeros(1, 1).expand(2, (1 << 20) + 1), {}, ValueError),
+    (torch.zeros(1, 1, 1).expand((1 << 24) + 1, 1, 1), {}, ValueError),
     (torch.zeros(4, 4), {}, ValueError),  # on the CPU: there is no fallback
 ])
 def test_orthogonalize_refuses(x, kw, error):

@@ -179,6 +179,16 @@ def test_views_empty_and_batches():
         assert orthogonalize(torch.zeros(shape, device=DEV)).shape == shape
 
 
+def test_batches_in_parts():
+    """more matrices than one launch takes: every one as alone, in the kernel for small ones and (nine steps) in the other"""
+    from hold_amd.muon import orthogonalize
+    for n, steps in (((1 << 21) + 3, 5), (9001, 9)):
+        x = make(n, 3, 2)
+        y = orthogonalize(x, steps=steps)
+        for at in (slice(0, 5), slice(4085, 4095), slice(8170, 8180), slice(n - 5, n)):
+            assert torch.equal(y[at], orthogonalize(x[at], steps=steps))
+
+
 def step64(p, g, m, lr, momentum, nesterov, wd, scale, f=1.0):
     p, g, m = (t.detach().cpu().double() for t in (p, g, m))
     m = momentum * m + (1 - momentum) * f * g
