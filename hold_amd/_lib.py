@@ -109,7 +109,7 @@ class GatedDesc(C.Structure):  # hold_gated_desc
                 ("ldwu", C.c_int64), ("b_gate", C.c_void_p), ("b_up", C.c_void_p), ("h", C.c_void_p), ("ldh", C.c_int64),
                 ("dh", C.c_void_p), ("lddh", C.c_int64), ("dx", C.c_void_p), ("dw_gate", C.c_void_p), ("dw_up", C.c_void_p),
                 ("db_gate", C.c_void_p), ("db_up", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
-                ("T", C.c_int64), ("D", C.c_int32), ("H", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32)]
+                ("T", C.c_int64), ("D", C.c_int32), ("H", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32), ("kept", C.c_void_p)]
 
 
 class OrthoDesc(C.Structure):  # hold_ortho_desc
@@ -212,6 +212,7 @@ SIGNATURES = {
     "hold_fused_sdf_r6_if": [_P, _I, _L, _P, _P, _P, _P, _P, _P, _I, _P, _P],
     "hold_trunk_r6_if": [_P, _I, _L, _P, _P, _P, C.POINTER(C.c_void_p), _I, _P, _P],
     "hold_gated_workspace": [C.POINTER(GatedDesc), _I, C.POINTER(_L)],  # host only: no stream
+    "hold_gated_kept": [C.POINTER(GatedDesc), C.POINTER(_L)],  # host only: no stream
     "hold_gated_fwd": [C.POINTER(GatedDesc), _P],
     "hold_gated_bwd": [C.POINTER(GatedDesc), _P],
     "hold_orthogonalize_workspace": [C.POINTER(OrthoDesc), C.POINTER(_L)],  # host only: no stream

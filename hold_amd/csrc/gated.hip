@@ -1,12 +1,15 @@
 // The gated layer  h = act(x Wg^T + bg) * (x Wu^T + bu)  in one kernel, and its backward pass.
 //
-//   dg = dh * u * act'(g)      du = dh * act(g)      (g, u: the two projections, computed again instead of kept: 4 T D H operations
-//   dx = dg Wg + du Wu         dWg = dg^T x          against 16 T H bytes written and read, less time up to D ~ 600 and no memory)
+//   dg = dh * u * act'(g)      du = dh * act(g)      (g, u: the two projections)
+//   dx = dg Wg + du Wu         dWg = dg^T x
 //   dWu = du^T x               dbg = sum_t dg, dbu = sum_t du
+//
+// u act'(g) and act(g) are kept from the forward pass where that is less time, and computed again, 4 T D H operations, where D is
+// short or the rows are few (`keeps` has the measurements).
 //
 // KERNELS.  gated_mma_kernel: both projections of a tile share the x tile in LDS, the epilogue applies bias, activation and product
 // (forward) or forms dg, du from dh and the recomputed g, u (backward), with the column sums for the bias gradients from the
-// unrounded values.  gated_dx_kernel: [dg | du] times [Wg; Wu] as one sum.  gated_dw_kernel: both weight gradients, the sum over
+// unrounded values.  gated_short_kernel: the same for D <= 256.  gated_kept_kernel: dg, du from what was kept.  gated_dx_kernel: [dg | du] times [Wg; Wu] as one sum.  gated_dw_kernel: both weight gradients, the sum over
 // tokens split over blocks into fp32 partial tiles that gated_finish_kernel adds in a fixed order.  gated_rows_kernel: T <= 64 rows.
 //
 // ROUNDINGS.  bf16: dg and du are rounded to bf16 once, as the operands of the next matrix instructions; everything before is fp32.
@@ -322,9 +325,15 @@ __global__ __launch_bounds__(256) void gated_pack_kernel(PackArgs a) {
 __global__ __launch_bounds__(256) void gated_pack_tokens_kernel(const float* x, int64_t ld, int64_t T, int D, int Dp, const int* rscale,
                                                                 const int* part, int nparts, uint16_t* out, int64_t limb, int* exps) {
   const int lane = threadIdx.x & 63;
+  __shared__ int tops[4];
   int top = NONE;
-  for (int i = lane; i < nparts; i += 64) top = part[i] > top ? part[i] : top;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < nparts; i += 256) top = part[i] > top ? part[i] : top;
   top = wave_max<64>(top);
+  if (lane == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = tops[i] > top ? tops[i] : top;
   const int R = top == NONE ? 0 : 15 - top;
   if (blockIdx.x == 0 && threadIdx.x == 0) exps[4] = R;
   for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < T; r += (int64_t)gridDim.x * 4) {
@@ -368,9 +377,32 @@ struct MmaArgs {
   const int* rscale;
   float* dbpart;                                 // [row tiles][2][H] column sums, or null
   int tm, tn;
+  void* kept;                                    // forward: [T][Hp / 4] times p and s of four columns
 };
 
-template <int MODE, bool BWD, int BM, int BN, int WM, int WN, bool PHASED, int S = 2>
+// What the forward pass leaves for the backward one, for four columns side by side: p = u act'(g) and s = act(g).  fp32: as they are, 32
+// bytes.  bf16: 24 bits of each, as four upper halves of p, of s and four pairs of their third bytes (p's below), 24 bytes: cut off,
+// not rounded, an error below 2^-15 of the value before dg and du are rounded to 2^-8.
+__device__ __forceinline__ void cut(f32x4 p, f32x4 s, u32x2 (&w)[3]) {
+  uint32_t a[4], b[4], v[6];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const float x = p[r], y = s[r];
+    a[r] = __builtin_bit_cast(uint32_t, x);
+    b[r] = __builtin_bit_cast(uint32_t, y);
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const uint32_t l0 = (a[2 * r] >> 8 & 0xff) | (b[2 * r] & 0xff00), l1 = (a[2 * r + 1] >> 8 & 0xff) | (b[2 * r + 1] & 0xff00);
+    v[r] = a[2 * r] >> 16 | (a[2 * r + 1] & 0xffff0000u);
+    v[2 + r] = b[2 * r] >> 16 | (b[2 * r + 1] & 0xffff0000u);
+    v[4 + r] = l0 | l1 << 16;
+  }
+#pragma unroll
+  for (int r = 0; r < 3; ++r) w[r] = u32x2{v[2 * r], v[2 * r + 1]};
+}
+
+template <int MODE, bool BWD, int BM, int BN, int WM, int WN, bool PHASED, int S = 2, bool KEEP = false>
 __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
   using Cr = Core<MODE, KC, KC, BM, BN, 2, WM, WN, S>;
   __shared__ __align__(1024) char smem[Cr::LDS];
@@ -399,6 +431,19 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
         dhs[BWD ? ni : 0][BWD ? mi : 0] = i < a.T && n > 0 ? load4<MODE>(a.dh, i * a.lddh + j, n) : f32x4{0.f, 0.f, 0.f, 0.f};
       }
   }
+  // Where much is kept the tiles of 256 rows, alone on their unit, send bf16's p and s or fp32's h (fp32's p and s are whole lines as they
+  // are) through LDS, half of each wave's rows at a time, so that whole lines leave: 16384 x 2048 -> 8192 in bf16 1300 -> 1064 us
+  // (916 with nothing kept), 16384 x 768 -> 4096 in fp32 690 -> 632 (538).  h alone is as fast from the registers.  16-byte chunks of a
+  // row are exchanged by its place among 16, which spreads a column's writes over the banks
+  constexpr bool STAGED = PHASED && KEEP;
+  constexpr bool CUT = KEEP && MODE == MODE_BF16, STAGED_H = STAGED && !CUT;
+  constexpr int ES = MODE == MODE_BF16 ? 2 : 4, HB = STAGED_H ? BN * ES : 0, PITCH = HB + (CUT ? BN * 6 : 0);
+  constexpr int PARTS = STAGED ? 2 : 1, MH = Cr::MI / PARTS, ROWS = WM * MH * 16;
+  static_assert(!STAGED || (ROWS * PITCH <= Cr::LDS && PITCH % 256 == 0), "the rows of a part fit");
+  auto place = [&](int row, int byte) { return smem + row * PITCH + (byte ^ (row & 15) << 4); };
+#pragma unroll
+  for (int part = 0; part < PARTS; ++part) {
+  if (STAGED) __syncthreads();
 #pragma unroll
   for (int ni = 0; ni < Cr::NI; ++ni) {
     const int jt = wn * (BN / WN) + 16 * ni + 4 * (lane >> 4), j = n0 + jt, n = a.H - j;
@@ -415,7 +460,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
     }
     f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int mi = 0; mi < Cr::MI; ++mi) {
+    for (int mi = part * MH; mi < (part + 1) * MH; ++mi) {
       const int64_t i = m0 + wm * (BM / WM) + 16 * mi + (lane & 15);
       const bool row = i < a.T;
       f32x4 g = acc[0][mi][ni], u = acc[1][mi][ni];
@@ -430,14 +475,29 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
       g += bg;
       u += bu;
       if (!BWD) {
-        f32x4 h;
+        f32x4 h, p, z;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float s, d;
-          activate<false, MODE == MODE_F16X3>(a.act, g[r], s, d);
+          activate<KEEP, MODE == MODE_F16X3>(a.act, g[r], s, d);
           h[r] = s * u[r];
+          if (KEEP) { p[r] = d * u[r]; z[r] = s; }
         }
-        if (row && n > 0) store4<MODE>(a.h, i * a.ldh + j, n, h);
+        if (row && n > 0) {
+          const int q = wm * MH * 16 + 16 * (mi - part * MH) + (lane & 15);
+          if (STAGED_H) store4<MODE>(place(q, jt * ES), 0, 4, h);
+          else store4<MODE>(a.h, i * a.ldh + j, n, h);
+          if constexpr (CUT) {
+            u32x2 w[3];
+            cut(p, z, w);
+#pragma unroll
+            for (int r = 0; r < 3; ++r) *(u32x2*)(STAGED ? place(q, HB + jt * 6 + 8 * r) : (char*)a.kept + (i * a.Hp + j) * 6 + 8 * r) = w[r];
+          } else if constexpr (KEEP) {
+            float* o = (float*)a.kept + (i * a.Hp + j) * 2;
+            *(f32x4*)o = p;
+            *(f32x4*)(o + 4) = z;
+          }
+        }
       } else {
         f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = dg;
         if (row && n > 0) {
@@ -488,6 +548,33 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
       }
     }
   }
+  if (STAGED) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < ROWS * PITCH / 16; e += 64 * WM * WN) {
+      const int q = e / (PITCH / 16), c = e % (PITCH / 16) * 16;
+      const int64_t i = m0 + q / (MH * 16) * (BM / WM) + part * MH * 16 + q % (MH * 16);
+      if (i >= a.T) continue;
+      const u32x4 w = *(const u32x4*)place(q, c);
+      if (c >= HB) {
+        if (n0 * 6 + c - HB < a.Hp * 6) *(u32x4*)((char*)a.kept + (i * a.Hp + n0) * 6 + c - HB) = w;
+      } else {
+        const int j = n0 + c / ES;
+        char* o = (char*)a.h + (i * a.ldh + j) * ES;
+        if (a.H - j >= 16 / ES) {
+          __builtin_memcpy(o, &w, 16);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16 / ES; ++r) {
+            const uint32_t v = w[r * ES / 4];
+            if (j + r >= a.H) continue;
+            if (ES == 4) ((uint32_t*)o)[r] = v;
+            else ((uint16_t*)o)[r] = (uint16_t)(v >> 16 * (r & 1));
+          }
+        }
+      }
+    }
+  }
+  }
   if (BWD && a.dbpart) {
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * BN; c += Cr::THREADS) {
@@ -502,6 +589,107 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
   }
 }
 
+// ---- dg and du from what was kept --------------------------------------------------------------------------------------------------------
+// Bound by its bytes: 12 a value in bf16, 20 in fp32.  A lane takes eight columns, a wave 512 of a row, a block 64 rows; four rows are
+// requested before the first is used.
+constexpr int KEPT_ROWS = 64;
+struct KeptArgs {
+  const void* kept; const void* dh; int64_t lddh;
+  int64_t T; int H; int64_t Hp;
+  uint16_t* dg; uint16_t* du; int64_t dlimb;
+  const int* rscale; const int* exps;
+  float* dbpart;
+  int cols;  // blocks side by side
+};
+template <int MODE>
+__global__ __launch_bounds__(256) void gated_kept_kernel(KeptArgs a) {
+  constexpr int W = MODE == MODE_BF16 ? 3 : 4, U = 4;  // 16-byte words of eight columns; rows in flight
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), tile = blockIdx.x / a.cols, j = (blockIdx.x % a.cols * 64 + lane) * 8;
+  const int64_t i0 = (int64_t)tile * KEPT_ROWS + wave;
+  const int n = a.H - j;
+  const int shift = MODE == MODE_F16X3 ? a.exps[6] - a.exps[5] : 0;
+  __shared__ __align__(16) float sums[2][4][512];
+  float sg[8], su[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) sg[r] = su[r] = 0.f;
+  if (n > 0)  // Hp ends less than eight columns behind H
+    for (int q = 0; q < KEPT_ROWS / 4; q += U) {
+      u32x4 w[U][W];
+      f32x4 dh[U][2];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int64_t i = i0 + 4 * (q + k);
+        if (i >= a.T) continue;
+        const u32x4* src = (const u32x4*)((const char*)a.kept + (i * a.Hp + j) * (MODE == MODE_BF16 ? 6 : 8));
+#pragma unroll
+        for (int v = 0; v < W; ++v) w[k][v] = src[v];
+        dh[k][0] = load4<MODE>(a.dh, i * a.lddh + j, n);
+        dh[k][1] = load4<MODE>(a.dh, i * a.lddh + j + 4, n - 4);
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int64_t i = i0 + 4 * (q + k);
+        if (i >= a.T) continue;
+        float dg[8], du[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          float p, s;
+          if constexpr (MODE == MODE_BF16) {
+            const int at = r / 4 * 6 + r % 4 / 2, sh = 16 * (r & 1);
+            const uint32_t l = w[k][(at + 4) / 4][(at + 4) % 4] >> sh;
+            p = __builtin_bit_cast(float, (w[k][at / 4][at % 4] >> sh) << 16 | (l & 0xff) << 8);
+            s = __builtin_bit_cast(float, (w[k][(at + 2) / 4][(at + 2) % 4] >> sh) << 16 | (l & 0xff00));
+          } else {
+            const uint32_t x = w[k][r / 4 * 2][r % 4], y = w[k][r / 4 * 2 + 1][r % 4];
+            p = __builtin_bit_cast(float, x);
+            s = __builtin_bit_cast(float, y);
+          }
+          const float t = dh[k][r / 4][r % 4];
+          dg[r] = r < n ? t * p : 0.f;  // the columns behind H are zeros
+          du[r] = r < n ? t * s : 0.f;
+          sg[r] += dg[r];
+          su[r] += du[r];
+        }
+        const int64_t o = i * a.Hp + j;
+        auto put = [&](uint16_t* to, const uint16_t (&v)[8]) {
+          *(u32x4*)(to + o) = u32x4{v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16};
+        };
+        uint16_t g0[8], u0[8], g1[8], u1[8];
+        const int e = MODE == MODE_F16X3 ? a.rscale[i] : 0, eg = e == NONE ? 0 : e, eu = e == NONE ? 0 : e + shift;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          if constexpr (MODE == MODE_BF16) {
+            g0[r] = bf16_bits(dg[r]);
+            u0[r] = bf16_bits(du[r]);
+          } else {
+            const Split x = split16(ldexpf(dg[r], eg)), y = split16(ldexpf(du[r], eu));
+            g0[r] = x.hi; g1[r] = x.lo; u0[r] = y.hi; u1[r] = y.lo;
+          }
+        }
+        put(a.dg, g0);
+        put(a.du, u0);
+        if constexpr (MODE != MODE_BF16) {
+          put(a.dg + a.dlimb, g1);
+          put(a.du + a.dlimb, u1);
+        }
+      }
+    }
+  if (a.dbpart) {  // the four waves' rows
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      sums[0][wave][lane * 8 + r] = sg[r];
+      sums[1][wave][lane * 8 + r] = su[r];
+    }
+    __syncthreads();
+    const int first = blockIdx.x % a.cols * 512;
+    for (int c = threadIdx.x; c < 1024; c += 256) {
+      const int t = c >> 9, col = c & 511;
+      if (first + col < a.H)
+        a.dbpart[((int64_t)tile * 2 + t) * a.H + first + col] = sums[t][0][col] + sums[t][1][col] + (sums[t][2][col] + sums[t][3][col]);
+    }
+  }
+}
+
 // ---- short rows: D <= 256 ------------------------------------------------------------------------------------------------------------------
 // With a sum this short a tile is mostly its start and its end, and the limbs' way through memory costs as much as the layer.  So: a block
 // keeps 64 columns of both weight matrices in LDS for its whole life, as fragments in the order of their reads, and its eight waves run
@@ -509,7 +697,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
 // them in registers, multiplies, and stores.  One launch, x read once a panel, nothing written but the result.
 // 131072 x 256 -> 256 in fp32: packing and tiles 177 us, this 124: 278 TFLOP/s (three products a term) and
 // 2.2 TB/s, neither near its bound -- a wave's splits, products and activations take turns, and two waves share a SIMD.
-constexpr int PANEL = 64, SHORT_WAVES = 8;
+constexpr int PANEL = 64, SHORT_WAVES = 8, SHORT_ROW = 256;
 
 struct ShortArgs {
   const void* x; int64_t ldx;
@@ -1002,9 +1190,9 @@ __global__ __launch_bounds__(256) void gated_few_kernel(RowsArgs a) {
 
 inline int ok() { return hipGetLastError() == hipSuccess ? HOLD_OK : HOLD_E_LAUNCH; }
 inline int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
-inline int64_t rows_grid(int64_t rows) {
+inline int64_t rows_grid(int64_t rows, int64_t most = 2048) {  // a row a wave; eight blocks a unit
   const int64_t b = (rows + 3) / 4;
-  return b < 1 ? 1 : (b > 4096 ? 4096 : b);
+  return b < 1 ? 1 : (b > most ? most : b);
 }
 
 // Tiles of 256 rows, one block a compute unit, or of 128, two a unit: by the time of the launch in rounds over the 256 units.  The small
@@ -1016,15 +1204,14 @@ bool large_tiles(int64_t n256, int64_t n128) {
   if (n128 <= 512) small = 0.58 * (n128 <= 256 ? 0.68 : 1.);
   return large <= small;
 }
-// in the backward pass, whose epilogues are longer, two blocks a unit hide them behind each other's products where the sum is short
-// (65536 x 384 -> 512 in fp32, the whole step: 1117 against 1146 us)
+// in the products with dg and du, two blocks a unit hide their ends behind each other's products where the sum is short
 constexpr int64_t SHORT_SUM = 16;
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // where everything of one call lies in its workspace (bytes; every part starts on a multiple of 256)
 struct Plan {
   bool copy_x, copy_w[2];
-  bool brief, big, little, dx_big, dw_big;  // brief: the kernel for short rows; big, little: tiles of 256 and of 64 rows
+  bool brief, big, little, keep, dx_big, dw_big;  // brief: the kernel for short rows; big, little: tiles of 256 and of 64 rows
   int64_t parts, part_rows;
   int64_t Dp, Hp, row_tiles, pack_blocks;
   int64_t dx_splits, dx_chunk, dw_splits, dw_chunk;
@@ -1042,6 +1229,15 @@ void split_sum(int64_t tiles, int64_t K, int64_t least, int64_t& splits, int64_t
   splits = cdiv(K, chunk);
 }
 
+// Whether the forward pass keeps u act'(g) and act(g) where a backward one may follow.  Whole steps, kept against computed again: fp32
+// 16384 x 768 -> 4096 2.35 against 3.0 ms, 65536 x 264 -> 512 0.94 against 1.03, in the kernel for short rows no less; bf16 16384 x
+// 2048 -> 8192 3.46 against 4.16 ms, 65536 x 640 -> 512 556 against 590 us, x 512 431 against 427; with less than some 2^21 values a step
+// is its launches (700 x 1024 -> 1024 in fp32: 165 against 161 us).  16384 x 8192 values are 0.8 GB in bf16, 1.1 in fp32
+bool keeps(const hold_gated_desc& d) {
+  return d.T > ROWS_MAX && d.T * d.H >= (1 << 21) && d.D > (d.dtype == HOLD_GATED_F32 ? SHORT_ROW : 512);
+}
+int64_t kept_bytes(const hold_gated_desc& d) { return d.T * up(d.H, 8) * (d.dtype == HOLD_GATED_F32 ? 8 : 6); }
+
 Plan plan(const hold_gated_desc& d, bool bwd) {
   Plan p = {};
   const bool f32 = d.dtype == HOLD_GATED_F32;
@@ -1053,21 +1249,23 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
   p.copy_w[1] = f32 || d.D % 8 || !aligned16(d.w_up, d.ldwu, 2);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o += up(bytes, 256); return at; };
-  p.brief = d.D <= 256;
+  p.brief = d.D <= SHORT_ROW;
   // some 256 blocks; a part's rows are whole rounds of its waves, and all panels of a part go to one XCD where the parts divide
   const int64_t panels = cdiv(d.H, PANEL), round = SHORT_WAVES * 16 * (bwd ? 1 : 2), rounds = cdiv(d.T, round);
   int64_t parts = cdiv(256, panels);
   parts = parts > rounds ? rounds : parts >= 8 ? (parts + 7) / 8 * 8 : parts;
   p.part_rows = cdiv(rounds, parts) * round;
   p.parts = cdiv(d.T, p.part_rows);
-  p.big = !(bwd && cdiv(p.Dp, step) <= SHORT_SUM) && large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64));
+  p.big = !bwd && large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64));
+  // (backward: only for what is not kept, sums or results too short for large tiles)
   // less than a block a unit of 128 x (64 + 64): tiles a quarter of that, four stages deep, their loads three steps ahead
   // (2019 x 2816 -> 32 in fp32: 80.9 -> 57.0 us; 1000 x 2048 -> 512 in bf16: 24.4 -> 16.9)
   p.little = !p.big && cdiv(d.T, 128) * cdiv(d.H, 64) <= 64;
-  p.row_tiles = p.brief ? p.parts * SHORT_WAVES : cdiv(d.T, p.big ? 256 : p.little ? 64 : 128);
-  p.pack_blocks = rows_grid(d.T + 2 * (int64_t)d.H);
+  p.keep = d.kept != nullptr;
+  p.row_tiles = p.keep ? cdiv(d.T, KEPT_ROWS) : p.brief ? p.parts * SHORT_WAVES : cdiv(d.T, p.big ? 256 : p.little ? 64 : 128);
+  p.pack_blocks = rows_grid(d.T + 2 * (int64_t)d.H, 4096);
   if (p.brief && !bwd) return p;  // takes everything as it is
-  p.x = p.copy_x && !(p.brief && f32) ? take(d.T * p.Dp * 2 * nl) : 0;
+  p.x = p.copy_x && !(f32 && (p.brief || (p.keep && bwd))) ? take(d.T * p.Dp * 2 * nl) : 0;
   p.w = p.copy_w[0] || p.copy_w[1] ? take(2 * (int64_t)d.H * p.Dp * 2 * nl) : 0;
   if (f32) {
     p.rowexp = take(d.T * 4);
@@ -1084,7 +1282,7 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
     }
     if (d.db_gate || d.db_up) p.dbpart = take(p.row_tiles * 2 * d.H * 4);
     const int64_t x256 = cdiv(d.T, 256) * cdiv(d.D, 256), x128 = cdiv(d.T, 128) * cdiv(d.D, 128);
-    p.dx_big = x256 >= 200 && 2 * cdiv(p.Hp, step) > SHORT_SUM && large_tiles(x256, x128);
+    p.dx_big = x256 >= 150 && 2 * cdiv(p.Hp, step) > SHORT_SUM && large_tiles(x256, x128);
     split_sum(p.dx_big ? 512 : x128, p.Hp, 512, p.dx_splits, p.dx_chunk);
     const int64_t w256 = 2 * cdiv(d.H, 256) * cdiv(d.D, 256), w128 = 2 * cdiv(d.H, 128) * cdiv(d.D, 128);
     p.dw_big = w256 >= 200 && cdiv(d.T, step) > SHORT_SUM && large_tiles(w256, w128);
@@ -1099,6 +1297,7 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
 int check(const hold_gated_desc* d) {
   if (!d || !d->x || !d->w_gate || !d->w_up || d->T < 1 || d->D < 1 || d->H < 1 || d->act < 0 || d->act > 3) return HOLD_E_ARG;
   if (d->dtype != HOLD_GATED_F32 && d->dtype != HOLD_GATED_BF16) return HOLD_E_ARG;
+  if (d->kept && (!keeps(*d) || (uintptr_t)d->kept % 16)) return HOLD_E_ARG;
   if (d->ldx < d->D || d->ldwg < d->D || d->ldwu < d->D) return HOLD_E_ARG;
   // the tile loads' 32-bit offsets: 256 rows of an operand, 64 rows of dg
   if (d->ldx > (1 << 21) || d->ldwg > (1 << 21) || d->ldwu > (1 << 21) || d->H > (1 << 21) || d->T > (1ll << 31)) return HOLD_E_ARG;
@@ -1120,7 +1319,7 @@ void operands(const hold_gated_desc& d, const Plan& p, char* ws, hipStream_t st,
     k.x = (const float*)d.x; k.ldx = d.ldx; k.T = d.T;
     k.w[0] = (const float*)d.w_gate; k.w[1] = (const float*)d.w_up; k.ldw[0] = d.ldwg; k.ldw[1] = d.ldwu;
     k.H = d.H; k.D = d.D; k.Dp = (int)p.Dp;
-    k.ox = p.brief ? nullptr : (uint16_t*)(ws + p.x); k.xlimb = WX;
+    k.ox = p.brief || (p.keep && BWD) ? nullptr : (uint16_t*)(ws + p.x); k.xlimb = WX;
     k.ow = (uint16_t*)(ws + p.w); k.wlimb = 2 * WW; k.second = WW;
     k.rowexp = (int*)(ws + p.rowexp); k.colexp = (int*)(ws + p.colexp); k.Hp = p.Hp;
     if (BWD) {
@@ -1183,11 +1382,25 @@ void launch_short(const hold_gated_desc& d, const MmaArgs& m, const Plan& p, hip
 
 template <int MODE, bool BWD>
 void launch_mma(const hold_gated_desc& d, MmaArgs a, const Plan& p, hipStream_t st) {
-  if (p.brief) {
+  if (p.keep && BWD) {
+    KeptArgs k = {};
+    k.kept = d.kept; k.dh = d.dh; k.lddh = d.lddh;
+    k.T = d.T; k.H = d.H; k.Hp = p.Hp;
+    k.dg = a.dg; k.du = a.du; k.dlimb = a.dlimb;
+    k.rscale = a.rscale; k.exps = a.exps; k.dbpart = a.dbpart;
+    k.cols = (int)cdiv(d.H, 512);
+    hipLaunchKernelGGL(gated_kept_kernel<MODE>, dim3((unsigned)(p.row_tiles * k.cols)), dim3(256), 0, st, k);
+  } else if (p.keep) {
+    a.kept = d.kept;
+    const int t = p.big ? 256 : 128;
+    a.tm = (int)cdiv(a.T, t); a.tn = (int)cdiv(a.H, t / 2);
+    if (p.big) hipLaunchKernelGGL((gated_mma_kernel<MODE, false, 256, 128, 4, 4, true, 2, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((gated_mma_kernel<MODE, false, 128, 64, 4, 2, false, 2, true>), dim3((unsigned)(a.tm * a.tn)), dim3(512), 0, st, a);
+  } else if (p.brief) {
     launch_short<MODE, BWD>(d, a, p, st);
-  } else if (p.big) {
+  } else if (!BWD && p.big) {
     a.tm = (int)cdiv(a.T, 256); a.tn = (int)cdiv(a.H, 128);
-    hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 256, 128, 4, 4, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
+    hipLaunchKernelGGL((gated_mma_kernel<MODE, false, 256, 128, 4, 4, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
   } else if (p.little) {
     a.tm = (int)cdiv(a.T, 64); a.tn = (int)cdiv(a.H, 32);
     hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 64, 32, 2, 1, false, 4>), dim3((unsigned)(a.tm * a.tn)), dim3(128), 0, st, a);
@@ -1303,6 +1516,12 @@ int bwd(const hold_gated_desc& d, hipStream_t st) {
 extern "C" int hold_gated_workspace(const hold_gated_desc* d, int32_t backward, int64_t* bytes) {
   if (check(d) != HOLD_OK || !bytes) return HOLD_E_ARG;
   *bytes = !backward && d->T <= ROWS_MAX ? 0 : plan(*d, backward != 0).bytes;
+  return HOLD_OK;
+}
+
+extern "C" int hold_gated_kept(const hold_gated_desc* d, int64_t* bytes) {
+  if (check(d) != HOLD_OK || !bytes) return HOLD_E_ARG;
+  *bytes = keeps(*d) ? kept_bytes(*d) : 0;
   return HOLD_OK;
 }
 

@@ -678,6 +678,9 @@ int hold_knn1_bwd(const float* q, int32_t B, int32_t Nq, const float* t, int32_t
  * hold_gated_workspace (host only): *bytes = the scratch of one call (256-byte aligned); the pointers
  * and leading dimensions of the descriptor have to be the call's own, and -- backward -- db_gate /
  * db_up null or not as in the call.
+ * hold_gated_kept (host only): *bytes = what a forward call leaves in `kept` for its backward one, 0 where
+ * computing the projections again is less time (`kept` is then NULL in both).  Both calls get the same
+ * `kept` (16-byte aligned), or neither.
  * hold_gated_bwd: dx, dw_gate + dw_up, db_gate, db_up are contiguous and may be null (dw: both or none);
  * dx, dw_gate and dw_up start on 16-byte boundaries.
  * ---------------------------------------------------------------------------------------- */
@@ -696,9 +699,11 @@ typedef struct hold_gated_desc {
   void* workspace;    int64_t workspace_bytes;
   int64_t T;
   int32_t D, H, dtype, act;
+  void* kept;                       /* hold_gated_kept bytes or NULL: forward writes, backward reads */
 } hold_gated_desc;
 
 int hold_gated_workspace(const hold_gated_desc* d, int32_t backward, int64_t* bytes);
+int hold_gated_kept(const hold_gated_desc* d, int64_t* bytes);
 int hold_gated_fwd(const hold_gated_desc* d, hold_stream_t stream);
 int hold_gated_bwd(const hold_gated_desc* d, hold_stream_t stream);
 

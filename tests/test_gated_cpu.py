@@ -68,6 +68,15 @@ def test_entry_points_refuse_bad_descriptors():
     assert L.hold_gated_bwd(C.byref(_desc(**full, workspace=4096, workspace_bytes=need - 1)), None) == -1
     for out in ("dx", "dw_gate", "dw_up"):  # not on a 16-byte boundary
         assert L.hold_gated_bwd(C.byref(_desc(**{**full, out: 4100}, workspace=4096, workspace_bytes=1 << 40)), None) == -1
+    # what is kept for a backward call: nothing for few rows, short ones or little work; a buffer that is not wanted, or not aligned
+    for want, kw in ((0, dict(T=64, H=1 << 17, D=300)), (0, dict(T=70000, D=256)), (0, dict(T=4000, D=300)), (0, dict(T=70000, D=512, dtype=1)),
+                     (70000 * 48 * 8, dict(T=70000, D=257)), (70000 * 48 * 6, dict(T=70000, H=41, D=513, dtype=1))):
+        kw = dict(ldx=1 << 10, ldwg=1 << 10, ldwu=1 << 10, **kw)
+        assert L.hold_gated_kept(C.byref(_desc(**kw)), C.byref(n)) == 0 and n.value == want, kw
+        if not want:
+            assert L.hold_gated_workspace(C.byref(_desc(**kw, kept=4096)), 1, C.byref(n)) == -1
+    assert L.hold_gated_fwd(C.byref(_desc(T=70000, D=300, kept=4104, h=4096, ldh=48, workspace=4096, workspace_bytes=1 << 40)), None) == -1
+    assert L.hold_gated_kept(C.byref(_desc(D=0)), C.byref(n)) == -1 and L.hold_gated_kept(C.byref(_desc()), None) == -1
     # few rows and short ones need no scratch forward; the sizes grow with the rows
     assert L.hold_gated_workspace(C.byref(_desc()), 0, C.byref(n)) == 0 and n.value == 0
     assert L.hold_gated_workspace(C.byref(_desc(T=64, D=300)), 0, C.byref(n)) == 0 and n.value == 0
