@@ -731,7 +731,8 @@ void launch_tiles(const Classes& cl, const NsArgs& s, const Step& st, const Item
 // The tile size by the launch's time, rounds of blocks over the 256 compute units at (per k + fixed) microseconds.  256 and 192: one block a
 // unit; 128: two; 64 (three stages of LDS): three; a last round that leaves units with fewer blocks is shorter.  Fitted to launches alone
 // on single matrices of 1500 .. 4096 and batches of 256 .. 1024 rows, each with every tile size: 4096^3 takes 255 us in 256 x 256
-// tiles, 2 x 154 in 128, 5.3 x 119 in 64; 36 matrices of 256 x 256 in 64 8 us a product, 14 in 128.
+// tiles, 2 x 154 in 128, 5.3 x 119 in 64; 36 matrices of 256 x 256 in 64 8 us a product, 14 in 128.  APPLY with a block a unit or less has
+// eight stages: sums up to 256 are requested at once (256 x 256: 8.6 -> 7.3 us; the symmetric products, 6.6 -> 7.3, gain nothing).
 struct TileCost {
   int size, units;                   // rows; blocks of a full round
   double full[2], two[2], alone[2];  // a round: full, of up to 512 blocks (64), of up to 256
@@ -761,6 +762,7 @@ int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStre
   if (best == 0) launch_tiles<KIND, 256, 4, 4, 2, true, LAST>(cl, s, st, a, n, stream);
   else if (best == 1) launch_tiles<KIND, 192, 3, 4, 2, false, LAST>(cl, s, st, a, n, stream);
   else if (best == 2) launch_tiles<KIND, 128, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
+  else if (KIND == APPLY && n <= 256) launch_tiles<KIND, 64, 2, 2, KIND == APPLY ? 8 : 3, false, LAST>(cl, s, st, a, n, stream);
   else launch_tiles<KIND, 64, 2, 2, 3, false, LAST>(cl, s, st, a, n, stream);
   return HOLD_OK;
 }
