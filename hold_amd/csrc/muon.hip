@@ -284,9 +284,13 @@ template <bool LAST> struct ItemArg { typedef NoItems type; };
 template <> struct ItemArg<true> { typedef Items type; };
 
 // Symmetric results (all but APPLY's): only the tiles on and below the diagonal; what is right of it is written as their mirror image, turned in LDS
+// rows of a tile: T; columns: as many, but 64 at least where an operand is read by k
+template <int KIND>
+constexpr int tile_cols(int T) { return KIND == APPLY && T == 32 ? 64 : T; }
 template <int KIND, int T, int WM, int WN, int S, bool PHASED, bool LAST, class CLASSES>
 __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs s, Step st, typename ItemArg<LAST>::type items) {
-  using Cr = Core<MODE_F16X3, KC, KIND == APPLY ? KS : KC, T, T, 1, WM, WN, S>;
+  constexpr int TC = tile_cols<KIND>(T);
+  using Cr = Core<MODE_F16X3, KC, KIND == APPLY ? KS : KC, T, TC, 1, WM, WN, S, T == 32 ? 64 : 32>;
   constexpr int PITCH = T + 8, TURN = KIND == APPLY ? 0 : T * PITCH * 2;
   __shared__ __align__(1024) char smem[Cr::LDS > TURN ? Cr::LDS : TURN];
   // the tile list is cut into an eighth for each XCD, as tile_of does: neighbours share a matrix
@@ -295,13 +299,13 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
   constexpr bool ONE = sizeof(CLASSES) == sizeof(OneClass);
   const int k = ONE ? 0 : last_below(cl.n, id, [&](int i) { return cl.k[i].tile; });
   const Class& c = cl.k[k];
-  const int m = c.m, n = c.n, mp = c.mp, np = c.np, tm = (mp + T - 1) / T, tn = KIND == APPLY ? (np + T - 1) / T : tm;
+  const int m = c.m, n = c.n, mp = c.mp, np = c.np, tm = (mp + T - 1) / T, tn = KIND == APPLY ? (np + TC - 1) / TC : tm;
   const int per = KIND == APPLY ? tm * tn : tm * (tm + 1) / 2, q = id - c.tile, mat = q / per, tile = q % per;
   int i0, j0;
   if (KIND == APPLY) {  // bands of 8 row tiles, column by column
     const int w = 8 * tn, band = tile / w, f0 = band * 8, h = tm - f0 < 8 ? tm - f0 : 8;
     i0 = (f0 + (tile - band * w) % h) * T;
-    j0 = (tile - band * w) / h * T;
+    j0 = (tile - band * w) / h * TC;
   } else {  // row bi of the triangle begins at tile bi (bi + 1) / 2
     int bi = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
     while (bi * (bi + 1) / 2 > tile) --bi;
@@ -338,7 +342,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
     for (int mi = 0; mi < Cr::MI; ++mi)
 #pragma unroll
       for (int ni = 0; ni < Cr::NI; ++ni) {
-        const int i = i0 + wm * (T / WM) + 16 * mi + (lane & 15), j = j0 + wn * (T / WN) + 16 * ni + 4 * (lane >> 4);
+        const int i = i0 + wm * (T / WM) + 16 * mi + (lane & 15), j = j0 + wn * (TC / WN) + 16 * ni + 4 * (lane >> 4);
         early[EARLY ? mi : 0][EARLY ? ni : 0] = adds && i < mp && j < opitch ? load_limbs(own + (int64_t)i * opitch + j, olimb) : f32x4{0.f, 0.f, 0.f, 0.f};
       }
   }
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
     const int it = wm * (T / WM) + 16 * mi + (lane & 15), i = i0 + it;
 #pragma unroll
     for (int ni = 0; ni < Cr::NI; ++ni) {
-      const int jt = wn * (T / WN) + 16 * ni + 4 * (lane >> 4), j = j0 + jt;
+      const int jt = wn * (TC / WN) + 16 * ni + 4 * (lane >> 4), j = j0 + jt;
       f32x4& v = acc[0][mi][ni];
       const bool in = i < mp && j < (KIND == APPLY ? np : mp);
       if (KIND == GRAM || KIND == PROD) {
@@ -401,7 +405,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const Split y = split16(acc[0][mi][ni][r]);
-            turn[(wn * (T / WN) + 16 * ni + 4 * (lane >> 4) + r) * PITCH + wm * (T / WM) + 16 * mi + (lane & 15)] = l ? y.lo : y.hi;
+            turn[(wn * (TC / WN) + 16 * ni + 4 * (lane >> 4) + r) * PITCH + wm * (T / WM) + 16 * mi + (lane & 15)] = l ? y.lo : y.hi;
           }
       __syncthreads();
       for (int e = threadIdx.x; e < T * T / 8; e += 64 * WM * WN) {
@@ -709,7 +713,7 @@ int64_t count_tiles(Classes& cl, int T) {
   for (int k = 0; k < cl.n; ++k) {
     Class& c = cl.k[k];
     c.tile = (int)n;
-    const int64_t tm = (c.mp + T - 1) / T, tn = (c.np + T - 1) / T;
+    const int64_t tm = (c.mp + T - 1) / T, tn = (c.np + tile_cols<KIND>(T) - 1) / tile_cols<KIND>(T);
     n += (KIND == APPLY ? tm * tn : tm * (tm + 1) / 2) * c.mats;
     if (n > (1 << 30)) return -1;
   }
@@ -758,11 +762,15 @@ int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStre
     if (best < 0 || t < least) { best = k; least = t; }
   }
   if (best < 0) return HOLD_E_ARG;
+  const int64_t few = best == 3 ? count_tiles<KIND>(cl, 32) : -1;
+  if (few > 0 && few <= 256) {
+    launch_tiles<KIND, 32, 2, 2, 4, false, LAST>(cl, s, st, a, (unsigned)few, stream);
+    return HOLD_OK;
+  }
   const unsigned n = (unsigned)count_tiles<KIND>(cl, COST[best].size);
   if (best == 0) launch_tiles<KIND, 256, 4, 4, 2, true, LAST>(cl, s, st, a, n, stream);
   else if (best == 1) launch_tiles<KIND, 192, 3, 4, 2, false, LAST>(cl, s, st, a, n, stream);
   else if (best == 2) launch_tiles<KIND, 128, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
-  else if (KIND == APPLY && n <= 256) launch_tiles<KIND, 64, 2, 2, KIND == APPLY ? 8 : 3, false, LAST>(cl, s, st, a, n, stream);
   else launch_tiles<KIND, 64, 2, 2, 3, false, LAST>(cl, s, st, a, n, stream);
   return HOLD_OK;
 }
