@@ -290,7 +290,7 @@ constexpr int tile_cols(int T) { return KIND == APPLY && T == 32 ? 64 : T; }
 template <int KIND, int T, int WM, int WN, int S, bool PHASED, bool LAST, class CLASSES>
 __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs s, Step st, typename ItemArg<LAST>::type items) {
   constexpr int TC = tile_cols<KIND>(T);
-  using Cr = Core<MODE_F16X3, KC, KIND == APPLY ? KS : KC, T, TC, 1, WM, WN, S, T == 32 ? 64 : 32>;
+  using Cr = Core<MODE_F16X3, KC, KIND == APPLY ? KS : KC, T, TC, 1, WM, WN, S, T == 32 || WM * WN == 8 && T == 64 ? 64 : 32>;
   constexpr int PITCH = T + 8, TURN = KIND == APPLY ? 0 : T * PITCH * 2;
   __shared__ __align__(1024) char smem[Cr::LDS > TURN ? Cr::LDS : TURN];
   // the tile list is cut into an eighth for each XCD, as tile_of does: neighbours share a matrix
@@ -735,8 +735,11 @@ void launch_tiles(const Classes& cl, const NsArgs& s, const Step& st, const Item
 // The tile size by the launch's time, rounds of blocks over the 256 compute units at (per k + fixed) microseconds.  256 and 192: one block a
 // unit; 128: two; 64 (three stages of LDS): three; a last round that leaves units with fewer blocks is shorter.  Fitted to launches alone
 // on single matrices of 1500 .. 4096 and batches of 256 .. 1024 rows, each with every tile size: 4096^3 takes 255 us in 256 x 256
-// tiles, 2 x 154 in 128, 5.3 x 119 in 64; 36 matrices of 256 x 256 in 64 8 us a product, 14 in 128.  APPLY with a block a unit or less has
-// eight stages: sums up to 256 are requested at once (256 x 256: 8.6 -> 7.3 us; the symmetric products, 6.6 -> 7.3, gain nothing).
+// tiles, 2 x 154 in 128, 5.3 x 119 in 64; 36 matrices of 256 x 256 in 64 8 us a product, 14 in 128.  Where
+// a launch of 64 is latency more than work it takes shorter ways: up to two blocks a unit (APPLY: one) in tiles of 32 x 32 (32 x 64) with
+// four stages of 64, sums up to 256 requested at once (a 256 x 256 matrix 120 -> 82 us, 3 x 1531 x 517 250 -> 206 in 16 bits; with more
+// blocks the loads count: 1024 x 1024 280 -> 295); else up to two blocks a unit with eight waves in steps of 64 (1024 x 1024 280 -> 245,
+// 16 x 256 x 256 123 -> 110; above, three blocks of four waves: 48 x 256 x 256 205 against 210).
 struct TileCost {
   int size, units;                   // rows; blocks of a full round
   double full[2], two[2], alone[2];  // a round: full, of up to 512 blocks (64), of up to 256
@@ -763,7 +766,7 @@ int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStre
   }
   if (best < 0) return HOLD_E_ARG;
   const int64_t few = best == 3 ? count_tiles<KIND>(cl, 32) : -1;
-  if (few > 0 && few <= 256) {
+  if (few > 0 && few <= (KIND == APPLY ? 256 : 512)) {
     launch_tiles<KIND, 32, 2, 2, 4, false, LAST>(cl, s, st, a, (unsigned)few, stream);
     return HOLD_OK;
   }
@@ -771,6 +774,7 @@ int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStre
   if (best == 0) launch_tiles<KIND, 256, 4, 4, 2, true, LAST>(cl, s, st, a, n, stream);
   else if (best == 1) launch_tiles<KIND, 192, 3, 4, 2, false, LAST>(cl, s, st, a, n, stream);
   else if (best == 2) launch_tiles<KIND, 128, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
+  else if (n <= 512) launch_tiles<KIND, 64, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
   else launch_tiles<KIND, 64, 2, 2, 3, false, LAST>(cl, s, st, a, n, stream);
   return HOLD_OK;
 }
