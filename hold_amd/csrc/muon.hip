@@ -772,7 +772,7 @@ int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStre
   }
   const unsigned n = (unsigned)count_tiles<KIND>(cl, COST[best].size);
   if (best == 0) launch_tiles<KIND, 256, 4, 4, 2, true, LAST>(cl, s, st, a, n, stream);
-  else if (best == 1) launch_tiles<KIND, 192, 3, 4, 2, false, LAST>(cl, s, st, a, n, stream);
+  else if (best == 1) launch_tiles<KIND, 192, 3, 4, 2, true, LAST>(cl, s, st, a, n, stream);
   else if (best == 2) launch_tiles<KIND, 128, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
   else if (n <= 512) launch_tiles<KIND, 64, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
   else launch_tiles<KIND, 64, 2, 2, 3, false, LAST>(cl, s, st, a, n, stream);
