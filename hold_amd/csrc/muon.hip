@@ -739,7 +739,8 @@ void launch_tiles(const Classes& cl, const NsArgs& s, const Step& st, const Item
 // a launch of 64 is latency more than work it takes shorter ways: up to two blocks a unit (APPLY: one) in tiles of 32 x 32 (32 x 64) with
 // four stages of 64, sums up to 256 requested at once (a 256 x 256 matrix 120 -> 82 us, 3 x 1531 x 517 250 -> 206 in 16 bits; with more
 // blocks the loads count: 1024 x 1024 280 -> 295); else up to two blocks a unit with eight waves in steps of 64 (1024 x 1024 280 -> 245,
-// 16 x 256 x 256 123 -> 110; above, three blocks of four waves: 48 x 256 x 256 205 against 210).
+// 16 x 256 x 256 123 -> 110; above, three blocks of four waves: 48 x 256 x 256 205 against 210).  Tiles of 128 in phases where both
+// operands are read by rows: GRAM of 6 x 1024 x 4096 124 -> 113 us; APPLY's 175 stay 174.
 struct TileCost {
   int size, units;                   // rows; blocks of a full round
   double full[2], two[2], alone[2];  // a round: full, of up to 512 blocks (64), of up to 256
@@ -773,7 +774,7 @@ int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStre
   const unsigned n = (unsigned)count_tiles<KIND>(cl, COST[best].size);
   if (best == 0) launch_tiles<KIND, 256, 4, 4, 2, true, LAST>(cl, s, st, a, n, stream);
   else if (best == 1) launch_tiles<KIND, 192, 3, 4, 2, true, LAST>(cl, s, st, a, n, stream);
-  else if (best == 2) launch_tiles<KIND, 128, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
+  else if (best == 2) launch_tiles<KIND, 128, 2, 4, 2, KIND != APPLY, LAST>(cl, s, st, a, n, stream);
   else if (n <= 512) launch_tiles<KIND, 64, 2, 4, 2, false, LAST>(cl, s, st, a, n, stream);
   else launch_tiles<KIND, 64, 2, 2, 3, false, LAST>(cl, s, st, a, n, stream);
   return HOLD_OK;
