@@ -1258,9 +1258,9 @@ Plan plan(const hold_gated_desc& d, bool bwd) {
   p.parts = cdiv(d.T, p.part_rows);
   p.big = !bwd && large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64));
   // (backward: only for what is not kept, sums or results too short for large tiles)
-  // less than a block a unit of 128 x (64 + 64): tiles a quarter of that, four stages deep, their loads three steps ahead
-  // (2019 x 2816 -> 32 in fp32: 80.9 -> 57.0 us; 1000 x 2048 -> 512 in bf16: 24.4 -> 16.9)
-  p.little = !p.big && cdiv(d.T, 128) * cdiv(d.H, 64) <= 64;
+  // up to half a block a unit of 128 x (64 + 64): tiles a quarter of that, four stages deep, their loads three steps ahead (2019 x 2816 ->
+  // 32 in fp32: 80.9 -> 57.0 us; 1000 x 1000 -> 1000, 128 blocks: 39 -> 32, in bf16 17 -> 13; 2000 x 700 -> 600, 160: 25 against 32)
+  p.little = !p.big && cdiv(d.T, 128) * cdiv(d.H, 64) <= 128;
   p.keep = d.kept != nullptr;
   p.row_tiles = p.keep ? cdiv(d.T, KEPT_ROWS) : p.brief ? p.parts * SHORT_WAVES : cdiv(d.T, p.big ? 256 : p.little ? 64 : 128);
   p.pack_blocks = rows_grid(d.T + 2 * (int64_t)d.H, 4096);

@@ -78,7 +78,7 @@ def close(got, want, what=""):
     assert not bool((over > 0).any()), (what, float(over.max()), float(((a - b).abs() / bound.clamp(min=1e-300)).max()))
 
 
-SIZES = [(1, 1, 1), (1, 256, 256), (3, 7, 5), (4, 129, 66), (16, 64, 200), (17, 33, 9), (64, 260, 31), (65, 8, 8), (65, 40, 72), (127, 64, 64),
+SIZES = [(1, 1, 1), (1, 256, 256), (3, 7, 5), (4, 129, 66), (16, 64, 200), (17, 33, 9), (64, 260, 31), (9, 1100, 20), (20, 1025, 40), (60, 2050, 17), (65, 8, 8), (65, 40, 72), (127, 64, 64),
          (129, 65, 63), (130, 256, 256), (300, 136, 520), (257, 31, 1), (200, 1, 130), (1000, 72, 24), (100, 300, 24), (128, 264, 40),
          (700, 257, 1500)]
 
