@@ -9,10 +9,12 @@
 //
 // KERNELS.  gated_mma_kernel: both projections of a tile share the x tile in LDS, the epilogue applies bias, activation and product
 // (forward) or forms dg, du from dh and the recomputed g, u (backward), with the column sums for the bias gradients from the
-// unrounded values.  gated_short_kernel: the same for D <= 256.  gated_kept_kernel: dg, du from what was kept.  gated_dx_kernel: [dg | du] times [Wg; Wu] as one sum.  gated_dw_kernel: both weight gradients, the sum over
-// tokens split over blocks into fp32 partial tiles that gated_finish_kernel adds in a fixed order.  gated_rows_kernel: T <= 64 rows.
+// unrounded values.  gated_short_kernel: the same for D <= 256.  gated_kept_kernel: dg, du from what was kept.  gated_dx_kernel: [dg | du]
+// times [Wg; Wu] as one sum.  gated_dw_kernel: both weight gradients, the sum over tokens split over blocks into fp32 partial tiles that
+// gated_finish_kernel adds in a fixed order.  gated_rows_kernel, gated_few_kernel: T <= 4, T <= 64.
 //
-// ROUNDINGS.  bf16: dg and du are rounded to bf16 once, as the operands of the next matrix instructions; everything before is fp32.
+// ROUNDINGS.  bf16: dg and du are rounded to bf16 once, as the operands of the next matrix instructions; before, what is kept
+// is cut to 24 bits, and everything else is fp32.
 // fp32: every operand is split into two fp16 limbs (tile16.h) after an exact power-of-two scale: a row of x by its own largest
 // magnitude; the two weight matrices by one exponent each (the same limbs serve the product over D and the one over H); a row of dg,
 // du by a bound of its magnitude from the row maxima of x and dh and the weights' maximum (some log2 D bits above the typical value, of
