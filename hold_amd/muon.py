@@ -15,7 +15,7 @@ import struct
 
 import torch
 
-from . import _lib
+from . import _lib, config
 from ._lib import MuonDesc, MuonItem, OrthoDesc, check, ptr, stream_ptr
 
 #: (a, b, c) of  s -> a s + b s^3 + c s^5
@@ -148,7 +148,11 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
 
     with f = grad_mul, clipped to a global norm where ``clip_norm`` > 0 and ``sumsq`` (a one-element device tensor with the sum of all
     gradients' squares before grad_mul) are given.  Every tensor is 2-D with contiguous rows; no two of the params and momenta may
-    share memory.  All matrices of all shapes go through together, 36 a group: few launches, no host synchronisation."""
+    share memory.  All matrices of all shapes go through together, 36 a group: few launches, no host synchronisation.
+
+    The version counters of params and momenta move as under any in-place operation, and cached weight packs of the framework's
+    models become stale (hold_amd.config.bump_weights_epoch).  Neither happens where a captured graph is replayed: a program that
+    replays a step calls bump_weights_epoch() itself before it uses such a model."""
     what = "muon_step"
     coef = _coefficients(coefficients, steps, what)
     params, grads, momenta = list(params), list(grads), list(momenta)
@@ -208,5 +212,8 @@ def muon_step(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_d
         code = L.hold_muon_step(C.byref(d), stream_ptr())
         if code == -1:
             raise _diverges(what)
+        # written through raw pointers: autograd and the models' weight packs have to be told
+        torch.autograd.graph.increment_version(params + momenta)
+        config.bump_weights_epoch()
         check(code, "hold_muon_step")
 
