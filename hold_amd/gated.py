@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -92,6 +93,12 @@ def _forward(x, w_gate, w_up, b_gate, b_up, act, keep=None):
     return h, _on(x.device, act, x, w_gate, w_up, b_gate, b_up, h, None, None, keep) if h.numel() else None
 
 
+def _no_tangents(*tensors):
+    """a dual tensor has no requires_grad to be seen by: it is refused, its tangent would be lost"""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("gated_linear: forward-mode differentiation is not offered")
+
+
 class _GatedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, b_gate, b_up, act):
@@ -103,6 +110,7 @@ class _GatedFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh):
+        _no_tangents(dh)
         *given, kept = ctx.saved_tensors
         need = list(ctx.needs_input_grad[:5])
         need[1] = need[2] = need[1] or need[2]  # the weights' gradients come together
@@ -119,10 +127,10 @@ class _GatedFn(torch.autograd.Function):
 def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
     """``act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up)``: x [..., D], w_gate and w_up [H, D], biases [H] or None -> [..., H].
 
-    All tensors on one GPU and of one type, float32 or bfloat16.  Differentiable once in every tensor.  Up to 64 rows go through a
-    kernel for few rows that reads the weights as they are, once; more through the tiled ones.  A captured training step takes its
-    gradients by ``torch.autograd.grad``, or by ``backward`` while no eager graph of the same leaves lives (autograd would
-    otherwise make the capture wait for the eager graph's stream)."""
+    All tensors on one GPU and of one type, float32 or bfloat16.  Differentiable once in every tensor, in reverse mode (a tensor
+    with a forward-mode tangent is refused).  Up to 64 rows go through a kernel for few rows that reads the weights as they are,
+    once; more through the tiled ones.  A captured training step takes its gradients by ``torch.autograd.grad``, or by ``backward``
+    while no eager graph of the same leaves lives (autograd would otherwise make the capture wait for the eager graph's stream)."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"gated_linear: activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
@@ -139,6 +147,7 @@ def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, activation="silu"):
             tensors.append(b)
     if dtype not in _DTYPES or any(t.dtype is not dtype for t in tensors):
         raise TypeError(f"gated_linear: float32 or bfloat16 throughout is wanted, got {[str(t.dtype) for t in tensors]}")
+    _no_tangents(*tensors)
     if device.type != "cuda" or any(t.device != device for t in tensors):
         raise ValueError(f"gated_linear: all tensors have to be on one GPU, got {[str(t.device) for t in tensors]}")
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):

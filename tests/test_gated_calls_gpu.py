@@ -1,0 +1,33 @@
+"""Calls of hold_amd.gated.gated_linear that its documentation allows or names: views, and ways of differentiation."""
+import pytest
+import torch
+
+from parity_common import ROOT  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def test_forward_mode_is_refused():
+    """a tangent is never dropped: a dual tensor in any place is refused, with gradients recorded or not; plain ones inside the level go on"""
+    import torch.autograd.forward_ad as fa
+    from hold_amd.gated import gated_linear
+    for T in (5, 100):
+        t = [torch.randn(s, device=DEV) for s in ((T, 24), (16, 24), (16, 24), (16,), (16,))]
+        want = gated_linear(*t)
+        with fa.dual_level():
+            assert torch.equal(gated_linear(*t), want)
+            for k in range(5):
+                a = list(t)
+                a[k] = fa.make_dual(t[k], torch.ones_like(t[k]))
+                with pytest.raises(NotImplementedError):
+                    gated_linear(*a)
+                with torch.no_grad(), pytest.raises(NotImplementedError):
+                    gated_linear(*a)
+                a[0 if k else 1] = a[0 if k else 1].clone().requires_grad_(True)
+                with pytest.raises(NotImplementedError):
+                    gated_linear(*a)
+            leaf = t[0].clone().requires_grad_(True)
+            y = gated_linear(leaf, *t[1:])
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, leaf, fa.make_dual(torch.ones_like(y), torch.ones_like(y)))
