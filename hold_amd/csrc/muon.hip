@@ -186,6 +186,12 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(Items a, Firsts t, Step s,
   if (threadIdx.x == 0) part[it.part + q] = (w[0] + w[1]) + (w[2] + w[3]);
 }
 
+// 2^xs / (|X|_F + eps); a matrix of zeros without eps is divided by one: it stays zero.  (A norm of NaN stays NaN.)
+__device__ __forceinline__ double norm_factor(double sumsq, float eps, int xs) {
+  const double n = sqrt(sumsq) + (double)eps;
+  return ldexp(1. / (n == 0. ? 1. : n), xs);
+}
+
 // X0 as limbs [min][max] (rounded up to 8, zeros behind), scaled by 2^xs: 64 x 64 tiles of the source through LDS, transposed where it is tall
 __global__ __launch_bounds__(256) void ns_load_kernel(Items a, Firsts t, Step s, const double* part, uint16_t* ws, int64_t limb, int xs) {
   const int k = last_below(a.n, blockIdx.x, [&](int i) { return t.first[i]; });
@@ -231,7 +237,7 @@ __global__ __launch_bounds__(256) void ns_load_kernel(Items a, Firsts t, Step s,
     }
   }
   __syncthreads();
-  const double inv = ldexp(1. / (sqrt((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3])) + (double)s.eps), xs);
+  const double inv = norm_factor((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), s.eps, xs);
   uint16_t* x = ws + it.x + (int64_t)mat * mp * np;
   for (int e = threadIdx.x; e < 512; e += 256) {
     const int i = e >> 3, j = (e & 7) * 8;
@@ -512,7 +518,7 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(Items a, Firsts t, Step 
   sum = 0.;
 #pragma unroll
   for (int w = 0; w < 16; ++w) sum += red[w];
-  const double inv = ldexp(1. / (sqrt(sum) + (double)s.eps), st.xs);
+  const double inv = norm_factor(sum, s.eps, st.xs);
 #pragma unroll 4
   for (int e = threadIdx.x; e < count; e += 1024) {
     const int r = e / it.cols, c = e - r * it.cols;

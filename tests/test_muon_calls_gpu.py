@@ -40,3 +40,21 @@ def test_a_step_is_seen_by_autograd():
     assert p._version > at[0] and m._version > at[1]
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("shape", [(20, 30), (300, 200), (700, 1200)])
+def test_zeros_without_eps(shape):
+    """eps = 0: a matrix of zeros stays zero beside others, an unused parameter beside a moving one; NaN stays NaN"""
+    from hold_amd.muon import muon_step, orthogonalize
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn(3, *shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(3)).to(dtype)
+        want = orthogonalize(x, eps=0.0)
+        x[1] = 0
+        got = orthogonalize(x, eps=0.0)
+        assert not got[1].any() and torch.equal(got[::2], want[::2])
+        x[1, 4, 5] = float("nan")
+        assert torch.isnan(orthogonalize(x, eps=0.0)[1]).all()
+    p, z = torch.ones(shape, device=DEV), torch.zeros(shape, device=DEV)
+    m = z.clone()
+    muon_step([p], [z], [m], lr=0.5, weight_decay=0.5, eps=0.0)
+    assert torch.equal(p, torch.full_like(p, 0.75)) and not m.any()
