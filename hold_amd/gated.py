@@ -29,14 +29,14 @@ MAX_WIDTH = 1 << 21
 _SHORT = 256  # up to so many features nothing is kept for the backward pass
 
 
-def _rows(t):
-    """[..., n] as [rows, n] with a unit inner stride and a positive row stride of at least n (copied where it is not so already)"""
+def _rows(t, most=MAX_WIDTH):
+    """[..., n] as [rows, n] with a unit inner stride and a row stride of n to ``most`` (copied where it is not so already)"""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     if not t.is_contiguous():
         rows, n = t.shape
         ld, inner = t.stride()
-        if n > 1 and inner != 1 or rows > 1 and ld < n:
+        if n > 1 and inner != 1 or rows > 1 and not n <= ld <= most:
             t = t.contiguous()
     return t
 
@@ -60,7 +60,7 @@ def _call(act, x, w_gate, w_up, b_gate, b_up, h, dh, out, kept):
     if dh is None:
         d.h, d.ldh = h.data_ptr(), H
     else:
-        dh = _rows(dh)
+        dh = _rows(dh, 1 << 62)
         d.dh, d.lddh = dh.data_ptr(), dh.stride(0) if T > 1 else H
         d.dx, d.dw_gate, d.dw_up, d.db_gate, d.db_up = (None if t is None else t.data_ptr() for t in out)
     L, n, what = _lib.lib(), C.c_int64(0), "gated_linear" if dh is None else "gated_linear (backward)"
