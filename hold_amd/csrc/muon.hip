@@ -6,13 +6,9 @@
 // Three products a step (GRAM: A; POLY: C = a I + b A + c A A; APPLY: C X) for ALL matrices of a call in one launch each: a list of
 // matrices of any shapes (or a batch of equal ones) is cut into tiles, and a block finds its matrix in the tile counts.
 //
-// WIDE MATRICES (n columns, m rows, n >= 1.5 m) spend most of a step on X's two products.  C is a polynomial of A, so A of the next step is
-// C A C, and k steps on X are one with Q = C_k .. C_1: of the steps' products k - 1 GRAMs and APPLYs turn into three symmetric m x m
-// products each (PROD), which for 5 steps of 1024 x 4096 in groups of 2 and 3 leaves 38 of 65 units of m^3.  Groups stay short because A's
-// rounding errors grow by a^2 = 12 a step where X's grow by a.  For a spectrum as narrow as a random matrix's that costs nothing
-// (1024 x 2048: 2.6e-6 of the norm against 2.3e-6 step by step and 3.4e-6 for float32's plain evaluation), for one spread over two
-// decades 2.0e-5 against 2.1e-6, for rank 64 and noise 1.0e-4 against 1.5e-5: nothing to a weight's update or to a result in 16 bits,
-// and done for those only.
+// Steps are taken one by one for every shape and type.  On wide matrices k steps could be joined into Q X with Q built from m x m products,
+// which saves a quarter of the operations; but A's rounding errors then grow by a^2 = 12 a step where X's grow by a, 1.0e-4 of the norm
+// against 1.5e-5 for a matrix of rank 64 and noise, and no caller asked for that.
 //
 // ARITHMETIC.  Small singular values grow by a^steps (485 with the usual coefficients), and with them every rounding of X relative to
 // the largest one; bf16's 2^-9 would be the result there.  So X, A and C = a I + b A + c A A are kept as two fp16 limbs (tile16.h,
@@ -273,15 +269,14 @@ __device__ __forceinline__ f32x4 load_limbs(const uint16_t* p, int64_t limb) {
   return v;
 }
 
-enum { GRAM = 0, POLY = 1, APPLY = 2, PROD = 3 };
+enum { GRAM = 0, POLY = 1, APPLY = 2 };
 struct NsArgs {
   const uint16_t* x;  // X: hi at the item's place, lo `limb` further
   uint16_t* y;        // the next X
-  const uint16_t* l;  // m x m operands: POLY's A; APPLY's C; PROD's two factors
-  const uint16_t* r;
-  uint16_t* o;        // m x m result of GRAM, POLY and PROD
+  const uint16_t* l;  // m x m operand: POLY's A; APPLY's C - a I
+  uint16_t* o;        // m x m result of GRAM and POLY
   int64_t xlimb, climb;
-  float a, b, c;      // POLY, already in the scales of its operands and its result; APPLY: a, where C comes without a I
+  float a, b, c;      // the polynomial's, already in the scales of what they are multiplied with and of the result
   int shift;          // exponent from the accumulated sum to the stored limbs
 };
 
@@ -329,19 +324,18 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
     B[0] = Operand{s.x + xo + (int64_t)j0 * np, s.xlimb, np, mp - j0, np};
   } else if (KIND != APPLY) {
     A = Operand{s.l + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
-    B[0] = Operand{(KIND == POLY ? s.l : s.r) + co + (int64_t)j0 * mp, s.climb, mp, mp - j0, mp};
+    B[0] = Operand{s.l + co + (int64_t)j0 * mp, s.climb, mp, mp - j0, mp};
   } else {
     A = Operand{s.l + co + (int64_t)i0 * mp, s.climb, mp, mp - i0, mp};
     B[0] = Operand{s.x + xo + j0, s.xlimb, np, np - j0, mp};
   }
-  // POLY adds b A, APPLY a X (where C comes without a I: X itself, in one rounding, instead of the limbs of a diagonal that is large against
+  // POLY adds b A, APPLY a X (C comes without a I: X itself, in one rounding, instead of the limbs of a diagonal that is large against
   // the rest of C; in front of the sum every addition would round at its size).  The small tiles' launches are latencies: there the own tile
   // is requested before the products, not behind them
   constexpr bool EARLY = (KIND == POLY || KIND == APPLY) && T <= 64;
   const uint16_t* own = KIND == POLY ? s.l + co : s.x + xo;
   const int64_t olimb = KIND == POLY ? s.climb : s.xlimb;
   const int opitch = KIND == APPLY ? np : mp;
-  const bool adds = KIND == POLY || (KIND == APPLY && s.a != 0.f);
   f32x4 early[EARLY ? Cr::MI : 1][EARLY ? Cr::NI : 1];
   if (EARLY) {
 #pragma unroll
@@ -349,7 +343,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
 #pragma unroll
       for (int ni = 0; ni < Cr::NI; ++ni) {
         const int i = i0 + wm * (T / WM) + 16 * mi + (lane & 15), j = j0 + wn * (TC / WN) + 16 * ni + 4 * (lane >> 4);
-        early[EARLY ? mi : 0][EARLY ? ni : 0] = adds && i < mp && j < opitch ? load_limbs(own + (int64_t)i * opitch + j, olimb) : f32x4{0.f, 0.f, 0.f, 0.f};
+        early[EARLY ? mi : 0][EARLY ? ni : 0] = i < mp && j < opitch ? load_limbs(own + (int64_t)i * opitch + j, olimb) : f32x4{0.f, 0.f, 0.f, 0.f};
       }
   }
   if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
@@ -364,7 +358,7 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
       const int jt = wn * (TC / WN) + 16 * ni + 4 * (lane >> 4), j = j0 + jt;
       f32x4& v = acc[0][mi][ni];
       const bool in = i < mp && j < (KIND == APPLY ? np : mp);
-      if (KIND == GRAM || KIND == PROD) {
+      if (KIND == GRAM) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], s.shift);
         if (in) store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
@@ -372,11 +366,11 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_mma_kernel(CLASSES cl, NsArgs
         if (in) {
           const f32x4 u = EARLY ? early[EARLY ? mi : 0][EARLY ? ni : 0] : load_limbs(own + (int64_t)i * opitch + j, olimb);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = fmaf(s.c, v[r], s.b * u[r]) + (i == j + r ? s.a : 0.f);
+          for (int r = 0; r < 4; ++r) v[r] = fmaf(s.c, v[r], s.b * u[r]);
           store_limbs(sym + (int64_t)i * mp + j, s.climb, v);
         }
       } else {
-        if (adds && in) v += s.a * (EARLY ? early[EARLY ? mi : 0][EARLY ? ni : 0] : load_limbs(own + (int64_t)i * opitch + j, olimb));
+        if (in) v += s.a * (EARLY ? early[EARLY ? mi : 0][EARLY ? ni : 0] : load_limbs(own + (int64_t)i * opitch + j, olimb));
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], s.shift);
         if constexpr (!LAST) {
@@ -622,7 +616,6 @@ inline int ok() { return hipGetLastError() == hipSuccess ? HOLD_OK : HOLD_E_LAUN
 // The bounds of the singular values of X, and of the entries of A and C, through the iteration; false: they leave the range of the limbs
 struct Bounds {
   int xs[33], as[33], cs[33];  // exponents of the scales of X, A, C: largest entry to below 2^14, a factor of 4 under fp16's range
-  int cb[33], ab[33];          // exponents above the bounds of C's and A's singular values
 };
 bool follow(const float* coef, int steps, Bounds& o) {
   double r = 1.;
@@ -630,16 +623,14 @@ bool follow(const float* coef, int steps, Bounds& o) {
     if (!(r < 1e9) || !(r > 1e-9)) return false;
     o.xs[k] = 14 - (int)ceil(log2(r));
     if (k == steps) break;
-    o.ab[k] = (int)ceil(2. * log2(r));
-    o.as[k] = 14 - o.ab[k];
+    o.as[k] = 14 - (int)ceil(2. * log2(r));
     const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2], S = r * r;
     if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
     auto P = [&](double s) { return fabs(a + b * s + c * s * s); };
-    double top = fmax(fmax(P(0.), P(S)), fabs(b * S + c * S * S));  // of C with and without a I
+    double top = fmax(fmax(P(0.), P(S)), fabs(b * S + c * S * S));  // of a I + C, and of C, which is what is stored
     if (c != 0. && -b / (2. * c) > 0. && -b / (2. * c) < S) top = fmax(fmax(top, P(-b / (2. * c))), fabs(b * b / (4. * c)));
     if (!(top < 1e9) || !(top > 1e-9)) return false;
-    o.cb[k] = (int)ceil(log2(top));
-    o.cs[k] = 14 - o.cb[k];
+    o.cs[k] = 14 - (int)ceil(log2(top));
     // the largest |s (a + b s^2 + c s^4)| on [0, r]: its ends and where a + 3 b s^2 + 5 c s^4 = 0
     double next = r * P(S);
     auto at = [&](double s2) {
@@ -661,19 +652,12 @@ bool follow(const float* coef, int steps, Bounds& o) {
 
 inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// the workspace of one group of items: partial sums, X twice, A and C (and Q and one more where steps are joined), all limbs
+// the workspace of one group of items: partial sums, X twice, A and C, all limbs
 struct Room {
-  int64_t part, x, y, mm[4], xn, cn, bytes;
+  int64_t part, x, y, mm[2], xn, cn, bytes;
 };
-// Whether an item's steps are joined: measured on 6 x 1024 x 4096 (1.57 -> 1.05 ms) and 3 x 1531 x 517 (274 -> 249 us); with less
-// work launches are what counts, and a result in float32 keeps float32's exactness
-bool joined(const Item& it, bool exact) {
-  if (exact) return false;
-  const double m = it.rows < it.cols ? it.rows : it.cols, n = it.rows < it.cols ? it.cols : it.rows;
-  return n >= 1.5 * m && m * m * n * it.count >= 1e9;
-}
 // sorts the items by shape, finds the classes and lays out the workspace
-Room room(Items& a, Classes& cl, bool join) {
+Room room(Items& a, Classes& cl) {
   auto small = [](const Item& i) { return i.rows < i.cols ? i.rows : i.cols; };
   auto large = [](const Item& i) { return i.rows < i.cols ? i.cols : i.rows; };
   for (int k = 1; k < a.n; ++k) {  // by insertion: equal shapes keep their order
@@ -707,7 +691,7 @@ Room room(Items& a, Classes& cl, bool join) {
   r.part = take(parts * 8);
   r.x = take(xn * 4);
   r.y = take(xn * 4);
-  for (int k = 0; k < (join ? 4 : 2); ++k) r.mm[k] = take(cn * 4);
+  for (int k = 0; k < 2; ++k) r.mm[k] = take(cn * 4);
   r.xn = xn; r.cn = cn;
   r.bytes = o;
   return r;
@@ -786,16 +770,15 @@ int launch(Classes& cl, const NsArgs& s, const Step& st, const Items& a, hipStre
   return HOLD_OK;
 }
 
-int run_group(Items& a, bool join, const Step& st, const float* coef, int steps, char* ws, hipStream_t stream) {
+int run_group(Items& a, const Step& st, const float* coef, int steps, char* ws, hipStream_t stream) {
   Bounds bo;
   if (!follow(coef, steps, bo)) return HOLD_E_ARG;
   Classes cl;
-  const Room r = room(a, cl, join);
+  const Room r = room(a, cl);
   double* part = (double*)(ws + r.part);
   uint16_t* x = (uint16_t*)(ws + r.x);
   uint16_t* y = (uint16_t*)(ws + r.y);
-  uint16_t* mm[4];
-  for (int k = 0; k < 4; ++k) mm[k] = (uint16_t*)(ws + r.mm[k]);
+  uint16_t* mm[2] = {(uint16_t*)(ws + r.mm[0]), (uint16_t*)(ws + r.mm[1])};
   Firsts tn = {}, tl = {};
   int64_t nn = 0, nl = 0;
   for (int k = 0; k < a.n; ++k) {
@@ -819,67 +802,29 @@ int run_group(Items& a, bool join, const Step& st, const float* coef, int steps,
     s.shift = bo.as[k] - 2 * bo.xs[k];
     if (rc == HOLD_OK) rc = launch<GRAM, false>(cl, s, st, a, stream);
   };
-  auto poly = [&](int k, uint16_t* o, bool whole) {  // whole: with a I
+  auto poly = [&](int k) {  // C without a I
     s.l = mm[0];
-    s.o = o;
-    s.a = whole ? (float)ldexp((double)coef[3 * k], bo.cs[k]) : 0.f;
+    s.o = mm[1];
     s.b = (float)ldexp((double)coef[3 * k + 1], bo.cs[k] - bo.as[k]);
     s.c = (float)ldexp((double)coef[3 * k + 2], bo.cs[k] - 2 * bo.as[k]);
     if (rc == HOLD_OK) rc = launch<POLY, false>(cl, s, st, a, stream);
   };
-  auto prod = [&](const uint16_t* l, const uint16_t* p, uint16_t* o, int shift) {
-    s.l = l;
-    s.r = p;
-    s.o = o;
-    s.shift = shift;
-    if (rc == HOLD_OK) rc = launch<PROD, false>(cl, s, st, a, stream);
-  };
-  auto apply = [&](const uint16_t* c, int cs, int from, int to, float own) {  // X of step `from` -> X before step `to`
-    s.a = own;
-    s.l = c;
+  auto apply = [&](int k) {
+    const bool last = k + 1 == steps;
+    s.a = (float)ldexp((double)coef[3 * k], bo.cs[k]);
+    s.l = mm[1];
     s.x = x;
     s.y = y;
-    s.shift = (to == steps ? 0 : bo.xs[to]) - cs - bo.xs[from];
-    if (rc == HOLD_OK) rc = to == steps ? launch<APPLY, true>(cl, s, st, a, stream) : launch<APPLY, false>(cl, s, st, a, stream);
+    s.shift = (last ? 0 : bo.xs[k + 1]) - bo.cs[k] - bo.xs[k];
+    if (rc == HOLD_OK) rc = last ? launch<APPLY, true>(cl, s, st, a, stream) : launch<APPLY, false>(cl, s, st, a, stream);
     uint16_t* z = x;
     x = y;
     y = z;
   };
-  if (!join) {
-    for (int k = 0; k < steps; ++k) {
-      gram(k);
-      poly(k, mm[1], false);
-      apply(mm[1], bo.cs[k], k, k + 1, (float)ldexp((double)coef[3 * k], bo.cs[k]));
-    }
-  } else {
-    const int groups = (steps + 2) / 3;
-    for (int g = 0, k = 0; g < groups; ++g) {
-      const int first = k, end = steps * (g + 1) / groups;
-      uint16_t *A = mm[0], *C = mm[1], *Q = mm[2], *T = mm[3];
-      int qb = 0;  // exponent above Q's singular values
-      gram(k);
-      for (; k < end; ++k) {
-        const uint16_t* c = C;
-        if (k == first) {
-          poly(k, Q, true);
-          c = Q;
-          qb = bo.cb[k];
-        } else {
-          poly(k, C, true);
-          qb += bo.cb[k];
-          prod(C, Q, T, 14 - qb - bo.cs[k] - (14 - (qb - bo.cb[k])));
-          uint16_t* z = Q;
-          Q = T;
-          T = z;
-        }
-        if (k + 1 < end) {  // A <- (C A) C
-          const int ts = 14 - bo.cb[k] - bo.ab[k];
-          prod(c, A, T, ts - bo.cs[k] - bo.as[k]);
-          prod(T, c, A, bo.as[k + 1] - ts - bo.cs[k]);
-        }
-      }
-      apply(Q, 14 - qb, first, end, 0.f);
-    }
+  for (int k = 0; k < steps; ++k) {
+    gram(k);
+    poly(k);
+    apply(k);
   }
   return rc == HOLD_OK ? ok() : rc;
 }
@@ -908,10 +853,6 @@ int run_small(const Items& a, const Step& st, const float* coef, int steps, hipS
   return ok();
 }
 
-// how an item is computed: in one block's LDS, step by step, or with steps joined
-enum { SMALL = 0, PLAIN = 1, JOIN = 2 };
-int way_of(const Item& it, bool exact, int steps) { return small(it, steps) ? SMALL : joined(it, exact) ? JOIN : PLAIN; }
-
 bool sizes_ok(int64_t rows, int64_t cols, int64_t count) {
   return rows >= 1 && cols >= 1 && count >= 1 && rows <= (1 << 20) && cols <= (1 << 20) && count <= (1 << 24);
 }
@@ -937,28 +878,29 @@ bool read_item(const hold_muon_desc* d, int k, Item& it) {
   return true;
 }
 // a launch has less than 2^32 threads: a batch that would pass 2^21 blocks goes in parts, one after the other in the same workspace
-int32_t part_of(const Item& it, int way) {
-  if (way == SMALL) return 1 << 21;
+int32_t part_of(const Item& it, int steps) {
+  if (small(it, steps)) return 1 << 21;
   const int64_t blocks = ((int64_t)it.rows + 71) / 64 * (((int64_t)it.cols + 71) / 64) + 512, n = (1 << 21) / blocks;
   return n < 1 ? 1 : (int32_t)n;
 }
-// calls f(items, way) for the groups of a step, up to MAXI items that are computed alike; false: a bad item
+// calls f(items, little) for the groups of a step, up to MAXI items that are computed alike: in one block's LDS each (little), or all in
+// every launch; false: a bad item
 template <class F>
 bool groups_of(const hold_muon_desc* d, F f) {
-  for (int way = JOIN; way >= SMALL; --way) {
+  for (const bool little : {false, true}) {
     Items a;
     a.n = 0;
     for (int k = 0; k < d->n_items; ++k) {
       Item it;
       if (!read_item(d, k, it)) return false;
-      if (way_of(it, false, d->steps) != way) continue;
+      if (small(it, d->steps) != little) continue;
       a.it[a.n++] = it;
       if (a.n == MAXI) {
-        if (!f(a, way)) return false;
+        if (!f(a, little)) return false;
         a.n = 0;
       }
     }
-    if (a.n && !f(a, way)) return false;
+    if (a.n && !f(a, little)) return false;
   }
   return true;
 }
@@ -969,10 +911,9 @@ extern "C" int hold_orthogonalize_workspace(const hold_ortho_desc* d, int64_t* b
   Items a;
   Classes cl;
   if (!one_item(d, a) || !bytes) return HOLD_E_ARG;
-  const int way = way_of(a.it[0], d->dtype == HOLD_MUON_F32, d->steps);
-  const int32_t part = part_of(a.it[0], way);
+  const int32_t part = part_of(a.it[0], d->steps);
   if (a.it[0].count > part) a.it[0].count = part;
-  *bytes = way == SMALL ? 256 : room(a, cl, way == JOIN).bytes;
+  *bytes = small(a.it[0], d->steps) ? 256 : room(a, cl).bytes;
   return HOLD_OK;
 }
 
@@ -985,16 +926,15 @@ extern "C" int hold_orthogonalize(const hold_ortho_desc* d, hold_stream_t stream
   st.eps = d->eps;
   st.dtype = d->dtype;
   const Item whole = a.it[0];
-  const int way = way_of(whole, d->dtype == HOLD_MUON_F32, d->steps);
   const int64_t bytes = whole.stride * (d->dtype == HOLD_MUON_F32 ? 4 : 2);
-  const int32_t part = part_of(whole, way);
+  const int32_t part = part_of(whole, d->steps);
   for (int32_t k = 0; k < d->batch; k += part) {
     Item& it = a.it[0] = whole;
     it.g = (const char*)d->x + k * bytes;
     it.p = (char*)d->out + k * bytes;
     it.count = d->batch - k < part ? d->batch - k : part;
-    const int rc = way == SMALL ? run_small(a, st, d->coef, d->steps, (hipStream_t)stream)
-                                : run_group(a, way == JOIN, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+    const int rc = small(whole, d->steps) ? run_small(a, st, d->coef, d->steps, (hipStream_t)stream)
+                                          : run_group(a, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
     if (rc != HOLD_OK) return rc;
   }
   return HOLD_OK;
@@ -1003,10 +943,10 @@ extern "C" int hold_orthogonalize(const hold_ortho_desc* d, hold_stream_t stream
 extern "C" int hold_muon_workspace(const hold_muon_desc* d, int64_t* bytes) {
   if (!d || !bytes || d->n_items < 1 || !d->items) return HOLD_E_ARG;
   *bytes = 256;
-  return groups_of(d, [&](Items& a, int way) {
-    if (way == SMALL) return true;
+  return groups_of(d, [&](Items& a, bool little) {
+    if (little) return true;
     Classes cl;
-    const int64_t n = room(a, cl, way == JOIN).bytes;
+    const int64_t n = room(a, cl).bytes;
     if (n > *bytes) *bytes = n;
     return true;
   }) ? HOLD_OK : HOLD_E_ARG;
@@ -1030,9 +970,9 @@ extern "C" int hold_muon_step(const hold_muon_desc* d, hold_stream_t stream) {
   st.clip = d->clip_norm;
   st.sumsq = d->sumsq;
   int rc = HOLD_OK;  // groups share the workspace: they run one after the other
-  groups_of(d, [&](Items& a, int way) {
-    rc = way == SMALL ? run_small(a, st, d->coef, d->steps, (hipStream_t)stream)
-                      : run_group(a, way == JOIN, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
+  groups_of(d, [&](Items& a, bool little) {
+    rc = little ? run_small(a, st, d->coef, d->steps, (hipStream_t)stream)
+                : run_group(a, st, d->coef, d->steps, (char*)d->workspace, (hipStream_t)stream);
     return rc == HOLD_OK;
   });
   return rc;

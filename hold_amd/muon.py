@@ -6,7 +6,8 @@ matrices by such a matrix; ``hold_amd.optim.FlatMuon`` runs it over a model's hi
 
 Inside, matrices are kept in two fp16 limbs (2^-22 of the largest value) and multiplied with float32 accumulation whatever the
 input's type: the iteration multiplies the smallest singular values by up to a^steps (485 by default), and the rounding errors
-with them.
+with them.  The iteration is one for updates and results of every type; its error is of float32's own size in the matrix's norm, and a
+16-bit result is rounded once, at the end.
 """
 from __future__ import annotations
 
