@@ -9,17 +9,17 @@
 //
 // KERNELS.  gated_mma_kernel: both projections of a tile share the x tile in LDS, the epilogue applies bias, activation and product
 // (forward) or forms dg, du from dh and the recomputed g, u (backward), with the column sums for the bias gradients from the
-// unrounded values.  gated_short_kernel: the same for D <= 256.  gated_kept_kernel: dg, du from what was kept.  gated_dx_kernel: [dg | du]
+// unrounded values.  gated_short_kernel: the same for D <= 256 in bf16.  gated_kept_kernel: dg, du from what was kept.  gated_dx_kernel: [dg | du]
 // times [Wg; Wu] as one sum.  gated_dw_kernel: both weight gradients, the sum over tokens split over blocks into fp32 partial tiles that
 // gated_finish_kernel adds in a fixed order.  gated_rows_kernel, gated_few_kernel: T <= 4, T <= 64.
 //
-// ROUNDINGS.  bf16: dg and du are rounded to bf16 once, as the operands of the next matrix instructions; before, what is kept
-// is cut to 24 bits, and everything else is fp32.
-// fp32: every operand is split into two fp16 limbs (tile16.h) after an exact power-of-two scale: a row of x by its own largest
-// magnitude; the two weight matrices by one exponent each (the same limbs serve the product over D and the one over H); a row of dg,
-// du by a bound of its magnitude from the row maxima of x and dh and the weights' maximum (some log2 D bits above the typical value, of
-// the 39 that the limbs span), du's 2^(eu - eg) times dg's, the ratio of the weight matrices' scales: so both halves of dx meet at one
-// scale.  For dW the rows' scales are taken back on the x side: x_t 2^(R - r_t), R from the largest row.
+// ROUNDINGS.  fp32: fp32 products and sums on v_mfma_f32_16x16x4_f32, for any number of rows.  Two fp16 limbs a value under a row's common
+// scale take half the time (131072 x 256 -> 256 125 against 276 us, a step of 16384 x 768 -> 4096 2.35 against 5.24 ms) and lose digits
+// without a sign where a row of x, of a weight or of dg spans more than some four decades (3e-3 relative at ten, 512 features); three bf16
+// limbs keep every exponent, but an infinity times a limb of zero is NaN.
+// bf16: dg and du are rounded to bf16 once, as the operands of the next matrix instructions (gradients 2.35e-3 from the
+// exact ones, 1.66e-3 with that rounding left out and only the result's own; a second limb of each would double both products, two
+// thirds of a training step); before, what is kept is cut to 24 bits, and everything else is fp32.
 #include "tile16.h"
 
 #include "../../include/hold_hip.h"
@@ -133,6 +133,20 @@ __device__ __forceinline__ void store4(void* p, int64_t i, int n, f32x4 v) {
   }
 }
 
+// eight, on a 16-byte boundary
+template <int MODE>
+__device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[8]) {
+  if constexpr (MODE == MODE_BF16) {
+    u32x4 w;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) w[r] = bf16_bits(v[2 * r]) | (uint32_t)bf16_bits(v[2 * r + 1]) << 16;
+    *(u32x4*)((uint16_t*)p + i) = w;
+  } else {
+    *(f32x4*)((float*)p + i) = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4*)((float*)p + i + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  }
+}
+
 template <int MODE> constexpr int chunk_k() { return MODE == MODE_BF16 ? 8 : 4; }  // elements in 16 bytes
 
 // 16 bytes of a row from element c on, zeros from element K on
@@ -158,225 +172,38 @@ __device__ __forceinline__ float lane_value(u32x4 v, int i) {
   return __builtin_bit_cast(float, MODE == MODE_BF16 ? (i & 1 ? w & 0xffff0000u : w << 16) : w);
 }
 
-template <int K>
-__device__ __forceinline__ int wave_max(int v) {
-#pragma unroll
-  for (int o = K / 2; o > 0; o >>= 1) {
-    const int u = __shfl_xor(v, o, 64);
-    v = u > v ? u : v;
-  }
-  return v;
-}
-__device__ __forceinline__ float wave_fmax(float v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
-
-constexpr int NPART = 256;  // blocks that look for the weights' maxima
-// exponents kept by a backward call in fp32 (ints): [0] Wg, [1] Wu, [2] bg, [3] bu (exp_above of the largest magnitude, NONE of nothing),
-// [4] R, [5] and [6] the exponents by which Wg and Wu are scaled (a matrix of zeros takes the other's)
-constexpr int NONE = -100000;
-__device__ __forceinline__ int exp_or_none(float m) { return m > 0.f ? exp_above(m) : NONE; }
-
-// a wave's rows: 4 consecutive elements a lane, 256 a piece
-__device__ __forceinline__ f32x4 row4(const float* p, int c, int K) { return load4<MODE_F16X3>(p, c, K - c); }
-
-__device__ __forceinline__ float row_max(const float* p, int K) {
-  const int lane = threadIdx.x & 63;
-  float m = 0.f;
-  for (int c = 4 * lane; c < K; c += 256) {
-    const f32x4 v = row4(p, c, K);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) m = fmaxf(m, finite_abs(v[r]));
-  }
-  return wave_fmax(m);
-}
-
-// largest finite magnitude of the weights and biases, per block of the grid: part[which][block]
-__global__ __launch_bounds__(256) void gated_amax_kernel(const float* wg, int64_t ldg, const float* wu, int64_t ldu, const float* bg,
-                                                         const float* bu, int H, int D, float* part) {
-  const int which = blockIdx.y;
-  float m = 0.f;
-  if (which < 2) {
-    const float* p = which ? wu : wg;
-    const int64_t ld = which ? ldu : ldg;
-    for (int r = blockIdx.x * 4 + (threadIdx.x >> 6); r < H; r += gridDim.x * 4) m = fmaxf(m, row_max(p + r * ld, D));
-  } else {
-    const float* p = which == 2 ? bg : bu;
-    if (p)
-      for (int c = blockIdx.x * 256 + threadIdx.x; c < H; c += gridDim.x * 256) m = fmaxf(m, finite_abs(p[c]));
-    m = wave_fmax(m);
-  }
-  __shared__ float s[4];
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) part[which * NPART + blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-}
-
-__device__ __forceinline__ float part_max(const float* part, int which) {  // every wave of a block by itself; NPART values
-  const int lane = threadIdx.x & 63;
-  const f32x4 v = *(const f32x4*)(part + which * NPART + 4 * lane);
-  static_assert(NPART == 256, "four values a lane");
-  return wave_fmax(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
-}
-
-// 4 scaled values as limbs; columns behind K up to Kp as zeros
-__device__ __forceinline__ void put_limbs(uint16_t* o, int64_t limb, f32x4 v, int k) {
-  Split y[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) y[r] = split16(ldexpf(v[r], k));
-  *(u32x2*)o = u32x2{y[0].hi | (uint32_t)y[1].hi << 16, y[2].hi | (uint32_t)y[3].hi << 16};
-  *(u32x2*)(o + limb) = u32x2{y[0].lo | (uint32_t)y[1].lo << 16, y[2].lo | (uint32_t)y[3].lo << 16};
-}
-// one row to limbs by 2^k
-__device__ __forceinline__ void pack_row(const float* p, int K, int Kp, int k, uint16_t* o, int64_t limb) {
-  const int lane = threadIdx.x & 63;
-  for (int c = 4 * lane; c < Kp; c += 256) put_limbs(o + c, limb, row4(p, c, K), k);
-}
-
-struct PackArgs {
-  const float* x; int64_t ldx, T;
-  const float* w[2]; int64_t ldw[2];
-  int H, D, Dp;
-  uint16_t* ox; int64_t xlimb;  // null: x's rows are only measured
-  uint16_t* ow; int64_t wlimb, second;
-  int* rowexp;       // [T]
-  int* colexp;       // [2][Hp]: the exponent of a weight row's scale
-  int64_t Hp;
-  // backward
-  const float* part; // the weights' maxima: one scale a matrix, and the exponents below
-  int* exps;
-  const float* dh; int64_t lddh; int act;
-  int* rscale; int* rpart;
-};
-
-// All rows to limbs [rows][Dp], a wave a row: x's scaled to [2^14, 2^15) by their own exponents, the weights' too (forward, where they only
-// meet x) or by one a matrix (backward, where the sum also runs over H).  Backward: also the scale exponent r_t of a row of dg and du and
-// the block's largest exponent of x_t 2^-r_t:
-//   |g| <= D max|x_t| max|Wg| + max|bg|, |u| likewise; |act(g)| <= |g| (sigmoid: 1); |act'| < 2 (relu: 1, sigmoid: 1/4)
-template <bool BWD>
-__global__ __launch_bounds__(256) void gated_pack_kernel(PackArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int e[4] = {NONE, NONE, NONE, NONE}, ws[2] = {0, 0}, ld2 = 0, top = NONE;
-  if (BWD) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = exp_or_none(part_max(a.part, i));
-    ws[0] = e[0] != NONE ? e[0] : e[1] != NONE ? e[1] : 15;
-    ws[1] = e[1] != NONE ? e[1] : e[0] != NONE ? e[0] : 15;
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-      a.exps[5] = ws[0];
-      a.exps[6] = ws[1];
-    }
-    while ((1 << ld2) < a.D) ++ld2;
-  }
-  const int64_t rows = a.T + 2 * (int64_t)a.H;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < rows; r += (int64_t)gridDim.x * 4) {
-    if (r >= a.T) {
-      const int w = r - a.T >= a.H, j = (int)(r - a.T) - w * a.H;
-      const float* p = a.w[w] + j * a.ldw[w];
-      int ex = BWD ? ws[w] : 0;
-      if (!BWD) {
-        ex = exp_or_none(row_max(p, a.D));
-        ex = ex == NONE ? 15 : ex;
-      }
-      if (lane == 0) a.colexp[w * a.Hp + j] = ex;
-      pack_row(p, a.D, a.Dp, 15 - ex, a.ow + w * a.second + (int64_t)j * a.Dp, a.wlimb);
-      continue;
-    }
-    const float* p = a.x + r * a.ldx;
-    uint16_t* o = a.ox + r * a.Dp;
-    int ex;
-    if (a.Dp <= 256) {  // the row stays in registers
-      const f32x4 v = row4(p, 4 * lane, a.D);
-      ex = exp_or_none(wave_fmax(fmaxf(fmaxf(finite_abs(v[0]), finite_abs(v[1])), fmaxf(finite_abs(v[2]), finite_abs(v[3])))));
-      if (4 * lane < a.Dp && a.ox) put_limbs(o + 4 * lane, a.xlimb, v, ex == NONE ? 0 : 15 - ex);
-    } else {
-      ex = exp_or_none(row_max(p, a.D));
-      if (a.ox) pack_row(p, a.D, a.Dp, ex == NONE ? 0 : 15 - ex, o, a.xlimb);
-    }
-    if (lane == 0) a.rowexp[r] = ex;
-    if (BWD) {
-      const int ed = exp_or_none(row_max(a.dh + r * a.lddh, a.H));
-      auto proj = [&](int w) {  // exponent above a projection's magnitude
-        const int m = (ex == NONE || e[w] == NONE) ? NONE : ex + e[w] + ld2, b = e[2 + w];
-        return (m > b ? m : b) == NONE ? NONE : (m > b ? m : b) + 1;
-      };
-      const int eg = proj(0), eu = proj(1);
-      const int ea = a.act == ACT_SIGMOID ? 0 : eg, edg = eu + (a.act == ACT_SIGMOID ? -2 : a.act == ACT_RELU ? 0 : 1);
-      // r_t of dg such that dg 2^r_t and du 2^(r_t + shift) both stay below 2^15
-      const int shift = ws[1] - ws[0], top2 = edg > ea + shift ? edg : ea + shift;
-      const bool none = ed == NONE || top2 < -50000;
-      const int k = none ? NONE : 15 - (ed + top2);
-      if (lane == 0) a.rscale[r] = k;
-      if (!none && ex != NONE && ex - k > top) top = ex - k;
-    }
-  }
-  if (BWD) {
-    __shared__ int s[4];
-    if (lane == 0) s[wave] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const int u = s[0] > s[1] ? s[0] : s[1], v = s[2] > s[3] ? s[2] : s[3];
-      a.rpart[blockIdx.x] = u > v ? u : v;
-    }
-  }
-}
-
-// x_t 2^(R - r_t) as limbs for the sum over tokens; rows without a gradient are zeros (where finite).  exps[4] = R
-__global__ __launch_bounds__(256) void gated_pack_tokens_kernel(const float* x, int64_t ld, int64_t T, int D, int Dp, const int* rscale,
-                                                                const int* part, int nparts, uint16_t* out, int64_t limb, int* exps) {
-  const int lane = threadIdx.x & 63;
-  __shared__ int tops[4];
-  int top = NONE;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < nparts; i += 256) top = part[i] > top ? part[i] : top;
-  top = wave_max<64>(top);
-  if (lane == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = tops[i] > top ? tops[i] : top;
-  const int R = top == NONE ? 0 : 15 - top;
-  if (blockIdx.x == 0 && threadIdx.x == 0) exps[4] = R;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < T; r += (int64_t)gridDim.x * 4) {
-    const int k = rscale[r];
-    for (int c = 4 * lane; c < Dp; c += 256) {
-      f32x4 v = row4(x + r * ld, c, D);
-      if (k == NONE) v *= 0.f;
-      put_limbs(out + r * Dp + c, limb, v, k == NONE ? 0 : R - k);
-    }
-  }
-}
-
-// bf16 rows whose base, stride or length the tile loads cannot take -> [rows][Kp], zeros behind K; up to three matrices of equal length
+// rows whose base, stride or length the tile loads cannot take -> [rows][Kp], zeros behind K; up to three matrices of equal length
 struct CopyArgs {
-  const uint16_t* x[3]; int64_t ld[3], rows[3];
-  uint16_t* out[3];
+  const void* x[3]; int64_t ld[3], rows[3];
+  void* out[3];
   int K, Kp;
 };
+template <int MODE>
 __global__ __launch_bounds__(256) void gated_copy_rows_kernel(CopyArgs a) {
+  constexpr int N = chunk_k<MODE>();
   const int lane = threadIdx.x & 63;
   const int64_t all = a.rows[0] + a.rows[1] + a.rows[2];
   for (int64_t q = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); q < all; q += (int64_t)gridDim.x * 4) {
     const int w = q < a.rows[0] ? 0 : q < a.rows[0] + a.rows[1] ? 1 : 2;
     const int64_t r = q - (w > 0 ? a.rows[0] : 0) - (w > 1 ? a.rows[1] : 0);
-    const uint16_t* p = a.x[w] + r * a.ld[w];
-    uint16_t* o = a.out[w] + r * a.Kp;
-    for (int c = 8 * lane; c < a.Kp; c += 512) *(u32x4*)(o + c) = chunk16<MODE_BF16>(p, 0, c, a.K);
+    u32x4* o = (u32x4*)a.out[w] + r * (a.Kp / N);
+    for (int c = lane; c < a.Kp / N; c += 64) o[c] = chunk16<MODE>(a.x[w], r * a.ld[w], c * N, a.K);
   }
 }
 
+// element i of an operand of the tile loads
+template <int MODE>
+__device__ __forceinline__ const uint16_t* element(const void* p, int64_t i) { return (const uint16_t*)p + i * halves<MODE>(); }
+
 // ---- both projections and what follows them -------------------------------------------------------------------------------------------
 struct MmaArgs {
-  const uint16_t* x; int64_t ldx, xlimb;         // operands as the tile loads take them: [T][Dp]
-  const uint16_t* wg; const uint16_t* wu; int64_t ldwg, ldwu, wlimb;
+  const void* x; int64_t ldx;                    // operands as the tile loads take them: [T][K]
+  const void* wg; const void* wu; int64_t ldwg, ldwu;
   const void* bg; const void* bu;
   int64_t T; int H; int K; int act;
-  const int* rowexp; const int* colexp; const int* exps;  // fp32: the scales of x's rows, of the weights' rows; backward's exponents
   void* h; int64_t ldh;                          // forward
   const void* dh; int64_t lddh;                  // backward
-  uint16_t* dg; uint16_t* du; int64_t Hp, dlimb; // [T][Hp] limbs of dg and du
-  const int* rscale;
+  void* dg; void* du; int64_t Hp;                // [T][Hp] dg and du
   float* dbpart;                                 // [row tiles][2][H] column sums, or null
   int tm, tn;
   void* kept;                                    // forward: [T][Hp / 4] times p and s of four columns
@@ -414,13 +241,13 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
   const int n0 = tn * BN;
   typename Cr::Acc acc;
   Cr::zero(acc);
-  const Operand A = {a.x + m0 * a.ldx, a.xlimb, a.ldx, a.T - m0, a.K};
-  const Operand B[2] = {{a.wg + (int64_t)n0 * a.ldwg, a.wlimb, a.ldwg, a.H - n0, a.K}, {a.wu + (int64_t)n0 * a.ldwu, a.wlimb, a.ldwu, a.H - n0, a.K}};
+  const Operand A = {element<MODE>(a.x, m0 * a.ldx), 0, a.ldx, a.T - m0, a.K};
+  const Operand B[2] = {{element<MODE>(a.wg, (int64_t)n0 * a.ldwg), 0, a.ldwg, a.H - n0, a.K},
+                        {element<MODE>(a.wu, (int64_t)n0 * a.ldwu), 0, a.ldwu, a.H - n0, a.K}};
   if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
   else Cr::run(smem, A, B, acc);
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  const int shift = MODE == MODE_F16X3 && BWD ? a.exps[6] - a.exps[5] : 0;
   float* sums = (float*)smem;  // [WM][2][BN]
   f32x4 dhs[BWD ? Cr::NI : 1][BWD ? Cr::MI : 1];  // all of them requested before the first store
   if (BWD) {
@@ -433,13 +260,11 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
         dhs[BWD ? ni : 0][BWD ? mi : 0] = i < a.T && n > 0 ? load4<MODE>(a.dh, i * a.lddh + j, n) : f32x4{0.f, 0.f, 0.f, 0.f};
       }
   }
-  // Where much is kept the tiles of 256 rows, alone on their unit, send bf16's p and s or fp32's h (fp32's p and s are whole lines as they
-  // are) through LDS, half of each wave's rows at a time, so that whole lines leave: 16384 x 2048 -> 8192 in bf16 1300 -> 1064 us
-  // (916 with nothing kept), 16384 x 768 -> 4096 in fp32 690 -> 632 (538).  h alone is as fast from the registers.  16-byte chunks of a
-  // row are exchanged by its place among 16, which spreads a column's writes over the banks
-  constexpr bool STAGED = PHASED && KEEP;
-  constexpr bool CUT = KEEP && MODE == MODE_BF16, STAGED_H = STAGED && !CUT;
-  constexpr int ES = MODE == MODE_BF16 ? 2 : 4, HB = STAGED_H ? BN * ES : 0, PITCH = HB + (CUT ? BN * 6 : 0);
+  // Where much is kept the tiles of 256 rows, alone on their unit, send p and s through LDS, half of each wave's rows at a time, so that
+  // whole lines leave: 16384 x 2048 -> 8192 in bf16 1300 -> 1064 us (916 with nothing kept); h alone is as fast from the registers.
+  // 16-byte chunks of a row are exchanged by its place among 16, which spreads a column's writes over the banks
+  constexpr bool CUT = KEEP && MODE == MODE_BF16, STAGED = PHASED && CUT;
+  constexpr int PITCH = CUT ? BN * 6 : 0;
   constexpr int PARTS = STAGED ? 2 : 1, MH = Cr::MI / PARTS, ROWS = WM * MH * 16;
   static_assert(!STAGED || (ROWS * PITCH <= Cr::LDS && PITCH % 256 == 0), "the rows of a part fit");
   auto place = [&](int row, int byte) { return smem + row * PITCH + (byte ^ (row & 15) << 4); };
@@ -452,48 +277,29 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
     f32x4 bg = {0.f, 0.f, 0.f, 0.f}, bu = {0.f, 0.f, 0.f, 0.f};
     if (a.bg && n > 0) bg = load4<MODE>(a.bg, j, n);
     if (a.bu && n > 0) bu = load4<MODE>(a.bu, j, n);
-    int eg[4] = {0, 0, 0, 0}, eu[4] = {0, 0, 0, 0};
-    if (MODE == MODE_F16X3 && n > 0) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {  // [2][Hp]: four entries are inside
-        eg[r] = a.colexp[j + r] - 15;
-        eu[r] = a.colexp[a.Hp + j + r] - 15;
-      }
-    }
     f32x4 sg = {0.f, 0.f, 0.f, 0.f}, su = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int mi = part * MH; mi < (part + 1) * MH; ++mi) {
       const int64_t i = m0 + wm * (BM / WM) + 16 * mi + (lane & 15);
       const bool row = i < a.T;
-      f32x4 g = acc[0][mi][ni], u = acc[1][mi][ni];
-      if (MODE == MODE_F16X3) {
-        const int e = row ? a.rowexp[i] : NONE, ex = e == NONE ? 0 : e - 15;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          g[r] = ldexpf(g[r], ex + eg[r]);
-          u[r] = ldexpf(u[r], ex + eu[r]);
-        }
-      }
-      g += bg;
-      u += bu;
+      const f32x4 g = acc[0][mi][ni] + bg, u = acc[1][mi][ni] + bu;
       if (!BWD) {
         f32x4 h, p, z;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float s, d;
-          activate<KEEP, MODE == MODE_F16X3>(a.act, g[r], s, d);
+          activate<KEEP, MODE == MODE_F32>(a.act, g[r], s, d);
           h[r] = s * u[r];
           if (KEEP) { p[r] = d * u[r]; z[r] = s; }
         }
         if (row && n > 0) {
           const int q = wm * MH * 16 + 16 * (mi - part * MH) + (lane & 15);
-          if (STAGED_H) store4<MODE>(place(q, jt * ES), 0, 4, h);
-          else store4<MODE>(a.h, i * a.ldh + j, n, h);
+          store4<MODE>(a.h, i * a.ldh + j, n, h);
           if constexpr (CUT) {
             u32x2 w[3];
             cut(p, z, w);
 #pragma unroll
-            for (int r = 0; r < 3; ++r) *(u32x2*)(STAGED ? place(q, HB + jt * 6 + 8 * r) : (char*)a.kept + (i * a.Hp + j) * 6 + 8 * r) = w[r];
+            for (int r = 0; r < 3; ++r) *(u32x2*)(STAGED ? place(q, jt * 6 + 8 * r) : (char*)a.kept + (i * a.Hp + j) * 6 + 8 * r) = w[r];
           } else if constexpr (KEEP) {
             float* o = (float*)a.kept + (i * a.Hp + j) * 2;
             *(f32x4*)o = p;
@@ -507,7 +313,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             float s, d;
-            activate<true, MODE == MODE_F16X3>(a.act, g[r], s, d);
+            activate<true, MODE == MODE_F32>(a.act, g[r], s, d);
             dg[r] = r < n ? dh[r] * u[r] * d : 0.f;
             du[r] = r < n ? dh[r] * s : 0.f;
           }
@@ -516,23 +322,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
         su += du;
         if (row && j < a.Hp) {  // Hp is a multiple of 8: all four columns are inside, the ones behind H as zeros
           const int64_t o = i * a.Hp + j;
-          if (MODE == MODE_BF16) {
-            store4<MODE>(a.dg, o, 4, dg);
-            store4<MODE>(a.du, o, 4, du);
-          } else {
-            const int k = a.rscale[i] == NONE ? 0 : a.rscale[i], ku = a.rscale[i] == NONE ? 0 : k + shift;
-            uint16_t hg[4], lg[4], hu[4], lu[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const Split x = split16(ldexpf(dg[r], k)), y = split16(ldexpf(du[r], ku));
-              hg[r] = x.hi; lg[r] = x.lo; hu[r] = y.hi; lu[r] = y.lo;
-            }
-            auto pack = [](const uint16_t (&v)[4]) { return u32x2{v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16}; };
-            *(u32x2*)(a.dg + o) = pack(hg);
-            *(u32x2*)(a.dg + a.dlimb + o) = pack(lg);
-            *(u32x2*)(a.du + o) = pack(hu);
-            *(u32x2*)(a.du + a.dlimb + o) = pack(lu);
-          }
+          store4<MODE>(a.dg, o, 4, dg);
+          store4<MODE>(a.du, o, 4, du);
         }
       }
     }
@@ -552,28 +343,12 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_mma_kernel(MmaArgs a) {
   }
   if (STAGED) {
     __syncthreads();
-    for (int e = threadIdx.x; e < ROWS * PITCH / 16; e += 64 * WM * WN) {
-      const int q = e / (PITCH / 16), c = e % (PITCH / 16) * 16;
+    constexpr int CHUNKS = STAGED ? PITCH / 16 : 1;
+    for (int e = threadIdx.x; e < ROWS * CHUNKS; e += 64 * WM * WN) {
+      const int q = e / CHUNKS, c = e % CHUNKS * 16;
       const int64_t i = m0 + q / (MH * 16) * (BM / WM) + part * MH * 16 + q % (MH * 16);
       if (i >= a.T) continue;
-      const u32x4 w = *(const u32x4*)place(q, c);
-      if (c >= HB) {
-        if (n0 * 6 + c - HB < a.Hp * 6) *(u32x4*)((char*)a.kept + (i * a.Hp + n0) * 6 + c - HB) = w;
-      } else {
-        const int j = n0 + c / ES;
-        char* o = (char*)a.h + (i * a.ldh + j) * ES;
-        if (a.H - j >= 16 / ES) {
-          __builtin_memcpy(o, &w, 16);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16 / ES; ++r) {
-            const uint32_t v = w[r * ES / 4];
-            if (j + r >= a.H) continue;
-            if (ES == 4) ((uint32_t*)o)[r] = v;
-            else ((uint16_t*)o)[r] = (uint16_t)(v >> 16 * (r & 1));
-          }
-        }
-      }
+      if (n0 * 6 + c < a.Hp * 6) *(u32x4*)((char*)a.kept + (i * a.Hp + n0) * 6 + c) = *(const u32x4*)place(q, c);
     }
   }
   }
@@ -598,8 +373,7 @@ constexpr int KEPT_ROWS = 64;
 struct KeptArgs {
   const void* kept; const void* dh; int64_t lddh;
   int64_t T; int H; int64_t Hp;
-  uint16_t* dg; uint16_t* du; int64_t dlimb;
-  const int* rscale; const int* exps;
+  void* dg; void* du;
   float* dbpart;
   int cols;  // blocks side by side
 };
@@ -609,7 +383,6 @@ __global__ __launch_bounds__(256) void gated_kept_kernel(KeptArgs a) {
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), tile = blockIdx.x / a.cols, j = (blockIdx.x % a.cols * 64 + lane) * 8;
   const int64_t i0 = (int64_t)tile * KEPT_ROWS + wave;
   const int n = a.H - j;
-  const int shift = MODE == MODE_F16X3 ? a.exps[6] - a.exps[5] : 0;
   __shared__ __align__(16) float sums[2][4][512];
   float sg[8], su[8];
 #pragma unroll
@@ -653,27 +426,8 @@ __global__ __launch_bounds__(256) void gated_kept_kernel(KeptArgs a) {
           su[r] += du[r];
         }
         const int64_t o = i * a.Hp + j;
-        auto put = [&](uint16_t* to, const uint16_t (&v)[8]) {
-          *(u32x4*)(to + o) = u32x4{v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16};
-        };
-        uint16_t g0[8], u0[8], g1[8], u1[8];
-        const int e = MODE == MODE_F16X3 ? a.rscale[i] : 0, eg = e == NONE ? 0 : e, eu = e == NONE ? 0 : e + shift;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          if constexpr (MODE == MODE_BF16) {
-            g0[r] = bf16_bits(dg[r]);
-            u0[r] = bf16_bits(du[r]);
-          } else {
-            const Split x = split16(ldexpf(dg[r], eg)), y = split16(ldexpf(du[r], eu));
-            g0[r] = x.hi; g1[r] = x.lo; u0[r] = y.hi; u1[r] = y.lo;
-          }
-        }
-        put(a.dg, g0);
-        put(a.du, u0);
-        if constexpr (MODE != MODE_BF16) {
-          put(a.dg + a.dlimb, g1);
-          put(a.du + a.dlimb, u1);
-        }
+        store8<MODE>(a.dg, o, dg);
+        store8<MODE>(a.du, o, du);
       }
     }
   if (a.dbpart) {  // the four waves' rows
@@ -692,13 +446,11 @@ __global__ __launch_bounds__(256) void gated_kept_kernel(KeptArgs a) {
   }
 }
 
-// ---- short rows: D <= 256 ------------------------------------------------------------------------------------------------------------------
-// With a sum this short a tile is mostly its start and its end, and the limbs' way through memory costs as much as the layer.  So: a block
-// keeps 64 columns of both weight matrices in LDS for its whole life, as fragments in the order of their reads, and its eight waves run
-// over rows without meeting again: a wave loads 16 MI whole rows as they are (128 bytes of a row at a time), finds their scales and splits
-// them in registers, multiplies, and stores.  One launch, x read once a panel, nothing written but the result.
-// 131072 x 256 -> 256 in fp32: packing and tiles 177 us, this 124: 278 TFLOP/s (three products a term) and
-// 2.2 TB/s, neither near its bound -- a wave's splits, products and activations take turns, and two waves share a SIMD.
+// ---- short rows in bf16: D <= 256 ----------------------------------------------------------------------------------------------------------
+// With a sum this short a tile is mostly its start and its end.  So: a block keeps 64 columns of both weight matrices in LDS for its whole
+// life, as fragments in the order of their reads, and its eight waves run over rows without meeting again: a wave loads 16 MI whole rows as
+// they are (128 bytes of a row at a time), multiplies, and stores.  One launch, x read once a panel, nothing written but the result.
+// (In fp32 the matrix instructions take sixteen times as long, and the tiles' start and end are nothing beside them.)
 constexpr int PANEL = 64, SHORT_WAVES = 8, SHORT_ROW = 256;
 
 struct ShortArgs {
@@ -709,63 +461,25 @@ struct ShortArgs {
   int D, H, act, panels, parts;
   void* h; int64_t ldh;      // forward
   const void* dh; int64_t lddh;  // backward, as MmaArgs
-  uint16_t* dg; uint16_t* du; int64_t Hp, dlimb;
-  const int* rscale; const int* exps;
+  void* dg; void* du; int64_t Hp;
   float* dbpart;             // [parts waves][2][H], or null
 };
 
-// 16 rows x 32 KS of k as fragments: a lane holds row lane % 16 (clamped to the last), 8 k's of every 32.  fp32: scaled to [2^14, 2^15), `e` = the
-// row's exponent, limbs; the largest magnitude ignores NaN, and a row with an infinity, scaled by 1, keeps infinities or NaN
+// 16 rows x 32 KS of k as fragments: a lane holds row lane % 16 (clamped to the last), 8 k's of every 32
 // FULL: D = 32 KS, no chunk ends inside a row
-template <int MODE, int KS, bool FULL>
-__device__ __forceinline__ void short_rows(const void* p, int64_t ld, int64_t row, int64_t rows, int D, s16x8 (&f)[KS][limbs<MODE>()], int& e) {
+template <int KS, bool FULL>
+__device__ __forceinline__ void short_rows(const void* p, int64_t ld, int64_t row, int64_t rows, int D, s16x8 (&f)[KS]) {
   const int lane = threadIdx.x & 63, kl = 8 * (lane >> 4);
   int64_t r = row + (lane & 15);
   r = r < rows ? r : rows - 1;
-  if constexpr (MODE == MODE_BF16) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) f[k][0] = __builtin_bit_cast(s16x8, chunk16<MODE_BF16>(p, r * ld, 32 * k + kl, FULL ? 32 * KS + 8 : D));
-    e = 0;
-  } else {
-    u32x4 v[KS][2];
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int q = 0; q < 2; ++q) v[k][q] = chunk16<MODE_F16X3>(p, r * ld, 32 * k + kl + 4 * q, FULL ? 32 * KS + 8 : D);
-    float m = 0.f;
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m = fmaxf(m, fabsf(lane_value<MODE_F16X3>(v[k][q], i)));
-    m = fmaxf(m, __shfl_xor(m, 16, 64));
-    m = fmaxf(m, __shfl_xor(m, 32, 64));
-    e = m > 0.f && m < __builtin_inff() ? exp_above(m) : 15;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      u32x4 hi, lo;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float a = ldexpf(lane_value<MODE_F16X3>(v[k][q >> 1], 2 * (q & 1)), 15 - e), b = ldexpf(lane_value<MODE_F16X3>(v[k][q >> 1], 2 * (q & 1) + 1), 15 - e);
-        typedef float f32x2 __attribute__((ext_vector_type(2)));
-        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-        const f16x2 h = __builtin_convertvector(f32x2{a, b}, f16x2);
-        const f16x2 l = __builtin_convertvector(f32x2{a - (float)h[0], b - (float)h[1]}, f16x2);
-        hi[q] = __builtin_bit_cast(uint32_t, h);
-        lo[q] = __builtin_bit_cast(uint32_t, l);
-      }
-      f[k][0] = __builtin_bit_cast(s16x8, hi);
-      f[k][1] = __builtin_bit_cast(s16x8, lo);
-    }
-  }
+  for (int k = 0; k < KS; ++k) f[k] = __builtin_bit_cast(s16x8, chunk16<MODE_BF16>(p, r * ld, 32 * k + kl, FULL ? 32 * KS + 8 : D));
 }
 
-template <int MODE, bool BWD, int KS, int MI, bool FULL>
+template <bool BWD, int KS, int MI, bool FULL>
 __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs a) {
-  constexpr int NL = limbs<MODE>(), NF = PANEL / 16;
-  __shared__ __align__(16) s16x8 panel[KS][2 * NF][NL][64];
-  __shared__ __align__(16) int colexp[2][PANEL];
+  constexpr int NF = PANEL / 16;
+  __shared__ __align__(16) s16x8 panel[KS][2 * NF][64];
   __shared__ __align__(16) float bias[2][PANEL];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   // all panels of a part's rows on one XCD (blocks go to the XCDs in turn): its L2 serves the rows after the first
@@ -775,17 +489,13 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
   const int n0 = pan * PANEL;
   {  // a wave: 16 columns of one of the matrices
     const int w = wave / NF, q = wave % NF;
-    s16x8 f[KS][NL];
-    int e;
-    short_rows<MODE, KS, FULL>(a.w[w], a.ldw[w], n0 + 16 * q, a.H, a.D, f, e);
+    s16x8 f[KS];
+    short_rows<KS, FULL>(a.w[w], a.ldw[w], n0 + 16 * q, a.H, a.D, f);
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int l = 0; l < NL; ++l) panel[k][wave][l][lane] = f[k][l];
+    for (int k = 0; k < KS; ++k) panel[k][wave][lane] = f[k];
     if (lane < 16) {
       const int j = n0 + 16 * q + lane;
-      colexp[w][16 * q + lane] = e - 15;
-      bias[w][16 * q + lane] = a.b[w] && j < a.H ? load1<MODE>(a.b[w], j) : 0.f;
+      bias[w][16 * q + lane] = a.b[w] && j < a.H ? load1<MODE_BF16>(a.b[w], j) : 0.f;
     }
   }
   static_assert(SHORT_WAVES == 2 * NF, "a wave for each 16 columns of the panel");
@@ -796,18 +506,15 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
   for (int w = 0; w < 2; ++w)
 #pragma unroll
     for (int f = 0; f < (BWD ? NF : 1); ++f) sum[w][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int shift = MODE == MODE_F16X3 && BWD ? a.exps[6] - a.exps[5] : 0;
   const int64_t begin = part * a.chunk, end = begin + a.chunk < a.T ? begin + a.chunk : a.T;
   for (int64_t row = begin + wave * 16 * MI; row < end; row += SHORT_WAVES * 16 * MI) {
-    s16x8 x[MI][KS][NL];
-    int ex[MI];
+    s16x8 x[MI][KS];
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
-      short_rows<MODE, KS, FULL>(a.x, a.ldx, row + 16 * m, a.T, a.D, x[m], ex[m]);
+      short_rows<KS, FULL>(a.x, a.ldx, row + 16 * m, a.T, a.D, x[m]);
       __builtin_amdgcn_sched_barrier(0);
     }
     f32x4 dhs[MI][BWD ? NF : 1];  // on their way while the products run
-    int rs[MI];
     if (BWD) {
 #pragma unroll
       for (int m = 0; m < MI; ++m) {
@@ -815,9 +522,8 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
           const int j = n0 + 16 * f + jl;
-          dhs[m][BWD ? f : 0] = i < a.T && j < a.H ? load4<MODE>(a.dh, i * a.lddh + j, a.H - j) : f32x4{0.f, 0.f, 0.f, 0.f};
+          dhs[m][BWD ? f : 0] = i < a.T && j < a.H ? load4<MODE_BF16>(a.dh, i * a.lddh + j, a.H - j) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        rs[m] = MODE == MODE_F16X3 ? (i < a.T ? a.rscale[i] : NONE) : 0;
       }
     }
     f32x4 acc[2][MI][NF];
@@ -833,17 +539,13 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         __builtin_amdgcn_sched_barrier(0);  // and read a matrix at a time
-        s16x8 b[NF][NL];
+        s16x8 b[NF];
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
+        for (int f = 0; f < NF; ++f) b[f] = panel[k][w * NF + f][lane];
 #pragma unroll
-          for (int l = 0; l < NL; ++l) b[f][l] = panel[k][w * NF + f][l][lane];
+        for (int m = 0; m < MI; ++m)
 #pragma unroll
-        for (int p = NL == 2 ? 0 : 2; p < 3; ++p)
-#pragma unroll
-          for (int m = 0; m < MI; ++m)
-#pragma unroll
-            for (int f = 0; f < NF; ++f) acc[w][m][f] = mfma<MODE>(b[f][p == 0 ? NL - 1 : 0], x[m][k][p == 1 ? NL - 1 : 0], acc[w][m][f]);
+          for (int f = 0; f < NF; ++f) acc[w][m][f] = mfma<MODE_BF16>(b[f], x[m][k], acc[w][m][f]);
       }
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
@@ -852,31 +554,23 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
         const int j = n0 + 16 * f + jl, n = a.H - j;
-        f32x4 g = acc[0][m][f], u = acc[1][m][f];
-        if (MODE == MODE_F16X3) {
-          const int4 cg = *(const int4*)&colexp[0][16 * f + jl], cu = *(const int4*)&colexp[1][16 * f + jl];
-          const int e0 = ex[m] - 15;
-          g = f32x4{ldexpf(g[0], e0 + cg.x), ldexpf(g[1], e0 + cg.y), ldexpf(g[2], e0 + cg.z), ldexpf(g[3], e0 + cg.w)};
-          u = f32x4{ldexpf(u[0], e0 + cu.x), ldexpf(u[1], e0 + cu.y), ldexpf(u[2], e0 + cu.z), ldexpf(u[3], e0 + cu.w)};
-        }
-        g += *(const f32x4*)&bias[0][16 * f + jl];
-        u += *(const f32x4*)&bias[1][16 * f + jl];
+        const f32x4 g = acc[0][m][f] + *(const f32x4*)&bias[0][16 * f + jl], u = acc[1][m][f] + *(const f32x4*)&bias[1][16 * f + jl];
         if (!BWD) {
           f32x4 h;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             float s, d;
-            activate<false, MODE == MODE_F16X3>(a.act, g[r], s, d);
+            activate<false, false>(a.act, g[r], s, d);
             h[r] = s * u[r];
           }
-          if (live && n > 0) store4<MODE>(a.h, i * a.ldh + j, n, h);
+          if (live && n > 0) store4<MODE_BF16>(a.h, i * a.ldh + j, n, h);
         } else {
           f32x4 dg = {0.f, 0.f, 0.f, 0.f}, du = dg;
           if (live) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               float s, d;
-              activate<true, MODE == MODE_F16X3>(a.act, g[r], s, d);
+              activate<true, false>(a.act, g[r], s, d);
               if (r < n) {
                 dg[r] = dhs[m][BWD ? f : 0][r] * u[r] * d;
                 du[r] = dhs[m][BWD ? f : 0][r] * s;
@@ -887,13 +581,8 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
           sum[1][BWD ? f : 0] += du;
           if (live && j < a.Hp) {  // as the tiles' epilogue
             const int64_t o = i * a.Hp + j;
-            if (MODE == MODE_BF16) {
-              store4<MODE>(a.dg, o, 4, dg);
-              store4<MODE>(a.du, o, 4, du);
-            } else {
-              put_limbs(a.dg + o, a.dlimb, dg, rs[m] == NONE ? 0 : rs[m]);
-              put_limbs(a.du + o, a.dlimb, du, rs[m] == NONE ? 0 : rs[m] + shift);
-            }
+            store4<MODE_BF16>(a.dg, o, 4, dg);
+            store4<MODE_BF16>(a.du, o, 4, du);
           }
         }
       }
@@ -910,17 +599,16 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
 #pragma unroll
           for (int o = 1; o < 16; o <<= 1) v[r] += __shfl_xor(v[r], o, 64);
         const int j = n0 + 16 * f + jl;
-        if ((lane & 15) == 0 && j < a.H) store4<MODE_F16X3>(a.dbpart, (((int64_t)part * SHORT_WAVES + wave) * 2 + w) * a.H + j, a.H - j, v);
+        if ((lane & 15) == 0 && j < a.H) store4<MODE_F32>(a.dbpart, (((int64_t)part * SHORT_WAVES + wave) * 2 + w) * a.H + j, a.H - j, v);
       }
   }
 }
 
 // ---- dx = dg Wg + du Wu -----------------------------------------------------------------------------------------------------------------
 struct DxArgs {
-  const uint16_t* dg; const uint16_t* du; int64_t Hp, dlimb;
-  const uint16_t* wg; const uint16_t* wu; int64_t ldwg, ldwu, wlimb;
+  const void* dg; const void* du; int64_t Hp;
+  const void* wg; const void* wu; int64_t ldwg, ldwu;
   int64_t T; int H, D;
-  const int* rscale; const int* exps;
   void* dx;
   int64_t chunk; int splits;  // the sum over H is split, `chunk` each
   float* part;                // [split][T][D], where splits > 1
@@ -938,43 +626,37 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dx_kernel(DxArgs a) {
   const int n0 = tn * BN;
   typename Cr::Acc acc;
   Cr::zero(acc);
-  const int64_t cols = (a.D + 7) / 8 * 8 - n0;
+  const int64_t cols = (a.D + chunk_k<MODE>() - 1) / chunk_k<MODE>() * chunk_k<MODE>() - n0;
 #pragma unroll 1
   for (int up = 0; up < 2; ++up) {
     const int64_t ld = up ? a.ldwu : a.ldwg;
-    const Operand A = {(up ? a.du : a.dg) + m0 * a.Hp + k0, a.dlimb, a.Hp, a.T - m0, ka};
-    const Operand B[1] = {{(up ? a.wu : a.wg) + k0 * ld + n0, a.wlimb, ld, cols, kb}};
+    const Operand A = {element<MODE>(up ? a.du : a.dg, m0 * a.Hp + k0), 0, a.Hp, a.T - m0, ka};
+    const Operand B[1] = {{element<MODE>(up ? a.wu : a.wg, k0 * ld + n0), 0, ld, cols, kb}};
     if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
     else Cr::run(smem, A, B, acc);
   }
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  const int ew = MODE == MODE_F16X3 ? a.exps[5] - 15 : 0;
 #pragma unroll
   for (int mi = 0; mi < Cr::MI; ++mi) {
     const int64_t i = m0 + wm * (BM / WM) + 16 * mi + (lane & 15);
     if (i >= a.T) continue;
-    const int k = MODE == MODE_F16X3 ? (a.rscale[i] == NONE ? ew : ew - a.rscale[i]) : 0;
 #pragma unroll
     for (int ni = 0; ni < Cr::NI; ++ni) {
       const int j = n0 + wn * (BN / WN) + 16 * ni + 4 * (lane >> 4);
-      f32x4 v = acc[0][mi][ni];
-      if (MODE == MODE_F16X3)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], k);
+      const f32x4 v = acc[0][mi][ni];
       if (j >= a.D) continue;
       if (a.splits == 1) store4<MODE>(a.dx, i * a.D + j, a.D - j, v);
-      else store4<MODE_F16X3>(a.part, (sp * a.T + i) * a.D + j, a.D - j, v);
+      else store4<MODE_F32>(a.part, (sp * a.T + i) * a.D + j, a.D - j, v);
     }
   }
 }
 
 // ---- dWg = dg^T x, dWu = du^T x -----------------------------------------------------------------------------------------------------------
 struct DwArgs {
-  const uint16_t* d[2]; int64_t Hp, dlimb;
-  const uint16_t* x; int64_t ldx, xlimb;
+  const void* d[2]; int64_t Hp;
+  const void* x; int64_t ldx;
   int64_t T; int H, D;
   int64_t chunk; int splits;
-  const int* exps;
   void* out[2];   // the results, where splits == 1
   float* part;    // [split][2][H][D], elsewhere
   int tm, tn;
@@ -991,12 +673,11 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dw_kernel(DwArgs a) {
   const int64_t t0 = (int64_t)sp * a.chunk, K = a.T - t0 < a.chunk ? a.T - t0 : a.chunk;
   typename Cr::Acc acc;
   Cr::zero(acc);
-  const Operand A = {a.d[w] + t0 * a.Hp + m0, a.dlimb, a.Hp, a.Hp - m0, K};
-  const Operand B[1] = {{a.x + t0 * a.ldx + n0, a.xlimb, a.ldx, (a.D + 7) / 8 * 8 - n0, K}};
+  const Operand A = {element<MODE>(a.d[w], t0 * a.Hp + m0), 0, a.Hp, a.Hp - m0, K};
+  const Operand B[1] = {{element<MODE>(a.x, t0 * a.ldx + n0), 0, a.ldx, (a.D + chunk_k<MODE>() - 1) / chunk_k<MODE>() * chunk_k<MODE>() - n0, K}};
   if constexpr (PHASED) Cr::run_phased(smem, A, B, acc);
   else Cr::run(smem, A, B, acc);
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-  const int e = MODE == MODE_F16X3 ? -a.exps[4] - (w ? a.exps[6] - a.exps[5] : 0) : 0;
 #pragma unroll
   for (int mi = 0; mi < Cr::MI; ++mi) {
     const int i = m0 + wm * (BM / WM) + 16 * mi + (lane & 15);
@@ -1005,12 +686,9 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dw_kernel(DwArgs a) {
     for (int ni = 0; ni < Cr::NI; ++ni) {
       const int j = n0 + wn * (BN / WN) + 16 * ni + 4 * (lane >> 4);
       if (j >= a.D) continue;
-      f32x4 v = acc[0][mi][ni];
-      if (MODE == MODE_F16X3)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], e);
+      const f32x4 v = acc[0][mi][ni];
       if (a.splits == 1) store4<MODE>(a.out[w], (int64_t)i * a.D + j, a.D - j, v);
-      else store4<MODE_F16X3>(a.part, (((int64_t)sp * 2 + w) * a.H + i) * a.D + j, a.D - j, v);
+      else store4<MODE_F32>(a.part, (((int64_t)sp * 2 + w) * a.H + i) * a.D + j, a.D - j, v);
     }
   }
 }
@@ -1051,12 +729,12 @@ __global__ __launch_bounds__(256) void gated_finish_kernel(FinishArgs a) {
   const int m = n - i < 4 ? (int)(n - i) : 4;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < a.splits[r]; ++s) v += load4<MODE_F16X3>(a.part[r], ((int64_t)s * a.sets[r] + w) * n + i, m);
+  for (int s = 0; s < a.splits[r]; ++s) v += load4<MODE_F32>(a.part[r], ((int64_t)s * a.sets[r] + w) * n + i, m);
   store4<MODE>(a.out[r][w], i, m, v);
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------
-// T <= 64: bound by the weights' bytes, which are read once, 16 a lane, as they are; no product of limbs, fp32 keeps fp32 arithmetic.
+// T <= 64: bound by the weights' bytes, which are read once, 16 a lane, as they are.
 constexpr int ROWS_MAX = 64;
 struct RowsArgs {
   const void* x; int64_t ldx;
@@ -1118,7 +796,7 @@ __global__ __launch_bounds__(256) void gated_rows_kernel(RowsArgs a) {
     if (a.b[0]) g += load1<MODE>(a.b[0], j);
     if (a.b[1]) u += load1<MODE>(a.b[1], j);
     float f, d;
-    activate<false, MODE == MODE_F16X3>(a.act, g, f, d);
+    activate<false, MODE == MODE_F32>(a.act, g, f, d);
     store1<MODE>(a.h, t * a.ldh + j, f * u);
   }
 }
@@ -1183,7 +861,7 @@ __global__ __launch_bounds__(256) void gated_few_kernel(RowsArgs a) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       float f, d;
-      activate<false, MODE == MODE_F16X3>(a.act, acc[0][n][q], f, d);
+      activate<false, MODE == MODE_F32>(a.act, acc[0][n][q], f, d);
       h[q] = f * acc[1][n][q];
     }
     if (t < a.T) store4<MODE>(a.h, t * a.ldh + j, n4, h);
@@ -1197,9 +875,9 @@ inline int64_t rows_grid(int64_t rows, int64_t most = 2048) {  // a row a wave; 
   return b < 1 ? 1 : (b > most ? most : b);
 }
 
-// Tiles of 256 rows, one block a compute unit, or of 128, two a unit: by the time of the launch in rounds over the 256 units.  The small
-// tiles' lower rate (1135 against 1310 TFLOP/s at 4096^3, more LDS reads and loads a product) counts little against a part-filled round.
-// Sums of 5 to 16 steps: 65536 x 384 -> 512 in fp32 200 against 219 us, 65536 x 1024 -> 2048 in bf16 493 against 574.
+// (bf16) Tiles of 256 rows, one block a compute unit, or of 128, two a unit: by the time of the launch in rounds over the 256 units.  The
+// small tiles' lower rate (1135 against 1310 TFLOP/s at 4096^3, more LDS reads and loads a product) counts little against a part-filled
+// round.  65536 x 1024 -> 2048: 493 against 574 us.  In fp32 the matrix instructions bound the tiles of 128 already.
 bool large_tiles(int64_t n256, int64_t n128) {
   const double large = (double)((n256 + 255) / 256);
   double small = 0.58 * (double)((n128 + 511) / 512);
@@ -1215,9 +893,9 @@ struct Plan {
   bool copy_x, copy_w[2];
   bool brief, big, little, keep, dx_big, dw_big;  // brief: the kernel for short rows; big, little: tiles of 256 and of 64 rows
   int64_t parts, part_rows;
-  int64_t Dp, Hp, row_tiles, pack_blocks;
+  int64_t Dp, Hp, row_tiles;
   int64_t dx_splits, dx_chunk, dw_splits, dw_chunk;
-  int64_t x, w, dg, xt, part, exps, rowexp, colexp, rscale, dbpart, dx_sums, dw_sums, spart, bytes;
+  int64_t x, w, dg, dbpart, dx_sums, dw_sums, bytes;
 };
 
 bool aligned16(const void* p, int64_t ld, int es) { return (uintptr_t)p % 16 == 0 && (ld * es) % 16 == 0; }
@@ -1232,62 +910,55 @@ void split_sum(int64_t tiles, int64_t K, int64_t least, int64_t& splits, int64_t
 }
 
 // Whether the forward pass keeps u act'(g) and act(g) where a backward one may follow.  Whole steps, kept against computed again: fp32
-// 16384 x 768 -> 4096 2.35 against 3.0 ms, 65536 x 264 -> 512 0.94 against 1.03, in the kernel for short rows no less; bf16 16384 x
-// 2048 -> 8192 3.46 against 4.16 ms, 65536 x 640 -> 512 556 against 590 us, x 512 431 against 427; with less than some 2^21 values a step
-// is its launches (700 x 1024 -> 1024 in fp32: 165 against 161 us).  16384 x 8192 values are 0.8 GB in bf16, 1.1 in fp32
+// 16384 x 768 -> 4096 5.24 against 6.54 ms, 65536 x 288 -> 512 1.38 against 1.58, 65536 x 256 -> 512 0.98 against 1.15, x 128 -> 512 0.63
+// against 0.67; bf16 16384 x 2048 -> 8192 3.46 against 4.16 ms, 65536 x 640 -> 512 556 against 590 us, x 512 431 against 427; with less
+// than some 2^21 values a step is its launches (700 x 1024 -> 1024 in fp32: 192 against 192 us).  Up to 256 features and 2^23 values
+// the 8 bytes a value are not spent for the rest (70000 x 256 -> 48 in fp32: 239 against 264).  16384 x 8192 values are 0.8 GB in bf16, 1.1 in fp32
 bool keeps(const hold_gated_desc& d) {
-  return d.T > ROWS_MAX && d.T * d.H >= (1 << 21) && d.D > (d.dtype == HOLD_GATED_F32 ? SHORT_ROW : 512);
+  const int64_t n = d.T * d.H;
+  if (d.T <= ROWS_MAX || n < (1 << 21)) return false;
+  return d.dtype == HOLD_GATED_F32 ? d.D > 256 || (d.D > 128 && n >= (1 << 23)) : d.D > 512;
 }
 int64_t kept_bytes(const hold_gated_desc& d) { return d.T * up(d.H, 8) * (d.dtype == HOLD_GATED_F32 ? 8 : 6); }
 
 Plan plan(const hold_gated_desc& d, bool bwd) {
   Plan p = {};
   const bool f32 = d.dtype == HOLD_GATED_F32;
-  const int nl = f32 ? 2 : 1, step = f32 ? 32 : 64;
-  p.Dp = up(d.D, 8);
+  const int es = f32 ? 4 : 2, step = f32 ? 32 : 64, whole = 16 / es;
+  p.Dp = up(d.D, whole);
   p.Hp = up(d.H, 8);
-  p.copy_x = f32 || d.D % 8 || !aligned16(d.x, d.ldx, 2);
-  p.copy_w[0] = f32 || d.D % 8 || !aligned16(d.w_gate, d.ldwg, 2);
-  p.copy_w[1] = f32 || d.D % 8 || !aligned16(d.w_up, d.ldwu, 2);
+  p.copy_x = d.D % whole || !aligned16(d.x, d.ldx, es);
+  p.copy_w[0] = d.D % whole || !aligned16(d.w_gate, d.ldwg, es);
+  p.copy_w[1] = d.D % whole || !aligned16(d.w_up, d.ldwu, es);
   int64_t o = 0;
   auto take = [&](int64_t bytes) { const int64_t at = o; o += up(bytes, 256); return at; };
-  p.brief = d.D <= SHORT_ROW;
+  p.brief = !f32 && d.D <= SHORT_ROW;
   // some 256 blocks; a part's rows are whole rounds of its waves, and all panels of a part go to one XCD where the parts divide
   const int64_t panels = cdiv(d.H, PANEL), round = SHORT_WAVES * 16 * (bwd ? 1 : 2), rounds = cdiv(d.T, round);
   int64_t parts = cdiv(256, panels);
   parts = parts > rounds ? rounds : parts >= 8 ? (parts + 7) / 8 * 8 : parts;
   p.part_rows = cdiv(rounds, parts) * round;
   p.parts = cdiv(d.T, p.part_rows);
-  p.big = !bwd && large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64));
+  p.big = !f32 && !bwd && large_tiles(cdiv(d.T, 256) * cdiv(d.H, 128), cdiv(d.T, 128) * cdiv(d.H, 64));
   // (backward: only for what is not kept, sums or results too short for large tiles)
   // up to half a block a unit of 128 x (64 + 64): tiles a quarter of that, four stages deep, their loads three steps ahead (2019 x 2816 ->
-  // 32 in fp32: 80.9 -> 57.0 us; 1000 x 1000 -> 1000, 128 blocks: 39 -> 32, in bf16 17 -> 13; 2000 x 700 -> 600, 160: 25 against 32)
+  // 32 in fp32: 180 -> 100 us; 1000 x 1000 -> 1000, 128 blocks: 72 -> 46, in bf16 17 -> 13; 2000 x 700 -> 600, 160: fp32 59 against 67, bf16
+  // 25 against 32)
   p.little = !p.big && cdiv(d.T, 128) * cdiv(d.H, 64) <= 128;
   p.keep = d.kept != nullptr;
   p.row_tiles = p.keep ? cdiv(d.T, KEPT_ROWS) : p.brief ? p.parts * SHORT_WAVES : cdiv(d.T, p.big ? 256 : p.little ? 64 : 128);
-  p.pack_blocks = rows_grid(d.T + 2 * (int64_t)d.H, 4096);
   if (p.brief && !bwd) return p;  // takes everything as it is
-  p.x = p.copy_x && !(f32 && (p.brief || (p.keep && bwd))) ? take(d.T * p.Dp * 2 * nl) : 0;
-  p.w = p.copy_w[0] || p.copy_w[1] ? take(2 * (int64_t)d.H * p.Dp * 2 * nl) : 0;
-  if (f32) {
-    p.rowexp = take(d.T * 4);
-    p.colexp = take(2 * p.Hp * 4);
-  }
+  p.x = p.copy_x ? take(d.T * p.Dp * es) : 0;
+  // (fp32 rows beyond the short ones: room for the weights' copies in any case, so that a call with weights of other strides finds it too)
+  p.w = p.copy_w[0] || p.copy_w[1] || (f32 && d.D > SHORT_ROW) ? take(2 * (int64_t)d.H * p.Dp * es) : 0;
   if (bwd) {
-    p.dg = take(2 * d.T * p.Hp * 2 * nl);
-    if (f32) {
-      p.part = take(4 * NPART * 4);
-      p.exps = take(8 * 4);
-      p.xt = take(d.T * p.Dp * 2 * nl);
-      p.rscale = take(d.T * 4);
-      p.spart = take(p.pack_blocks * 4);
-    }
+    p.dg = take(2 * d.T * p.Hp * es);
     if (d.db_gate || d.db_up) p.dbpart = take(p.row_tiles * 2 * d.H * 4);
     const int64_t x256 = cdiv(d.T, 256) * cdiv(d.D, 256), x128 = cdiv(d.T, 128) * cdiv(d.D, 128);
-    p.dx_big = x256 >= 150 && 2 * cdiv(p.Hp, step) > SHORT_SUM && large_tiles(x256, x128);
+    p.dx_big = !f32 && x256 >= 150 && 2 * cdiv(p.Hp, step) > SHORT_SUM && large_tiles(x256, x128);
     split_sum(p.dx_big ? 512 : x128, p.Hp, 512, p.dx_splits, p.dx_chunk);
     const int64_t w256 = 2 * cdiv(d.H, 256) * cdiv(d.D, 256), w128 = 2 * cdiv(d.H, 128) * cdiv(d.D, 128);
-    p.dw_big = w256 >= 200 && cdiv(d.T, step) > SHORT_SUM && large_tiles(w256, w128);
+    p.dw_big = !f32 && w256 >= 200 && cdiv(d.T, step) > SHORT_SUM && large_tiles(w256, w128);
     split_sum(p.dw_big ? 512 : w128, d.T, 512, p.dw_splits, p.dw_chunk);
     if (p.dx_splits > 1) p.dx_sums = take(p.dx_splits * d.T * d.D * 4);
     if (p.dw_splits > 1) p.dw_sums = take(p.dw_splits * 2 * (int64_t)d.H * d.D * 4);
@@ -1309,54 +980,32 @@ int check(const hold_gated_desc* d) {
   return HOLD_OK;
 }
 
-template <int MODE, bool BWD>
+template <int MODE>
 void operands(const hold_gated_desc& d, const Plan& p, char* ws, hipStream_t st, MmaArgs& a) {
-  const int64_t WX = d.T * p.Dp, WW = (int64_t)d.H * p.Dp;
-  a.x = (const uint16_t*)d.x; a.ldx = d.ldx; a.xlimb = 0;
-  a.wg = (const uint16_t*)d.w_gate; a.ldwg = d.ldwg;
-  a.wu = (const uint16_t*)d.w_up; a.ldwu = d.ldwu; a.wlimb = 0;
+  a.x = d.x; a.ldx = d.ldx;
+  a.wg = d.w_gate; a.ldwg = d.ldwg;
+  a.wu = d.w_up; a.ldwu = d.ldwu;
   a.Hp = p.Hp;
-  if (MODE == MODE_F16X3) {
-    PackArgs k = {};
-    k.x = (const float*)d.x; k.ldx = d.ldx; k.T = d.T;
-    k.w[0] = (const float*)d.w_gate; k.w[1] = (const float*)d.w_up; k.ldw[0] = d.ldwg; k.ldw[1] = d.ldwu;
-    k.H = d.H; k.D = d.D; k.Dp = (int)p.Dp;
-    k.ox = p.brief || (p.keep && BWD) ? nullptr : (uint16_t*)(ws + p.x); k.xlimb = WX;
-    k.ow = (uint16_t*)(ws + p.w); k.wlimb = 2 * WW; k.second = WW;
-    k.rowexp = (int*)(ws + p.rowexp); k.colexp = (int*)(ws + p.colexp); k.Hp = p.Hp;
-    if (BWD) {
-      float* part = (float*)(ws + p.part);
-      k.part = part; k.exps = (int*)(ws + p.exps);
-      k.dh = (const float*)d.dh; k.lddh = d.lddh; k.act = d.act;
-      k.rscale = (int*)(ws + p.rscale); k.rpart = (int*)(ws + p.spart);
-      hipLaunchKernelGGL(gated_amax_kernel, dim3(NPART, 4), dim3(256), 0, st, k.w[0], d.ldwg, k.w[1], d.ldwu, (const float*)d.b_gate,
-                         (const float*)d.b_up, d.H, d.D, part);
-      a.exps = k.exps;
-      a.rscale = k.rscale;
-    }
-    hipLaunchKernelGGL(gated_pack_kernel<BWD>, dim3((unsigned)p.pack_blocks), dim3(256), 0, st, k);
-    a.x = k.ox; a.ldx = p.Dp; a.xlimb = WX;
-    a.wg = k.ow; a.wu = k.ow + WW; a.ldwg = a.ldwu = p.Dp; a.wlimb = 2 * WW;
-    a.rowexp = k.rowexp; a.colexp = k.colexp;
-  } else if (p.copy_x || p.copy_w[0] || p.copy_w[1]) {
+  if (p.copy_x || p.copy_w[0] || p.copy_w[1]) {
     CopyArgs c = {};
     c.K = d.D; c.Kp = (int)p.Dp;
     int n = 0;
-    auto add = [&](const void* from, int64_t ld, int64_t rows, uint16_t* to) {
-      c.x[n] = (const uint16_t*)from; c.ld[n] = ld; c.rows[n] = rows; c.out[n] = to;
+    auto add = [&](const void*& from, int64_t& ld, int64_t rows, char* to) {
+      c.x[n] = from; c.ld[n] = ld; c.rows[n] = rows; c.out[n] = to;
+      from = to;
+      ld = p.Dp;
       ++n;
     };
-    uint16_t* w = (uint16_t*)(ws + p.w);
-    if (p.copy_x) { add(d.x, d.ldx, d.T, (uint16_t*)(ws + p.x)); a.x = c.out[n - 1]; a.ldx = p.Dp; }
-    if (p.copy_w[0]) { add(d.w_gate, d.ldwg, d.H, w); a.wg = w; a.ldwg = p.Dp; }
-    if (p.copy_w[1]) { add(d.w_up, d.ldwu, d.H, w + WW); a.wu = w + WW; a.ldwu = p.Dp; }
-    hipLaunchKernelGGL(gated_copy_rows_kernel, dim3((unsigned)rows_grid(c.rows[0] + c.rows[1] + c.rows[2])), dim3(256), 0, st, c);
+    if (p.copy_x) add(a.x, a.ldx, d.T, ws + p.x);
+    if (p.copy_w[0]) add(a.wg, a.ldwg, d.H, ws + p.w);
+    if (p.copy_w[1]) add(a.wu, a.ldwu, d.H, ws + p.w + (int64_t)d.H * p.Dp * 2 * halves<MODE>());
+    hipLaunchKernelGGL(gated_copy_rows_kernel<MODE>, dim3((unsigned)rows_grid(c.rows[0] + c.rows[1] + c.rows[2])), dim3(256), 0, st, c);
   }
   a.bg = d.b_gate; a.bu = d.b_up;
   a.T = d.T; a.H = d.H; a.K = (int)p.Dp; a.act = d.act;
 }
 
-template <int MODE, bool BWD>
+template <bool BWD>
 void launch_short(const hold_gated_desc& d, const MmaArgs& m, const Plan& p, hipStream_t st) {
   ShortArgs a = {};
   a.x = d.x; a.ldx = d.ldx;
@@ -1366,15 +1015,15 @@ void launch_short(const hold_gated_desc& d, const MmaArgs& m, const Plan& p, hip
   a.panels = (int)cdiv(d.H, PANEL); a.parts = (int)p.parts;
   a.h = m.h; a.ldh = m.ldh;
   a.dh = m.dh; a.lddh = m.lddh;
-  a.dg = m.dg; a.du = m.du; a.Hp = p.Hp; a.dlimb = m.dlimb;
-  a.rscale = m.rscale; a.exps = m.exps; a.dbpart = m.dbpart;
+  a.dg = m.dg; a.du = m.du; a.Hp = p.Hp;
+  a.dbpart = m.dbpart;
   const dim3 grid((unsigned)(a.panels * p.parts)), block(64 * SHORT_WAVES);
   constexpr int MI = BWD ? 1 : 2;
   const int ks = (d.D + 31) / 32;
   const bool full = d.D % 64 == 0;
 #define HOLD_SHORT(KS)                                                                                             \
-  if (full) hipLaunchKernelGGL((gated_short_kernel<MODE, BWD, KS, MI, true>), grid, block, 0, st, a);               \
-  else hipLaunchKernelGGL((gated_short_kernel<MODE, BWD, KS, MI, false>), grid, block, 0, st, a)
+  if (full) hipLaunchKernelGGL((gated_short_kernel<BWD, KS, MI, true>), grid, block, 0, st, a);               \
+  else hipLaunchKernelGGL((gated_short_kernel<BWD, KS, MI, false>), grid, block, 0, st, a)
   if (ks <= 2) { HOLD_SHORT(2); }
   else if (ks <= 4) { HOLD_SHORT(4); }
   else if (ks <= 6) { HOLD_SHORT(6); }
@@ -1388,21 +1037,24 @@ void launch_mma(const hold_gated_desc& d, MmaArgs a, const Plan& p, hipStream_t 
     KeptArgs k = {};
     k.kept = d.kept; k.dh = d.dh; k.lddh = d.lddh;
     k.T = d.T; k.H = d.H; k.Hp = p.Hp;
-    k.dg = a.dg; k.du = a.du; k.dlimb = a.dlimb;
-    k.rscale = a.rscale; k.exps = a.exps; k.dbpart = a.dbpart;
+    k.dg = a.dg; k.du = a.du;
+    k.dbpart = a.dbpart;
     k.cols = (int)cdiv(d.H, 512);
     hipLaunchKernelGGL(gated_kept_kernel<MODE>, dim3((unsigned)(p.row_tiles * k.cols)), dim3(256), 0, st, k);
   } else if (p.keep) {
     a.kept = d.kept;
     const int t = p.big ? 256 : 128;
     a.tm = (int)cdiv(a.T, t); a.tn = (int)cdiv(a.H, t / 2);
-    if (p.big) hipLaunchKernelGGL((gated_mma_kernel<MODE, false, 256, 128, 4, 4, true, 2, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((gated_mma_kernel<MODE, false, 128, 64, 4, 2, false, 2, true>), dim3((unsigned)(a.tm * a.tn)), dim3(512), 0, st, a);
+    if constexpr (MODE == MODE_BF16) {
+      if (p.big) hipLaunchKernelGGL((gated_mma_kernel<MODE, false, 256, 128, 4, 4, true, 2, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
+    }
+    if (!p.big) hipLaunchKernelGGL((gated_mma_kernel<MODE, false, 128, 64, 4, 2, false, 2, true>), dim3((unsigned)(a.tm * a.tn)), dim3(512), 0, st, a);
   } else if (p.brief) {
-    launch_short<MODE, BWD>(d, a, p, st);
+    launch_short<BWD>(d, a, p, st);
   } else if (!BWD && p.big) {
     a.tm = (int)cdiv(a.T, 256); a.tn = (int)cdiv(a.H, 128);
-    hipLaunchKernelGGL((gated_mma_kernel<MODE, false, 256, 128, 4, 4, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
+    if constexpr (MODE == MODE_BF16)
+      hipLaunchKernelGGL((gated_mma_kernel<MODE, false, 256, 128, 4, 4, true>), dim3((unsigned)(a.tm * a.tn)), dim3(1024), 0, st, a);
   } else if (p.little) {
     a.tm = (int)cdiv(a.T, 64); a.tn = (int)cdiv(a.H, 32);
     hipLaunchKernelGGL((gated_mma_kernel<MODE, BWD, 64, 32, 2, 1, false, 4>), dim3((unsigned)(a.tm * a.tn)), dim3(128), 0, st, a);
@@ -1443,7 +1095,7 @@ int fwd(const hold_gated_desc& d, hipStream_t st) {
   const Plan p = plan(d, false);
   if (p.bytes > d.workspace_bytes || (p.bytes && !d.workspace)) return HOLD_E_ARG;
   MmaArgs a = {};
-  if (!p.brief) operands<MODE, false>(d, p, (char*)d.workspace, st, a);
+  if (!p.brief) operands<MODE>(d, p, (char*)d.workspace, st, a);
   a.h = d.h; a.ldh = d.ldh;
   launch_mma<MODE, false>(d, a, p, st);
   return ok();
@@ -1454,32 +1106,26 @@ int bwd(const hold_gated_desc& d, hipStream_t st) {
   const Plan p = plan(d, true);
   if (p.bytes > d.workspace_bytes || !d.workspace) return HOLD_E_ARG;
   char* ws = (char*)d.workspace;
-  constexpr bool F32 = MODE == MODE_F16X3;
-  constexpr int NL = limbs<MODE>();
   MmaArgs a = {};
-  operands<MODE, true>(d, p, ws, st, a);
-  const int64_t XN = d.T * p.Dp, DN = d.T * p.Hp;
-  if (F32)
-    hipLaunchKernelGGL(gated_pack_tokens_kernel, dim3((unsigned)rows_grid(d.T)), dim3(256), 0, st, (const float*)d.x, d.ldx, d.T, d.D, (int)p.Dp,
-                       a.rscale, (const int*)(ws + p.spart), (int)p.pack_blocks, (uint16_t*)(ws + p.xt), XN,
-                       (int*)(ws + p.exps));
+  operands<MODE>(d, p, ws, st, a);
   a.dh = d.dh; a.lddh = d.lddh;
-  a.dg = (uint16_t*)(ws + p.dg); a.du = a.dg + NL * DN; a.dlimb = DN;
+  a.dg = ws + p.dg; a.du = ws + p.dg + d.T * p.Hp * 2 * halves<MODE>();
   a.dbpart = d.db_gate || d.db_up ? (float*)(ws + p.dbpart) : nullptr;
   launch_mma<MODE, true>(d, a, p, st);
   FinishArgs f = {};
   if (d.dx) {
     DxArgs x = {};
-    x.dg = a.dg; x.du = a.du; x.Hp = p.Hp; x.dlimb = DN;
-    x.wg = a.wg; x.wu = a.wu; x.ldwg = a.ldwg; x.ldwu = a.ldwu; x.wlimb = a.wlimb;
+    x.dg = a.dg; x.du = a.du; x.Hp = p.Hp;
+    x.wg = a.wg; x.wu = a.wu; x.ldwg = a.ldwg; x.ldwu = a.ldwu;
     x.T = d.T; x.H = d.H; x.D = d.D;
-    x.rscale = a.rscale; x.exps = a.exps;
     x.dx = d.dx; x.chunk = p.dx_chunk; x.splits = (int)p.dx_splits; x.part = (float*)(ws + p.dx_sums);
     const int t = p.dx_big ? 256 : 128;
     x.tm = (int)cdiv(d.T, t); x.tn = (int)cdiv(d.D, t);
     const unsigned blocks = (unsigned)(x.tm * x.tn * x.splits);
-    if (p.dx_big) hipLaunchKernelGGL((gated_dx_kernel<MODE, 256, 256, 4, 4, true>), dim3(blocks), dim3(1024), 0, st, x);
-    else hipLaunchKernelGGL((gated_dx_kernel<MODE, 128, 128, 2, 4, false>), dim3(blocks), dim3(512), 0, st, x);
+    if constexpr (MODE == MODE_BF16) {
+      if (p.dx_big) hipLaunchKernelGGL((gated_dx_kernel<MODE, 256, 256, 4, 4, true>), dim3(blocks), dim3(1024), 0, st, x);
+    }
+    if (!p.dx_big) hipLaunchKernelGGL((gated_dx_kernel<MODE, 128, 128, 2, 4, false>), dim3(blocks), dim3(512), 0, st, x);
     if (x.splits > 1) {
       f.part[0] = x.part; f.splits[0] = x.splits; f.sets[0] = 1; f.n[0] = d.T * d.D;
       f.out[0][0] = d.dx;
@@ -1488,16 +1134,18 @@ int bwd(const hold_gated_desc& d, hipStream_t st) {
   }
   if (d.dw_gate) {
     DwArgs w = {};
-    w.d[0] = a.dg; w.d[1] = a.du; w.Hp = p.Hp; w.dlimb = DN;
-    w.x = F32 ? (const uint16_t*)(ws + p.xt) : a.x; w.ldx = F32 ? p.Dp : a.ldx; w.xlimb = F32 ? XN : 0;
+    w.d[0] = a.dg; w.d[1] = a.du; w.Hp = p.Hp;
+    w.x = a.x; w.ldx = a.ldx;
     w.T = d.T; w.H = d.H; w.D = d.D;
-    w.chunk = p.dw_chunk; w.splits = (int)p.dw_splits; w.exps = a.exps;
+    w.chunk = p.dw_chunk; w.splits = (int)p.dw_splits;
     w.out[0] = d.dw_gate; w.out[1] = d.dw_up; w.part = (float*)(ws + p.dw_sums);
     const int t = p.dw_big ? 256 : 128;
     w.tm = (int)cdiv(d.H, t); w.tn = (int)cdiv(d.D, t);
     const unsigned blocks = (unsigned)(2 * w.tm * w.tn * w.splits);
-    if (p.dw_big) hipLaunchKernelGGL((gated_dw_kernel<MODE, 256, 256, 4, 4, true>), dim3(blocks), dim3(1024), 0, st, w);
-    else hipLaunchKernelGGL((gated_dw_kernel<MODE, 128, 128, 2, 4, false>), dim3(blocks), dim3(512), 0, st, w);
+    if constexpr (MODE == MODE_BF16) {
+      if (p.dw_big) hipLaunchKernelGGL((gated_dw_kernel<MODE, 256, 256, 4, 4, true>), dim3(blocks), dim3(1024), 0, st, w);
+    }
+    if (!p.dw_big) hipLaunchKernelGGL((gated_dw_kernel<MODE, 128, 128, 2, 4, false>), dim3(blocks), dim3(512), 0, st, w);
     if (w.splits > 1) {
       f.part[1] = w.part; f.splits[1] = w.splits; f.sets[1] = 2; f.n[1] = (int64_t)d.H * d.D;
       f.out[1][0] = d.dw_gate; f.out[1][1] = d.dw_up;
@@ -1529,11 +1177,11 @@ extern "C" int hold_gated_kept(const hold_gated_desc* d, int64_t* bytes) {
 
 extern "C" int hold_gated_fwd(const hold_gated_desc* d, hold_stream_t st) {
   if (check(d) != HOLD_OK || !d->h || d->ldh < d->H) return HOLD_E_ARG;
-  return d->dtype == HOLD_GATED_F32 ? fwd<MODE_F16X3>(*d, (hipStream_t)st) : fwd<MODE_BF16>(*d, (hipStream_t)st);
+  return d->dtype == HOLD_GATED_F32 ? fwd<MODE_F32>(*d, (hipStream_t)st) : fwd<MODE_BF16>(*d, (hipStream_t)st);
 }
 
 extern "C" int hold_gated_bwd(const hold_gated_desc* d, hold_stream_t st) {
   if (check(d) != HOLD_OK || !d->dh || d->lddh < d->H || (!d->dw_gate != !d->dw_up)) return HOLD_E_ARG;
   if (((uintptr_t)d->dx | (uintptr_t)d->dw_gate | (uintptr_t)d->dw_up) % 16) return HOLD_E_ARG;
-  return d->dtype == HOLD_GATED_F32 ? bwd<MODE_F16X3>(*d, (hipStream_t)st) : bwd<MODE_BF16>(*d, (hipStream_t)st);
+  return d->dtype == HOLD_GATED_F32 ? bwd<MODE_F32>(*d, (hipStream_t)st) : bwd<MODE_BF16>(*d, (hipStream_t)st);
 }

@@ -4,13 +4,15 @@ It stands beside the framework's other single-layer products (hold_amd.gemm: lin
 is a second projection's gate.  ``gated_linear`` takes weights in ``nn.Linear``'s layout [H, D]; the four activations of the gate are
 ``silu``, ``gelu`` (the exact one, by erf), ``relu`` and ``sigmoid``.
 
-Arithmetic: float32 tensors through two-limb fp16 products with float32 accumulation (errors of float32's own size), bfloat16 tensors
-through bf16 products with float32 accumulation, rounded once at the end; in the backward pass of bfloat16, dL/dg and dL/du are rounded
-to bfloat16 once as operands of the next products.  Results do not depend on the other rows of a batch, except that up to 4 and up to
-64 rows other kernels (of the same accuracy) compute them.  All sums have a fixed order.
+Arithmetic: float32 tensors through float32 products and sums on the matrix cores, whatever the values' range; bfloat16 tensors through
+bf16 products with float32 accumulation, rounded once at the end; in the backward pass of bfloat16, dL/dg and dL/du are rounded to
+bfloat16 once as operands of the next products.  Infinities and NaN come out where the formula has them.  Results do not depend on the
+other rows of a batch, except that up to 4 and up to 64 rows other kernels (of the same accuracy) compute them.  All sums have a fixed
+order.
 
 For a backward pass a call keeps its inputs, and u act'(g) and act(g) where reading them is less time than computing them again
-(more than 256 features in float32, 512 in bfloat16, and at least 2^21 results): 8 bytes a result in float32, 6 in bfloat16.
+(float32: more than 256 features and 2^21 results, or more than 128 and 2^23; bfloat16: more than 512 and 2^21): 8 bytes a result in
+float32, 6 in bfloat16.
 """
 from __future__ import annotations
 
@@ -26,7 +28,7 @@ from ._lib import GatedDesc, check, stream_ptr
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 MAX_WIDTH = 1 << 21
-_SHORT = 256  # up to so many features nothing is kept for the backward pass
+_SHORT = 128  # up to so many features nothing is kept for the backward pass
 
 
 def _rows(t, most=MAX_WIDTH):
