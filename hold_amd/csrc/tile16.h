@@ -346,8 +346,9 @@ struct Core {
     for (int kt = 0; kt < nk; ++kt) {
       const char* s = smem + at * STAGE;
       if (!all || kt == 0) {
-        if (S == 2 || all || kt + S - 1 > nk) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
+        // (the wave's own reads of the stage that is filled next are done too)
+        if (S == 2 || all || kt + S - 1 > nk) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(AHEAD) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
@@ -374,6 +375,7 @@ struct Core {
         }
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   }
