@@ -25,7 +25,7 @@ using namespace t16;
 
 namespace {
 
-constexpr int MAXI = 36;  // items of one launch (kernel arguments stay below 4 KB)
+constexpr int MAXI = 36;  // items of one launch; its arguments then take up to 4.7 KB (the last APPLY of several shapes)
 
 struct Item {
   const void* g;  // the matrix (orthogonalise), the gradient (step)
@@ -280,6 +280,7 @@ struct NsArgs {
   int shift;          // exponent from the accumulated sum to the stored limbs
 };
 
+static_assert(sizeof(Classes) + sizeof(NsArgs) + sizeof(Step) + sizeof(Items) <= 5120, "a launch's arguments stay small");
 struct NoItems {};
 template <bool LAST> struct ItemArg { typedef NoItems type; };
 template <> struct ItemArg<true> { typedef Items type; };
