@@ -11,8 +11,8 @@ OUT = os.path.join(_HERE, "libholdhip_dev.so" if os.environ.get("HOLD_DEV") == "
 # -pragma-unroll-threshold: the register-resident kernels (rmlp.hip / rchain.hip) write one k step as 48 MFMA gaps with
 # constant-index slices of work behind each; LLVM refuses to fully unroll `#pragma unroll` nests beyond 16 384 instructions
 # (pre-simplification) and the accumulator arrays would then be indexed dynamically -- i.e. live in scratch memory
-# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, some forms of which have given wrong results on this machine now and then (hipcc's
-# host pass warns that it does not know the feature: harmless)
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, a precaution that no test here speaks for or against and that costs nothing (the bench
+# line with them 91.8 k rays/s, without 93.9 k); hipcc's host pass warns that it does not know the feature: harmless
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-mllvm", "-pragma-unroll-threshold=1048576",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # developer build (HOLD_DEV=1 in the environment of the BUILD): adds the diagnostics kernels (csrc/dev/diag.hip) and

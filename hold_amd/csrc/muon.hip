@@ -728,7 +728,7 @@ void launch_tiles(const Classes& cl, const NsArgs& s, const Step& st, const Item
 // on single matrices of 1500 .. 4096 and batches of 256 .. 1024 rows, each with every tile size: 4096^3 takes 255 us in 256 x 256
 // tiles, 2 x 154 in 128, 5.3 x 119 in 64; 36 matrices of 256 x 256 in 64 8 us a product, 14 in 128.  Where
 // a launch of 64 is latency more than work it takes shorter ways: up to two blocks a unit (APPLY: one) in tiles of 32 x 32 (32 x 64) with
-// four stages of 64, sums up to 256 requested at once (a 256 x 256 matrix 120 -> 82 us, 3 x 1531 x 517 250 -> 206 in 16 bits; with more
+// four stages of 64, sums up to 256 requested at once (a 256 x 256 matrix 110 -> 80 us, 3 x 1531 x 517 in 16 bits 273 -> 232; with more
 // blocks the loads count: 1024 x 1024 280 -> 295); else up to two blocks a unit with eight waves in steps of 64 (1024 x 1024 280 -> 245,
 // 16 x 256 x 256 123 -> 110; above, three blocks of four waves: 48 x 256 x 256 205 against 210).  Tiles of 128 in phases where both
 // operands are read by rows: GRAM of 6 x 1024 x 4096 124 -> 113 us; APPLY's 175 stay 174.

@@ -157,7 +157,7 @@ __device__ __forceinline__ void dma_pair(const char* src, uint32_t lane16, uint3
 // empty asm right behind a builtin v_exp / v_log made the hazard recogniser pad a wait state -- 9 s_nop per k step); their
 // consumers are LAT_TRANS instruction slots away by construction of the schedule (tests/test_r6_pack_cpu.py checks the table)
 // arithmetic on value PAIRS, two volatile scalar instructions each: the packed fp32 instructions (v_pk_*_f32) would halve the
-// issue slots, but some of their forms have given wrong results on this machine now and then, so the library is built without them
+// issue slots, but the library is built without them (hold_amd/build.py)
 __device__ __forceinline__ float mul_v(float a, float b) { float r; asm volatile("v_mul_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
 __device__ __forceinline__ float add_v(float a, float b) { float r; asm volatile("v_add_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
 __device__ __forceinline__ float fma_v(float a, float b, float c) { float r; asm volatile("v_fma_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c)); return r; }
