@@ -196,7 +196,7 @@ template <int MODE>
 __device__ __forceinline__ const uint16_t* element(const void* p, int64_t i) { return (const uint16_t*)p + i * halves<MODE>(); }
 
 // ---- both projections and what follows them (fp32, 131072 x 256 -> 256: 277 us, 124 TFLOP/s, the matrix cores 78 % busy, no bank conflict;
-// the rest is tiles of eight steps starting and ending, two blocks a unit) -----------------------------------------------------------------------------------------
+// the rest is tiles of eight steps starting and ending, two blocks a unit) ----
 struct MmaArgs {
   const void* x; int64_t ldx;                    // operands as the tile loads take them: [T][K]
   const void* wg; const void* wu; int64_t ldwg, ldwu;
@@ -607,7 +607,7 @@ __global__ __launch_bounds__(64 * SHORT_WAVES) void gated_short_kernel(ShortArgs
   }
 }
 
-// ---- dx = dg Wg + du Wu (fp32, 65536 x 256 <- 512: 264 us, 130 TFLOP/s, the matrix cores 82 % busy) ---------------------------------------------------------------------------------------------------------------
+// ---- dx = dg Wg + du Wu (fp32, 65536 x 256 <- 512: 264 us, 130 TFLOP/s, the matrix cores 82 % busy) ----
 struct DxArgs {
   const void* dg; const void* du; int64_t Hp;
   const void* wg; const void* wu; int64_t ldwg, ldwu;
@@ -654,7 +654,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gated_dx_kernel(DxArgs a) {
   }
 }
 
-// ---- dWg = dg^T x, dWu = du^T x (fp32, the same layer: 256 us, 134 TFLOP/s, 85 % busy) ---------------------------------------------------------------------------------------------------------
+// ---- dWg = dg^T x, dWu = du^T x (fp32, the same layer: 256 us, 134 TFLOP/s, 85 % busy) ----
 struct DwArgs {
   const void* d[2]; int64_t Hp;
   const void* x; int64_t ldx;
